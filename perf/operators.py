@@ -212,7 +212,7 @@ def prepare(case, seed):
     pos = (ends[:, None] - T + np.arange(T)[None, :]).reshape(-1)
     st = {"case": case, "cache": cache, "table": table, "ends": i32(ends), "pos0": i32(ends - T), "positions": i32(pos),
           "tok_seg": i32(np.repeat(np.arange(B), T)), "seg_start": i32(np.arange(B) * T), "seg_len": i32(np.full(B, T)),
-          "len_host": np.full(B, T, dtype=np.int32), "pos0_host": (ends - T).astype(np.int32), "longest": int(ends.max())}
+          "len_host": np.full(B, T, dtype=np.int32), "pos0_host": (ends - T).astype(np.int32)}
     if case["op"] == "store":
         k, v = rows(n)
         # rows of the fused projection: queries, keys, values side by side
@@ -318,9 +318,9 @@ def run(st):
     K, D, P = case["kv_heads"], case["head_dim"], case["page_size"]
     if case["op"] == "attention":
         out = torch.empty_like(st["q"])
-        kernels.attention_kv4(st["q"], out, st["cache"], 0, P, st["positions"], st["tok_seg"], st["seg_start"], st["seg_len"], st["pos0"],
-                              st["table"], case["heads"], D, st["scale"], (st["len_host"], st["pos0_host"]), window=case["window"],
-                              sink=st["sink"], softcap=case["softcap"], keep_first=case["keep_first"], bias=st["bias"])
+        kernels.attention_kv4(st["q"], out, st["cache"], 0, P, st["seg_start"], st["seg_len"], st["pos0"], st["table"], case["heads"], D, st["scale"],
+                              (st["len_host"], st["pos0_host"]), window=case["window"], sink=st["sink"], softcap=case["softcap"],
+                              keep_first=case["keep_first"], bias=st["bias"])
         return out
     if case["op"] == "store":
         kernels.kv4_store(st["k"], st["v"], st["positions"], st["tok_seg"], st["table"], st["cache"], 0, P)
