@@ -1,0 +1,96 @@
+"""The cache in four bits: its numbers and its refusals, without a GPU."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import plain_kv4
+from xyntetik_runner_b200 import kernels
+
+
+def test_values_are_bfloat16_numbers():
+    """c s has at most eight significant bits for every code and every scale: three (or a power of two) times five."""
+    for m in range(16, 32):
+        for c in range(-8, 8):
+            x = c * -(m / 32.0) / 8.0
+            assert float(torch.tensor(x, dtype=torch.float64).to(torch.bfloat16)) == x
+        assert float(torch.tensor(24.0 * m, dtype=torch.float64).to(torch.bfloat16)) == 24.0 * m
+
+
+def test_a_group_is_near_what_it_holds():
+    """Half a step everywhere but at the smaller side's end, where seven steps reach: a step is the largest magnitude / 8, give or take 1 / 32."""
+    g = np.random.default_rng(3)
+    for _ in range(300):
+        x = g.standard_normal(32) * math.exp(g.uniform(-20, 20))
+        codes, s = plain_kv4.group(x)
+        off = np.abs(codes * s - x)
+        inside = x / s <= 7.5
+        assert np.all(off[inside] <= abs(s) * 0.5 * (1 + 1e-12)) and np.all(off <= abs(s) * 1.26)
+        assert abs(abs(s) * 8 / np.max(np.abs(x)) - 1) <= 1 / 32
+
+
+def test_sizes():
+    assert [kernels.kv4_held(d) for d in (1, 16, 64, 65, 128, 129, 256)] == [64, 64, 64, 128, 128, 256, 256]
+    assert kernels.kv4_block_bytes(128, 64) == 64 * 144 and kernels.kv4_block_bytes(40, 8) == 8 * 72
+    for hd in (0, 257, -1):
+        with pytest.raises(kernels.KernelError, match="heads of 1 to 256"):
+            kernels.kv4_held(hd)
+    for page in (0, 4, 12, 20, -8, 1 << 17):
+        with pytest.raises(kernels.KernelError, match="multiple of 8"):
+            kernels.kv4_block_bytes(64, page)
+    c = kernels.kv4_cache(3, 2, 4, 100, 16, "cpu")
+    assert c.shape == (3, 2, 4, 16 * 144) and c.dtype == torch.uint8 and not c.any()
+
+
+def _parts(K=2, D=64, P=16, n=4, S=2):
+    i = torch.zeros(n, dtype=torch.int32)
+    return dict(k=torch.zeros(n, K * D), v=torch.zeros(n, K * D), positions=i, tok_seg=i, block_tables=torch.zeros(S, 3, dtype=torch.int32),
+                cache=kernels.kv4_cache(3, 1, K, D, P, "cpu"), layer=0, page_size=P)
+
+
+@pytest.mark.parametrize("change, message", [
+    (dict(k=torch.zeros(4, 127)), "kv heads"), (dict(v=torch.zeros(3, 128)), "kv heads"), (dict(v=torch.zeros(4, 128, dtype=torch.bfloat16)), "one type"),
+    (dict(k=torch.zeros(128, 4).t()), "side by side"), (dict(positions=torch.zeros(4, dtype=torch.int64)), "int32"),
+    (dict(tok_seg=torch.zeros(3, dtype=torch.int32)), "int32"), (dict(block_tables=torch.zeros(6, dtype=torch.int32)), "block tables"),
+    (dict(cache=torch.zeros(3, 1, 2, 8)), "current CUDA device|uint8"), ({}, "current CUDA device")])
+def test_store_refuses(change, message):
+    with pytest.raises(kernels.KernelError, match=message):
+        kernels.kv4_store(**{**_parts(), **change})
+
+
+@pytest.mark.parametrize("change, message", [
+    (dict(out=torch.zeros(2, 2, 2, 8, 64)), "out is"), (dict(out=torch.zeros(2, 2, 3, 16, 64)), "out is"), (dict(keep_first=-1), "keep_first"),
+    (dict(first=torch.zeros(1, dtype=torch.int32)), "first"), (dict(tables=torch.zeros(2, 2, dtype=torch.int32)), "tables"), ({}, "current CUDA device")])
+def test_read_refuses(change, message):
+    p = _parts()
+    i = torch.zeros(2, dtype=torch.int32)
+    args = dict(cache=p["cache"], layer=0, page_size=16, block_tables=p["block_tables"], first=i, end=i, out=torch.zeros(2, 2, 2, 16, 64))
+    with pytest.raises(kernels.KernelError, match=message):
+        kernels.kv4_read(**{**args, **change})
+
+
+@pytest.mark.parametrize("change, message", [
+    (dict(heads=3), "query heads"), (dict(out=torch.zeros(4, 255)), "rows of the same tokens"), (dict(q=torch.zeros(4, 255)), "rows of the same tokens"),
+    (dict(q=torch.zeros(4, 256, dtype=torch.bfloat16)), "rows of the same tokens"), (dict(scale=0.0), "scale"), (dict(scale=math.nan), "scale"),
+    (dict(window=-1), "window"), (dict(softcap=-1.0), "window"), (dict(softcap=1.0, bias=torch.zeros(4, 3)), "without a cap|CUDA"),
+    (dict(sink=torch.zeros(3)), "sink"), (dict(lengths=(np.array([2, 2]), np.array([0, 0]))), "int32"),
+    (dict(lengths=(np.array([3, 2], dtype=np.int32), np.array([0, 0], dtype=np.int32))), "does not hold|do not hold|does not|not hold"),
+    (dict(lengths=(np.array([2, 2], dtype=np.int32), np.array([0, -1], dtype=np.int32))), "below zero"),
+    (dict(lengths=(np.array([2], dtype=np.int32), np.array([0], dtype=np.int32))), "one value a portion"),
+    (dict(seg_pos0=torch.zeros(2)), "seg_pos0"), ({}, "current CUDA device")])
+def test_attention_refuses(change, message):
+    p, i = _parts(), torch.zeros(2, dtype=torch.int32)
+    two = np.array([2, 2], dtype=np.int32)
+    args = dict(q=torch.zeros(4, 256), out=torch.zeros(4, 256), cache=p["cache"], layer=0, page_size=16, seg_start=i, seg_len=i, seg_pos0=i,
+                block_tables=p["block_tables"], heads=4, head_dim=64, scale=0.1, lengths=(two, two))
+    with pytest.raises(kernels.KernelError, match=message):
+        kernels.attention_kv4(**{**args, **change})
+
+
+def test_pages_that_are_read():
+    a = lambda *x: np.array(x, dtype=np.int32)
+    assert kernels.kv4_pages_read(a(1, 20), a(0, 15), 16, 0, 0) == 1 + 3
+    assert kernels.kv4_pages_read(a(0, 20), a(7, 15), 16, 0, 0) == 3
+    assert kernels.kv4_pages_read(a(1), a(100), 16, 10, 20) == 2 + 2           # rows 91 .. 100 lie in pages 5 and 6, the kept in 0 and 1
+    assert kernels.kv4_pages_read(a(1), a(40), 16, 20, 33) == 1 + 2            # kept rows that the window's pages hold are not there twice

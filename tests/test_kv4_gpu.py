@@ -1,0 +1,228 @@
+"""The cache in four bits on the device: store, read and attention against the plain form in 64 bits (plain_kv4.py)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import plain_kv4
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def i32(a):
+    return torch.tensor(np.asarray(a), dtype=torch.int32, device=DEV)
+
+
+def tables(lens, P, g, spare=2):
+    """Block tables of requests with these lengths, pages in a random order, and how many pages there are."""
+    need = [-(-n // P) for n in lens]
+    order = torch.randperm(sum(need) + spare, generator=g).tolist()
+    bt = np.full((len(lens), max(max(need), 1) + 1), -1, dtype=np.int32)
+    for r, n in enumerate(need):
+        bt[r, :n] = [order.pop() for _ in range(n)]
+    return bt, sum(need) + spare
+
+
+def same(a, b):
+    a, b = a.double().cpu(), b.double().cpu()
+    return torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(torch.nan_to_num(a), torch.nan_to_num(b))
+
+
+STORE = [  # lens held ahead, tokens, K, D, Vd, page, dtype, extra columns of a row
+    ([0], 1, 1, 64, 64, 8, BF16, 0), ([5, 0, 63], 9, 2, 128, 128, 16, BF16, 64), ([7], 40, 3, 100, 100, 24, F32, 3), ([30, 1], 5, 1, 16, 16, 64, BF16, 1),
+    ([0, 17], 33, 2, 256, 256, 8, F32, 0), ([2], 7, 2, 80, 48, 32, BF16, 8), ([2], 7, 2, 33, 65, 32, F32, 0), ([11], 3, 40, 192, 192, 40, BF16, 0),
+    ([0], 20, 1, 1, 1, 16, F32, 5)]
+
+
+@pytest.mark.parametrize("held,T,K,D,Vd,P,dtype,extra", STORE)
+def test_store_and_read(held, T, K, D, Vd, P, dtype, extra):
+    """Bytes as the plain form writes them, nothing else touched; values read back are what the bytes stand for, exactly."""
+    from xyntetik_runner_b200 import kernels
+    g = torch.Generator().manual_seed(D * 100 + P + T)
+    lens = [h + T for h in held]
+    bt, n_pages = tables(lens, P, g)
+    hs, B = plain_kv4.held(max(D, Vd)), len(held)
+    cache = torch.randint(0, 256, (n_pages, 2, K, kernels.kv4_block_bytes(max(D, Vd), P)), generator=g, dtype=torch.uint8)
+    n = B * T
+    row = torch.randn(n, K * (D + Vd) + extra, generator=g) * torch.exp(torch.randn(n, 1, generator=g) * 3)
+    row[0, :min(D, 32)] = 0.0                                        # a group of zeros
+    row[-1, K * D:K * D + min(Vd, 32)] *= 1e-35                      # below what is held
+    row = row.to(dtype)
+    pos = np.concatenate([h + np.arange(T) for h in held])
+    seg = np.repeat(np.arange(B), T)
+    want = cache.numpy().copy()
+    values = []
+    for plane, (at, E) in enumerate(((0, D), (K * D, Vd))):
+        full = torch.zeros(n * K, max(D, Vd), dtype=torch.float64)
+        full[:, :E] = row[:, at:at + K * E].double().reshape(n * K, E)
+        codes, scales, v = plain_kv4.quantised(full)
+        values.append(v.reshape(n, K, -1))
+        for t in range(n):
+            for h in range(K):
+                plain_kv4.put(want[bt[seg[t], pos[t] // P], 1, h], P, pos[t] % P, plane, codes[t * K + h], scales[t * K + h])
+    dev, rows = cache.to(DEV), row.to(DEV)
+    kernels.kv4_store(rows[:, :K * D], rows[:, K * D:K * (D + Vd)], i32(pos), i32(seg), i32(bt), dev, 1, P)
+    assert torch.equal(dev.cpu(), torch.from_numpy(want))
+    for out_dtype in (BF16, F32):
+        first, end = i32(held), i32(lens)
+        pages = sum((e - 1) // P - f // P + 1 for f, e in zip(held, lens))
+        out = torch.full((pages + 1, 2, K, P, max(D, Vd)), 7.0, dtype=out_dtype, device=DEV)
+        where = i32(np.full_like(bt, -9))
+        kernels.kv4_read(dev, 1, P, i32(bt), first, end, out, tables=where)
+        exp = torch.zeros(pages + 1, 2, K, P, max(D, Vd), dtype=torch.float64)
+        exp[-1] = 7.0                                                # a page behind the last is left as it was
+        j = 0
+        exp_where = np.full_like(bt, -9)
+        for r in range(B):
+            for pi in range(held[r] // P, (lens[r] - 1) // P + 1):
+                for p in range(max(pi * P, held[r]), min((pi + 1) * P, lens[r])):
+                    for plane in (0, 1):
+                        exp[j, plane, :, p - pi * P] = values[plane][r * T + p - held[r]]
+                exp_where[r, pi] = j
+                j += 1
+        assert torch.equal(out.double().cpu(), exp) and torch.equal(where.cpu(), torch.from_numpy(exp_where))
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, 2.0 ** 120, -2.0 ** 121, 2.0 ** 119, -2.0 ** -96, 2.0 ** -97, 0.0])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_borders_of_what_is_held(bad, dtype):
+    """One element of a group out of the common: the group as the plain form has it, its neighbours as ever."""
+    from xyntetik_runner_b200 import kernels
+    g = torch.Generator().manual_seed(5)
+    k = torch.randn(2, 128, generator=g)
+    k[0, 32:64] *= 2.0 ** -100 if abs(bad) < 1e-20 else 1.0
+    k[0, 40] = bad
+    k, v = k.to(dtype), torch.randn(2, 128, generator=g).to(dtype)
+    cache = kernels.kv4_cache(1, 1, 1, 128, 8, DEV)
+    bt = i32([[0]])
+    kernels.kv4_store(k.to(DEV), v.to(DEV), i32([0, 1]), i32([0, 0]), bt, cache, 0, 8)
+    out = torch.empty(1, 2, 1, 8, 128, dtype=F32, device=DEV)
+    kernels.kv4_read(cache, 0, 8, bt, i32([0]), i32([2]), out)
+    assert same(out[0, 0, 0, :2], plain_kv4.quantised(k)[2]) and same(out[0, 1, 0, :2], plain_kv4.quantised(v)[2])
+
+
+def test_halves_between_two_codes_go_to_even():
+    """x / s of exactly n + 1/2, for every scale of five bits."""
+    from xyntetik_runner_b200 import kernels
+    rows = []
+    for m in range(16, 32):
+        s = m / 16.0
+        half = [(c + 0.5) * s for c in range(-8, 7)] + [c * s for c in range(-7, 8)]
+        rows.append([8.0 * s] + half + [0.0])
+    k = torch.tensor(rows, dtype=torch.float32)
+    k = torch.cat([k, -k], dim=0)
+    n = k.shape[0]
+    for dtype in (F32, BF16):
+        x = k.to(dtype)
+        cache = kernels.kv4_cache(4, 1, 1, 32, 8, DEV)
+        bt = i32([[2, 0, 3, 1]])
+        kernels.kv4_store(x.to(DEV), x.to(DEV), i32(np.arange(n)), i32(np.zeros(n)), bt, cache, 0, 8)
+        out = torch.empty(4, 2, 1, 8, 32, dtype=F32, device=DEV)
+        kernels.kv4_read(cache, 0, 8, bt, i32([0]), i32([n]), out)
+        want = plain_kv4.quantised(x)[2]
+        for plane in (0, 1):
+            assert torch.equal(out[:, plane, 0].reshape(n, 32).double().cpu(), want)
+
+
+def test_pages_that_are_not_held():
+    """Tokens whose page is not held, or is not one of the cache's, are not written; rows on such pages are read as zeros; other requests are as ever."""
+    from xyntetik_runner_b200 import kernels
+    g = torch.Generator().manual_seed(6)
+    P, K, D = 8, 2, 64
+    bt = np.array([[3, -1, 1, 9], [0, 2, -5, 1 << 30]], dtype=np.int32)          # a cache of five pages
+    pos, seg = np.array([3, 9, 17, 25, 40, -1, 1, 12, 18, 26, 5]), np.array([0, 0, 0, 0, 0, 0, 1, 1, 1, 1, 2])
+    n = len(pos)
+    k = torch.randn(n, K * D, generator=g).to(BF16)
+    cache = kernels.kv4_cache(5, 1, K, D, P, DEV)
+    kernels.kv4_store(k.to(DEV), k.to(DEV), i32(pos), i32(seg), i32(bt), cache, 0, P)
+    want = np.zeros((5, 1, K, cache.shape[3]), dtype=np.uint8)
+    codes, scales, values = plain_kv4.quantised(k.reshape(n * K, D))
+    kept = [0, 2, 6, 7]
+    for t in kept:
+        for plane in (0, 1):
+            for h in range(K):
+                plain_kv4.put(want[bt[seg[t], pos[t] // P], 0, h], P, pos[t] % P, plane, codes[t * K + h], scales[t * K + h])
+    assert torch.equal(cache.cpu(), torch.from_numpy(want))
+    out = torch.full((8, 2, K, P, D), 5.0, dtype=BF16, device=DEV)
+    kernels.kv4_read(cache, 0, P, i32(bt), i32([0, 0]), i32([100, 32]), out)
+    exp = torch.zeros(8, 2, K, P, D, dtype=torch.float64)
+    for t in kept:
+        exp[4 * seg[t] + pos[t] // P, :, :, pos[t] % P] = values.reshape(n, K, D)[t]
+    got = out.double().cpu()
+    for t in kept:
+        assert torch.equal(got[4 * seg[t] + pos[t] // P, :, :, pos[t] % P], exp[4 * seg[t] + pos[t] // P, :, :, pos[t] % P])
+    for page in (1, 3, 6, 7):
+        assert not got[page].any()
+
+
+ATT = [  # contexts, tokens, H, K, D, page, dtype, window, keep, sink, cap, bias
+    ([1], 1, 1, 1, 64, 8, BF16, 0, 0, 0, 0, 0), ([1, 2, 33], 1, 4, 2, 128, 64, BF16, 0, 0, 0, 0, 0), ([64, 65, 129, 300], 1, 8, 2, 64, 64, BF16, 0, 0, 0, 0, 0),
+    ([700], 1, 8, 1, 128, 16, BF16, 0, 0, 1, 0, 0), ([333, 40], 1, 4, 4, 256, 24, BF16, 0, 0, 0, 0, 0), ([100, 31], 1, 5, 1, 100, 40, BF16, 0, 0, 0, 0, 0),
+    ([90], 3, 6, 2, 80, 32, BF16, 0, 0, 0, 0, 0), ([200, 17], 4, 16, 4, 128, 64, BF16, 0, 0, 1, 0, 0), ([150, 6], 6, 14, 2, 64, 8, BF16, 0, 0, 0, 20.0, 0),
+    ([500, 260], 1, 8, 2, 128, 64, BF16, 100, 0, 0, 0, 0), ([500, 60], 1, 8, 2, 128, 16, BF16, 33, 5, 1, 0, 40), ([400], 5, 4, 1, 64, 16, BF16, 64, 70, 0, 0, 200),
+    ([300], 1, 71, 1, 64, 64, BF16, 0, 0, 0, 0, 0), ([120], 2, 20, 1, 192, 64, BF16, 50, 3, 1, 0, 0), ([77], 1, 3, 3, 16, 8, BF16, 0, 0, 0, 0, 0),
+    ([1, 90], 1, 4, 2, 64, 64, F32, 0, 0, 0, 0, 0), ([333], 1, 8, 2, 128, 64, F32, 0, 0, 1, 30.0, 0), ([130, 20], 7, 6, 3, 100, 24, F32, 40, 9, 0, 0, 30),
+    ([60], 60, 4, 2, 128, 16, F32, 0, 0, 0, 0, 0), ([80], 3, 2, 1, 256, 64, F32, 0, 0, 0, 0, 0),
+    # portions that are read back for the prompt kernels, beside short ones
+    ([90], 70, 8, 2, 128, 64, BF16, 0, 0, 0, 0, 0), ([150], 33, 4, 2, 64, 16, BF16, 40, 5, 1, 0, 0), ([100], 80, 3, 1, 48, 24, BF16, 30, 10, 0, 0, 0),
+    ([70], 40, 3, 1, 100, 24, BF16, 0, 0, 0, 0, 0), ([120], 100, 2, 2, 256, 64, BF16, 0, 0, 0, 0, 0)]
+
+
+def attention_case(contexts, T, H, K, D, P, dtype, window, keep, sink, cap, bias, seed=1, layers=2, layer=1):
+    """(arguments of attention_kv4 but for q and out, q on the CPU, the held values of every request, plain options)"""
+    from xyntetik_runner_b200 import kernels
+    g = torch.Generator().manual_seed(seed * 1000 + D + P + sum(contexts))
+    Ts = [T] * len(contexts) if isinstance(T, int) else T
+    bt, n_pages = tables(contexts, P, g)
+    cache = torch.randint(0, 256, (n_pages, layers, K, kernels.kv4_block_bytes(D, P)), generator=g, dtype=torch.uint8).to(DEV)   # garbage, NaN scales among it
+    kv = [(torch.randn(c, K * D, generator=g) * 1.5).to(dtype) for c in contexts for _ in (0, 1)]
+    pos = np.concatenate([np.arange(c) for c in contexts])
+    seg = np.repeat(np.arange(len(contexts)), contexts)
+    kernels.kv4_store(torch.cat(kv[0::2]).to(DEV), torch.cat(kv[1::2]).to(DEV), i32(pos), i32(seg), i32(bt), cache, layer, P)
+    held = [plain_kv4.quantised(x.reshape(-1, D))[2].reshape(-1, K, D) for x in kv]
+    n = sum(Ts)
+    q = (torch.randn(n, H * D, generator=g) * 1.3).to(dtype)
+    sinks = torch.randn(H, generator=g) if sink else None
+    table = -torch.rand(H, bias, generator=g) * 30 if bias else None
+    starts = np.concatenate([[0], np.cumsum(Ts)[:-1]])
+    pos0 = np.array(contexts) - np.array(Ts)
+    if window:
+        # pages that no token of the portion sees any more are given back
+        for r, p0 in enumerate(pos0):
+            for pi in range(bt.shape[1]):
+                last = (pi + 1) * P - 1
+                if last < p0 - window + 1 and pi * P >= keep:
+                    bt[r, pi] = -1
+    args = dict(cache=cache, layer=layer, page_size=P, seg_start=i32(starts), seg_len=i32(Ts), seg_pos0=i32(pos0), block_tables=i32(bt), heads=H, head_dim=D,
+                scale=D ** -0.5, lengths=(np.array(Ts, dtype=np.int32), pos0.astype(np.int32)), window=window, sink=None if sinks is None else sinks.to(DEV),
+                softcap=cap, keep_first=keep, bias=None if table is None else table.to(DEV))
+    plain = dict(scale=D ** -0.5, window=window, keep=keep, sink=None if sinks is None else sinks.double(), softcap=cap, bias=None if table is None else table.double())
+    return args, q, held, plain, Ts, starts, pos0
+
+
+def check(got, q, held, plain, Ts, starts, pos0, H, D, dtype):
+    for r, T in enumerate(Ts):
+        s = starts[r]
+        if T == 0:
+            continue
+        o, size, raw = plain_kv4.attention(q[s:s + T].double().reshape(T, H, D), held[2 * r], held[2 * r + 1], int(pos0[r]), **plain)
+        tol = plain_kv4.tolerance(o, size, raw, D, dtype)
+        off = (got[s:s + T].double().cpu().reshape(T, H, D) - o).abs()
+        assert torch.all(off <= tol), f"request {r}: {float((off / tol).max()):.3g} of the tolerance"
+
+
+@pytest.mark.parametrize("contexts,T,H,K,D,P,dtype,window,keep,sink,cap,bias", ATT)
+def test_attention(contexts, T, H, K, D, P, dtype, window, keep, sink, cap, bias):
+    from xyntetik_runner_b200 import kernels
+    args, q, held, plain, Ts, starts, pos0 = attention_case(contexts, T, H, K, D, P, dtype, window, keep, sink, cap, bias)
+    wide = torch.zeros(q.shape[0], H * D + 24, dtype=dtype, device=DEV)          # q's rows lie in wider ones
+    wide[:, :H * D] = q.to(DEV)
+    for rows in (q.to(DEV), wide):
+        out = torch.full((q.shape[0] + 3, H * D), 9.0, dtype=dtype, device=DEV)
+        kernels.attention_kv4(rows, out[:q.shape[0]], **args)
+        kernels.tc_check_status(torch.device(DEV))
+        check(out, q, held, plain, Ts, starts, pos0, H, D, dtype)
+        assert torch.all(out[q.shape[0]:] == 9.0)

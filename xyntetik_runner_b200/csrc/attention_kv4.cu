@@ -1,0 +1,710 @@
+// Causal grouped-query attention over a paged cache in four bits (kv4.cuh), for decoded tokens and short portions, bfloat16 or float32
+// queries, head sizes up to 256.
+//
+// For the query at position p, head h, kv head h / (H/K):  s_t = (q . k_t) * scale over the keys it sees (attention_mask.cuh: causal, a
+// window, kept first keys), with a cap c tanh(s / c) or a bias by distance as options, a = softmax(s) (a sink joins its denominator),
+// o = sum_t a_t v_t; k_t and v_t are the held values, c s with c of four bits and s a bfloat16.  (src/model.c:3548-3589, 3409-3415;
+// the reference attends over its eight-bit cache in k_attn_dec, src/kernels.cu:2171-2270.)
+//
+// The keys are the M side of the matrix instruction (m16n8k16), the packed query rows (row i: token i / G, head i % G) the N side: eight
+// rows cost one instruction where rows on M would cost a half empty one.  S^T = K Q^T has a key's scores for two rows in a thread;
+// O^T = V^T P^T has two neighbouring elements of the value for the same two rows, so that the running maximum's factor is one number a
+// column in both.  P^T as the second product's operand is S^T turned by movmatrix.
+//
+// A fragment never leaves the thread that loads it: a thread's word of eight codes gives, pair by pair (a shift, a mask, and one fused
+// product and sum that takes off the bias and multiplies by the group's scale, exactly), the eight neighbouring elements of a key
+// that two k-steps want from it; and the words of two keys, their halves brought together by two byte permutations, give the pairs over KEYS
+// that the second product wants, for eight elements of the value.  The order of elements along k and of keys along k is free as long as both
+// operands share it: element order is the words', key order is `at_key` below, chosen so that neither load meets a bank twice too often.
+//
+// A warp walks tiles of its own (32 keys, 64 at head size 64) through a ring of bulk copies: four contiguous pieces a tile and page.
+// The warps of a block interleave the tiles of a span and meet once, at its end.  Spans of a request are combined by k_kv4_merge, in
+// ascending order.
+//
+// float32: a float32 number is the exact sum of three bfloat16 numbers, the held values are bfloat16 numbers, so that three products on
+// the tensor cores (q in pieces, p in pieces) give float32's precision.
+#include "kv4.cuh"
+#include "attention_mask.cuh"
+#include <math.h>
+
+#define A4_WARPS 4
+#define A4_THREADS (32 * A4_WARPS)
+#define A4_STAGES 3
+#define A4_PAGES 448                  // block-table entries of a span that are kept in shared memory
+#define A4_SPIN_LIMIT (1u << 22)
+#define A4_LOG2E 1.4426950408889634f
+
+struct A4Args {
+    const void* q; void* out;
+    Kv4Cache c;
+    const int* seg_start; const int* seg_len; const int* seg_pos0; const int* block_tables;
+    float* part_acc;                  // [n_seg][K * row_blocks][splits][rows][hs]
+    float* part_ml;                   // [n_seg][K * row_blocks][splits][rows][2]
+    int* status;
+    long long q_stride;
+    int H, G, D, max_pages, window, keep, splits, span_tiles, row_blocks, most_rows;
+    float scale, softcap;
+    const float* sink;
+    XrBias bias;
+    int wide, wide_out;               // 16-byte loads of q; four neighbouring outputs at once
+    int tile_shift;                   // pages of 2^tile_shift whole tiles (-1: pages of other sizes)
+};
+
+// Four neighbouring elements of an output row: divided by the row's sum, to which a sink adds exp(sink - maximum).
+template <bool F32>
+__device__ __forceinline__ void a4_out(const A4Args& a, int tok0, int kvh, int row, int d, float4 v, float m, float sum) {
+    if (d >= a.D) return;
+    const int head = kvh * a.G + row % a.G;
+    if (a.sink != nullptr) { float e; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(a.sink[head], A4_LOG2E, -m))); sum += e; }
+    const float inv = 1.0f / sum;
+    const float x[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+    const long long at = ((long long)(tok0 + row / a.G) * a.H + head) * a.D + d;
+    if constexpr (F32) {
+        float* dst = (float*)a.out + at;
+        if (a.wide_out) *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+        else
+            for (int e = 0; e < 4; e++) if (d + e < a.D) dst[e] = x[e];
+    } else {
+        __nv_bfloat16* dst = (__nv_bfloat16*)a.out + at;
+        if (a.wide_out) {
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0], x[1]), hi = __floats2bfloat162_rn(x[2], x[3]);
+            *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+        } else
+            for (int e = 0; e < 4; e++) if (d + e < a.D) dst[e] = __float2bfloat16_rn(x[e]);
+    }
+}
+
+__device__ __forceinline__ uint32_t a4_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ bool a4_wait(uint64_t* bar, uint32_t parity) {
+    for (uint32_t i = 0; i < A4_SPIN_LIMIT; i++) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(a4_smem(bar)), "r"(parity) : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+__device__ __forceinline__ void a4_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(a4_smem(dst)), "l"(src), "r"(bytes), "r"(a4_smem(bar)) : "memory");
+}
+__device__ __forceinline__ void a4_mma(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t a4_turn(uint32_t x) {            // transpose of an 8 x 8 matrix of 16-bit numbers over the warp
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+__device__ __forceinline__ float a4_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ uint32_t a4_pack(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// Takes the leading bfloat16 piece off a pair: returns it, leaves the (exact) rest.
+__device__ __forceinline__ uint32_t a4_piece(float& lo, float& hi) {
+    const uint32_t r = a4_pack(lo, hi);
+    lo -= __uint_as_float(r << 16);
+    hi -= __uint_as_float(r & 0xffff0000u);
+    return r;
+}
+// Row r of a 16-key subtile's S^T, and equally place r along k of the second product, is key 8 (r / 8) + at_key(r % 8): the places 2t of a
+// group of four threads are four neighbouring keys, and so are the places 2t + 1.
+__device__ __forceinline__ int a4_key(int r) { return (r & 8) + 4 * (r & 1) + (((r & 7) >> 1) ^ (r & 1)); }
+
+template <int NG> struct A4Tile { static constexpr int KEYS = NG == 2 ? 64 : 32; };
+
+// The tiles that the rows of a block see: those of the kept first keys, then those of the window.
+struct A4Walk { int lo, hi, t_lo, kept, n; };
+__device__ __forceinline__ A4Walk a4_walk(int first_pos, int last_pos, int window, int keep, int tile) {
+    A4Walk w;
+    w.lo = window > 0 ? max(0, first_pos - window + 1) : 0;
+    w.hi = last_pos;
+    w.t_lo = w.lo / tile;
+    w.kept = xr_kept_tiles(keep, w.lo, tile);
+    w.n = w.kept + w.hi / tile - w.t_lo + 1;
+    return w;
+}
+// Spans of a request: a.span_tiles tiles each, the last of the grid's takes what is left (a captured launch may meet longer requests
+// than the one it was planned for).
+__device__ __forceinline__ int a4_spans(const A4Args& a, const A4Walk& w) { return min((w.n + a.span_tiles - 1) / a.span_tiles, a.splits); }
+
+// NG: groups of 32 elements a held head (2, 4, 8); NT: eight-row tiles a block; F32: float32 queries and outputs, in pieces (NT 1);
+// EXTRA: a cap or a bias on the scores
+template <int NG, int NT, bool F32, bool EXTRA> struct A4Shape {
+    static constexpr int HS = NG * 32, TK = A4Tile<NG>::KEYS, SUB = TK / 16, KS = 2 * NG, RB = 8 * NT, P = F32 ? 3 : 1;
+    static constexpr int CODES = HS / 2, SCALES = HS / 16;           // bytes of a token's keys (or values)
+    static constexpr int STAGE = TK * 2 * (CODES + SCALES);
+    static constexpr int VW = NG / 2, MT = 4 * VW;                   // words of a value's row a thread takes; m-tiles of O^T
+    static constexpr bool Q_REGS = KS * 2 * NT * P <= 48;            // q's fragments in registers, else in shared memory
+    static constexpr int BLOCKS = NG <= 4 && NT == 1 && !F32 ? 4 : 2;            // blocks an SM (registers, shared memory)
+    static constexpr int SMEM = A4_WARPS * A4_STAGES * (STAGE + 8) + 4 * A4_PAGES + (Q_REGS ? 0 : P * NT * KS * 32 * 8) + 16;
+};
+
+template <int NG, int NT, bool F32, bool EXTRA>
+__global__ void __launch_bounds__(A4_THREADS, (A4Shape<NG, NT, F32, EXTRA>::BLOCKS))
+k_kv4_attention(A4Args a) {
+    xr_pdl_launch();
+    using S = A4Shape<NG, NT, F32, EXTRA>;
+    constexpr int HS = S::HS, TK = S::TK, SUB = S::SUB, KS = S::KS, RB = S::RB, P = S::P, CODES = S::CODES, SCALES = S::SCALES, STAGE = S::STAGE;
+    constexpr int VW = S::VW, MT = S::MT;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint64_t* bars = (uint64_t*)(smem + A4_WARPS * A4_STAGES * STAGE);
+    int* gave_up = (int*)(bars + A4_WARPS * A4_STAGES);
+    int* pages = gave_up + 4;
+    uint2* q_sm = (uint2*)(pages + A4_PAGES);                        // [P][NT][KS][32]
+    const int seg = blockIdx.z, kvh = blockIdx.y % a.c.K, rb = blockIdx.y / a.c.K, span = blockIdx.x;
+    xr_pdl_wait();
+    const int L = a.seg_len[seg];
+    const long long rows_all = (long long)L * a.G;
+    if (L < 1 || rows_all > a.most_rows || (long long)rb * RB >= rows_all) return;
+    const int row0 = rb * RB, rows = (int)min((long long)RB, rows_all - row0);
+    const int pos0 = a.seg_pos0[seg], tok0 = a.seg_start[seg];
+    const int first_pos = pos0 + row0 / a.G, last_pos = pos0 + (row0 + rows - 1) / a.G;
+    const A4Walk walk = a4_walk(first_pos, last_pos, a.window, a.keep, TK);
+    const int n_spans = a4_spans(a, walk);
+    if (span >= n_spans) return;
+    const int i_begin = span * a.span_tiles, i_end = span == n_spans - 1 ? walk.n : i_begin + a.span_tiles;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int* bt = a.block_tables + (size_t)seg * a.max_pages;
+    const int ps = a.c.page_size;
+    const int page0 = (int)((long long)xr_walk_tile(i_begin, walk.kept, walk.t_lo) * TK / ps);
+    for (int i = threadIdx.x; i < A4_PAGES; i += A4_THREADS) {
+        const int pi = page0 + i;
+        pages[i] = pi < a.max_pages && (long long)pi * ps <= walk.hi ? bt[pi] : -1;
+    }
+    if (threadIdx.x < A4_WARPS * A4_STAGES) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(a4_smem(&bars[threadIdx.x])), "r"(1));
+    if (threadIdx.x == 0) *gave_up = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+
+    // q: thread (row g, t) holds the elements that its words of a key hold, 8 NG t ..; k-step 2 w + half: elements 8 w + 4 half ..
+    uint32_t qf[S::Q_REGS ? P : 1][S::Q_REGS ? NT : 1][S::Q_REGS ? KS : 1][2];
+    if (S::Q_REGS || warp == 0) {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const int row = row0 + nt * 8 + g, live = nt * 8 + g < rows;
+            const long long base = live ? (long long)(tok0 + row / a.G) * a.q_stride + (long long)(kvh * a.G + row % a.G) * a.D : 0;
+#pragma unroll
+            for (int w = 0; w < NG; w++) {
+                const int d = 8 * (NG * t + w);
+                if constexpr (!F32) {
+                    uint32_t x[4] = {0, 0, 0, 0};
+                    const __nv_bfloat16* src = (const __nv_bfloat16*)a.q + base + d;
+                    if (a.wide) {
+                        if (live && d < a.D) { const uint4 v = *reinterpret_cast<const uint4*>(src); x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            if (live && d + e < a.D) x[e >> 1] |= (uint32_t)reinterpret_cast<const unsigned short*>(src)[e] << (16 * (e & 1));
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        if constexpr (S::Q_REGS) { qf[0][nt][2 * w + h][0] = x[2 * h]; qf[0][nt][2 * w + h][1] = x[2 * h + 1]; }
+                        else q_sm[(nt * KS + 2 * w + h) * 32 + lane] = make_uint2(x[2 * h], x[2 * h + 1]);
+                    }
+                } else {
+                    float x[8];
+                    const float* src = (const float*)a.q + base + d;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[e] = live && d + e < a.D ? src[e] : 0.f;
+#pragma unroll
+                    for (int p = 0; p < 3; p++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const uint32_t u = a4_piece(x[4 * h], x[4 * h + 1]), v = a4_piece(x[4 * h + 2], x[4 * h + 3]);
+                            if constexpr (S::Q_REGS) { qf[p][nt][2 * w + h][0] = u; qf[p][nt][2 * w + h][1] = v; }
+                            else q_sm[((p * NT + nt) * KS + 2 * w + h) * 32 + lane] = make_uint2(u, v);
+                        }
+                }
+            }
+        }
+    }
+    __syncthreads();
+    uint8_t* my_ring = smem + warp * A4_STAGES * STAGE;              // a stage: keys' codes, values' codes, keys' scales, values' scales
+    uint64_t* my_bars = bars + warp * A4_STAGES;
+    const uint8_t* head_run = a.c.base + a.c.layer_at + (long long)kvh * a.c.block();
+    // Lane 0 fetches tile i of the walk into stage s, a page's piece at a time.  Rows on a page that is not held are rows of zeros.
+    auto page_at = [&](int pi) -> int {
+        const int page = pi - page0 < A4_PAGES && pi >= page0 ? pages[pi - page0] : pi < a.max_pages ? bt[pi] : -1;
+        return page < a.c.n_pages ? page : -1;
+    };
+    auto piece = [&](uint8_t* st, int r, int page, int tok, int len, uint64_t* bar) {
+        const uint8_t* run = head_run + page * a.c.page_bytes;
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+            a4_copy(st + w * TK * CODES + r * CODES, run + a.c.codes_at(w) + tok * CODES, len * CODES, bar);
+            a4_copy(st + 2 * TK * CODES + w * TK * SCALES + r * SCALES, run + a.c.scales_at(w) + tok * SCALES, len * SCALES, bar);
+        }
+    };
+    auto fetch = [&](int i, int s) {
+        const long long k0 = (long long)xr_walk_tile(i, walk.kept, walk.t_lo) * TK;
+        uint8_t* st = my_ring + s * STAGE;
+        uint64_t* bar = &my_bars[s];
+        if (a.tile_shift >= 0) {
+            // (a page holds 2^tile_shift whole tiles)
+            const int tile = (int)(k0 / TK), page = page_at(tile >> a.tile_shift), tok = (tile & ((1 << a.tile_shift) - 1)) * TK;
+            if (page >= 0) {
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(a4_smem(bar)), "r"(STAGE) : "memory");
+                piece(st, 0, page, tok, TK, bar);
+                return;
+            }
+        }
+        uint32_t bytes = 0;
+        for (int pass = 0; pass < 2; pass++) {
+            for (int r = 0; r < TK;) {
+                const int pi = (int)((k0 + r) / ps), tok = (int)(k0 + r - (long long)pi * ps), len = min(TK - r, ps - tok), page = page_at(pi);
+                if (page >= 0) {
+                    if (pass == 0) bytes += len * 2 * (CODES + SCALES);
+                    else piece(st, r, page, tok, len, bar);
+                } else if (pass == 0) {
+                    for (int w = 0; w < 2; w++)
+                        for (int b = 0; b < len * SCALES; b += 4) *reinterpret_cast<uint32_t*>(st + 2 * TK * CODES + w * TK * SCALES + r * SCALES + b) = 0;
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                r += len;
+            }
+            // (all bytes are announced before the first copy, so that the barrier's phase cannot end among them)
+            if (pass == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(a4_smem(bar)), "r"(bytes) : "memory");
+        }
+    };
+    if (lane == 0) {
+#pragma unroll
+        for (int s = 0; s < A4_STAGES; s++)
+            if (i_begin + warp + s * A4_WARPS < i_end) fetch(i_begin + warp + s * A4_WARPS, s);
+    }
+    __syncwarp();
+
+    int pos_r[NT][2];                                                // positions of this thread's two columns (rows of q) of each tile
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) pos_r[nt][e] = pos0 + (row0 + min(nt * 8 + 2 * t + e, rows - 1)) / a.G;
+    const float sl = a.scale * A4_LOG2E;
+    float o[NT][MT][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+        for (int i = 0; i < MT; i++) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+        m[nt][0] = m[nt][1] = -INFINITY; l[nt][0] = l[nt][1] = 0.f;
+    }
+    const int key_a = a4_key(g);                                     // a subtile's key of row g (row g + 8: 8 further)
+    const int place_a = t, place_b = 4 + (t ^ 1);                    // ... of places 2t and 2t + 1
+    const int vgroup = g * VW / 4;
+    int stage = 0;
+    uint32_t phase = 0;
+    bool lost = false;
+    for (int i = i_begin + warp; i < i_end; i += A4_WARPS) {
+        const int k0 = xr_walk_tile(i, walk.kept, walk.t_lo) * TK;
+        const uint8_t* kc = my_ring + stage * STAGE;
+        const uint8_t* vc = kc + TK * CODES;
+        const uint8_t* ks = vc + TK * CODES;
+        const uint8_t* vs = ks + TK * SCALES;
+        if (!__all_sync(0xffffffffu, a4_wait(&my_bars[stage], phase))) { lost = true; break; }
+        float s[SUB][NT][4];
+#pragma unroll
+        for (int sub = 0; sub < SUB; sub++) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) s[sub][nt][0] = s[sub][nt][1] = s[sub][nt][2] = s[sub][nt][3] = 0.f;
+            const int ka = sub * 16 + key_a, kb = ka + 8;
+            uint32_t wa[NG], wb[NG];
+            if constexpr (NG == 2) {
+                const uint2 x = *reinterpret_cast<const uint2*>(kc + ka * CODES + 8 * t), y = *reinterpret_cast<const uint2*>(kc + kb * CODES + 8 * t);
+                wa[0] = x.x; wa[1] = x.y; wb[0] = y.x; wb[1] = y.y;
+            } else {
+#pragma unroll
+                for (int c = 0; c < NG / 4; c++) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(kc + ka * CODES + 4 * NG * t + 16 * c), y = *reinterpret_cast<const uint4*>(kc + kb * CODES + 4 * NG * t + 16 * c);
+                    wa[4 * c] = x.x; wa[4 * c + 1] = x.y; wa[4 * c + 2] = x.z; wa[4 * c + 3] = x.w;
+                    wb[4 * c] = y.x; wb[4 * c + 1] = y.y; wb[4 * c + 2] = y.z; wb[4 * c + 3] = y.w;
+                }
+            }
+#pragma unroll
+            for (int w0 = 0; w0 < NG; w0 += NG == 2 ? 2 : 4) {
+                // (a thread's words of one group share a scale)
+                const int grp = (NG * t + w0) / 4;
+                uint32_t sa = *reinterpret_cast<const unsigned short*>(ks + ka * SCALES + 2 * grp), sb = *reinterpret_cast<const unsigned short*>(ks + kb * SCALES + 2 * grp);
+                sa |= sa << 16; sb |= sb << 16;
+                const uint32_t ma = kv4_m24(sa), mb = kv4_m24(sb);
+#pragma unroll
+                for (int w = w0; w < w0 + (NG == 2 ? 2 : 4); w++) {
+                    const uint32_t a0 = kv4_scaled(kv4_pair<0>(wa[w]), sa, ma), a1 = kv4_scaled(kv4_pair<0>(wb[w]), sb, mb);
+                    const uint32_t a2 = kv4_scaled(kv4_pair<1>(wa[w]), sa, ma), a3 = kv4_scaled(kv4_pair<1>(wb[w]), sb, mb);
+                    const uint32_t b0 = kv4_scaled(kv4_pair<2>(wa[w]), sa, ma), b1 = kv4_scaled(kv4_pair<2>(wb[w]), sb, mb);
+                    const uint32_t b2 = kv4_scaled(kv4_pair<3>(wa[w]), sa, ma), b3 = kv4_scaled(kv4_pair<3>(wb[w]), sb, mb);
+#pragma unroll
+                    for (int p = P - 1; p >= 0; p--)
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            uint2 qa, qb;
+                            if constexpr (S::Q_REGS) { qa = make_uint2(qf[p][nt][2 * w][0], qf[p][nt][2 * w][1]); qb = make_uint2(qf[p][nt][2 * w + 1][0], qf[p][nt][2 * w + 1][1]); }
+                            else { qa = q_sm[((p * NT + nt) * KS + 2 * w) * 32 + lane]; qb = q_sm[((p * NT + nt) * KS + 2 * w + 1) * 32 + lane]; }
+                            a4_mma(s[sub][nt], a0, a1, a2, a3, qa.x, qa.y);
+                            a4_mma(s[sub][nt], b0, b1, b2, b3, qb.x, qb.y);
+                        }
+                }
+            }
+        }
+        // a tile that not every row sees whole
+        const bool edge = k0 + TK - 1 > first_pos || (a.window > 0 && k0 <= last_pos - a.window && k0 + TK > a.keep);
+        if constexpr (EXTRA) {
+#pragma unroll
+            for (int sub = 0; sub < SUB; sub++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        float& x = s[sub][nt][e];
+                        if (a.softcap > 0.f) {
+                            // c tanh(x scale / c) / scale, through one exponential: tanh(y) = 1 - 2 / (exp(2 y) + 1)
+                            const float cap = a.softcap / a.scale, ex = __expf(2.0f * x * (a.scale / a.softcap));
+                            x = F32 ? cap * tanhf(x * (a.scale / a.softcap)) : cap * (1.0f - __fdividef(2.0f, ex + 1.0f));
+                        } else {
+                            const int row = row0 + min(nt * 8 + 2 * t + (e & 1), rows - 1);
+                            x += xr_bias_at(a.bias.table + (size_t)(kvh * a.G + row % a.G) * a.bias.len, a.bias.len, pos_r[nt][e & 1] - (k0 + sub * 16 + key_a + 4 * (e & 2)));
+                        }
+                    }
+        }
+        if (edge) {
+#pragma unroll
+            for (int sub = 0; sub < SUB; sub++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int key = k0 + sub * 16 + key_a + 4 * (e & 2), pos = pos_r[nt][e & 1];
+                        if (!xr_sees(key, pos, a.window > 0 ? pos - a.window + 1 : 0, a.keep)) s[sub][nt][e] = -INFINITY;
+                    }
+        }
+        float off[NT][2], f[NT][2];
+        bool grown = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float mx = fmaxf(s[0][nt][e], s[0][nt][e + 2]);
+#pragma unroll
+                for (int sub = 1; sub < SUB; sub++) mx = fmaxf(mx, fmaxf(s[sub][nt][e], s[sub][nt][e + 2]));
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                const float was = m[nt][e];
+                m[nt][e] = fmaxf(was, mx * sl);
+                off[nt][e] = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
+                f[nt][e] = a4_exp2(was - off[nt][e]);
+                grown |= was != m[nt][e];
+            }
+        if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                l[nt][0] *= f[nt][0]; l[nt][1] *= f[nt][1];
+#pragma unroll
+                for (int d = 0; d < MT; d++) { o[nt][d][0] *= f[nt][0]; o[nt][d][1] *= f[nt][1]; o[nt][d][2] *= f[nt][0]; o[nt][d][3] *= f[nt][1]; }
+            }
+        }
+#pragma unroll
+        for (int sub = 0; sub < SUB; sub++) {
+            uint32_t pb[P][NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) { x[e] = a4_exp2(fmaf(s[sub][nt][e], sl, -off[nt][e & 1])); l[nt][e & 1] += x[e]; }
+#pragma unroll
+                for (int p = 0; p < P; p++) {
+                    pb[p][nt][0] = a4_turn(P == 1 ? a4_pack(x[0], x[1]) : a4_piece(x[0], x[1]));
+                    pb[p][nt][1] = a4_turn(P == 1 ? a4_pack(x[2], x[3]) : a4_piece(x[2], x[3]));
+                }
+            }
+            const int k1 = sub * 16 + place_a, k2 = sub * 16 + place_b;              // places 2t, 2t + 1; 8 further: 2t + 8, 2t + 9
+            uint32_t w[4][VW];
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const uint8_t* src = vc + ((c & 1 ? k2 : k1) + 8 * (c >> 1)) * CODES + 4 * VW * g;
+                if constexpr (VW == 1) w[c][0] = *reinterpret_cast<const uint32_t*>(src);
+                else if constexpr (VW == 2) { const uint2 x = *reinterpret_cast<const uint2*>(src); w[c][0] = x.x; w[c][1] = x.y; }
+                else { const uint4 x = *reinterpret_cast<const uint4*>(src); w[c][0] = x.x; w[c][1] = x.y; w[c][2] = x.z; w[c][3] = x.w; }
+            }
+            uint32_t sv[4];
+#pragma unroll
+            for (int c = 0; c < 4; c++) sv[c] = *reinterpret_cast<const unsigned short*>(vs + ((c & 1 ? k2 : k1) + 8 * (c >> 1)) * SCALES + 2 * vgroup);
+            if (edge) {
+                // What lies behind the last key or ahead of the window may be anything, scales that are no numbers too: no row sees it.
+                uint32_t none = 0;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const int at = (c & 1 ? k2 : k1) + 8 * (c >> 1), key = k0 + at;
+                    if (!xr_sees(key, walk.hi, walk.lo, a.keep)) sv[c] = 0;
+                    if ((sv[c] & 0x7f80) == 0x7f80) none |= 1u << (at & 15);
+                }
+                if (first_pos != last_pos && __any_sync(0xffffffffu, none != 0)) {
+                    // A value that is no number, and rows of several positions, some of which may not see it: it is left out of the
+                    // products, and the elements of its group become NaN for the rows that do see it.
+                    none |= __shfl_xor_sync(0xffffffffu, none, 1);
+                    none |= __shfl_xor_sync(0xffffffffu, none, 2);
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        if ((sv[c] & 0x7f80) == 0x7f80) sv[c] = 0;
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            bool hit = false;
+                            for (int b = 0; b < 16; b++)
+                                hit |= (none >> b & 1) && xr_sees(k0 + sub * 16 + b, pos_r[nt][e], a.window > 0 ? pos_r[nt][e] - a.window + 1 : 0, a.keep);
+                            if (hit) {
+#pragma unroll
+                                for (int d = 0; d < MT; d++) o[nt][d][e] = o[nt][d][e + 2] = __int_as_float(0x7fc00000);
+                            }
+                        }
+                }
+            }
+            const uint32_t s0 = sv[0] | (sv[1] << 16), s1 = sv[2] | (sv[3] << 16), m0 = kv4_m24(s0), m1 = kv4_m24(s1);
+#pragma unroll
+            for (int j = 0; j < VW; j++) {
+                // the halves of two keys' words side by side: pair i of them is element 2i (low halves) or 2i + 1 of both keys
+                const uint32_t lo0 = __byte_perm(w[0][j], w[1][j], 0x5410), hi0 = __byte_perm(w[0][j], w[1][j], 0x7632);
+                const uint32_t lo1 = __byte_perm(w[2][j], w[3][j], 0x5410), hi1 = __byte_perm(w[2][j], w[3][j], 0x7632);
+#define A4_VALUES(I)                                                                                                                              \
+                {                                                                                                                                 \
+                    const uint32_t a0 = kv4_scaled(kv4_pair<I>(lo0), s0, m0), a1 = kv4_scaled(kv4_pair<I>(hi0), s0, m0);                          \
+                    const uint32_t a2 = kv4_scaled(kv4_pair<I>(lo1), s1, m1), a3 = kv4_scaled(kv4_pair<I>(hi1), s1, m1);                          \
+                    _Pragma("unroll") for (int p = P - 1; p >= 0; p--)                                                                            \
+                        _Pragma("unroll") for (int nt = 0; nt < NT; nt++) a4_mma(o[nt][4 * j + I], a0, a1, a2, a3, pb[p][nt][0], pb[p][nt][1]);   \
+                }
+                A4_VALUES(0) A4_VALUES(1) A4_VALUES(2) A4_VALUES(3)
+#undef A4_VALUES
+            }
+        }
+        __syncwarp();
+        if (lane == 0 && i + A4_STAGES * A4_WARPS < i_end) fetch(i + A4_STAGES * A4_WARPS, stage);
+        if (++stage == A4_STAGES) { stage = 0; phase ^= 1; }
+    }
+    if (lost && lane == 0) {
+        // a copy did not arrive: what is still in flight is waited for (within the same limit) before the block may end
+        *gave_up = 1;
+        for (int s = 1; s < A4_STAGES; s++) {
+            if (++stage == A4_STAGES) { stage = 0; phase ^= 1; }
+            a4_wait(&my_bars[stage], phase);
+        }
+    }
+    // the warps' sums meet in the ring's memory: [warp][row][HS], then [warp][row] (maximum, sum)
+    __syncthreads();
+    if (threadIdx.x == 0 && *gave_up) atomicExch(a.status, 5);
+    float* acc_s = reinterpret_cast<float*>(smem);
+    float* ml_s = acc_s + A4_WARPS * RB * HS;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int r = nt * 8 + 2 * t + e;
+            float sum = l[nt][e];
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            float* dst = acc_s + (warp * RB + r) * HS + 8 * VW * g;
+#pragma unroll
+            for (int j = 0; j < VW; j++) {
+                *reinterpret_cast<float4*>(dst + 8 * j) = make_float4(o[nt][4 * j][e], o[nt][4 * j][e + 2], o[nt][4 * j + 1][e], o[nt][4 * j + 1][e + 2]);
+                *reinterpret_cast<float4*>(dst + 8 * j + 4) = make_float4(o[nt][4 * j + 2][e], o[nt][4 * j + 2][e + 2], o[nt][4 * j + 3][e], o[nt][4 * j + 3][e + 2]);
+            }
+            if (g == 0) { ml_s[(warp * RB + r) * 2] = m[nt][e]; ml_s[(warp * RB + r) * 2 + 1] = sum; }
+        }
+    __syncthreads();
+    const size_t item = ((size_t)seg * gridDim.y + blockIdx.y) * a.splits + span;
+    for (int q = threadIdx.x; q < rows * (HS / 4); q += A4_THREADS) {
+        const int r = q / (HS / 4), d = (q % (HS / 4)) * 4;
+        float mm = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < A4_WARPS; w++) mm = fmaxf(mm, ml_s[(w * RB + r) * 2]);
+        const float at = mm == -INFINITY ? 0.f : mm;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < A4_WARPS; w++) {
+            const float k = a4_exp2(ml_s[(w * RB + r) * 2] - at);
+            const float4 u = *reinterpret_cast<const float4*>(acc_s + (w * RB + r) * HS + d);
+            v.x += u.x * k; v.y += u.y * k; v.z += u.z * k; v.w += u.w * k;
+            sum += ml_s[(w * RB + r) * 2 + 1] * k;
+        }
+        if (n_spans == 1) a4_out<F32>(a, tok0, kvh, row0 + r, d, v, at, sum);
+        else {
+            *reinterpret_cast<float4*>(a.part_acc + (item * RB + r) * HS + d) = v;
+            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (item * RB + r) * 2) = make_float2(mm, sum);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// The spans of one (request, kv head, row block) in ascending order: grid (K * row blocks, requests).  A thread owns four neighbouring elements of
+// a row and every `groups`-th span; the groups' sums meet in shared memory in ascending order.
+// ---------------------------------------------------------------------------------------------
+#define A4_MERGE_THREADS 512
+#define A4_MAX_SPLITS 256
+template <int NG, int RB, bool F32>
+__global__ void __launch_bounds__(A4_MERGE_THREADS)
+k_kv4_merge(A4Args a) {
+    xr_pdl_launch();
+    constexpr int HS = NG * 32, QUADS = HS / 4, TK = A4Tile<NG>::KEYS;
+    __shared__ float wgt[RB][A4_MAX_SPLITS];
+    __shared__ float row_max[RB], row_sum[RB];
+    __shared__ float4 part[A4_MERGE_THREADS];
+    const int seg = blockIdx.y, kvh = blockIdx.x % a.c.K, rb = blockIdx.x / a.c.K;
+    xr_pdl_wait();
+    const int L = a.seg_len[seg];
+    const long long rows_all = (long long)L * a.G;
+    if (L < 1 || rows_all > a.most_rows || (long long)rb * RB >= rows_all) return;
+    const int row0 = rb * RB, rows = (int)min((long long)RB, rows_all - row0), pos0 = a.seg_pos0[seg];
+    const int n_spans = a4_spans(a, a4_walk(pos0 + row0 / a.G, pos0 + (row0 + rows - 1) / a.G, a.window, a.keep, TK));
+    if (n_spans == 1) return;                                        // (written already)
+    const size_t item = ((size_t)seg * gridDim.x + blockIdx.x) * a.splits;
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + item * RB;
+    const float4* acc = reinterpret_cast<const float4*>(a.part_acc) + item * RB * QUADS;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int r = warp; r < rows; r += A4_MERGE_THREADS / 32) {
+        float mm = -INFINITY;
+        for (int s = lane; s < n_spans; s += 32) mm = fmaxf(mm, __ldcg(&ml[(size_t)s * RB + r]).x);
+        mm = xr_warp_max(mm);
+        const float at = mm == -INFINITY ? 0.f : mm;
+        float sum = 0.f;
+        for (int s = lane; s < n_spans; s += 32) {
+            const float2 x = __ldcg(&ml[(size_t)s * RB + r]);
+            const float k = a4_exp2(x.x - at);
+            wgt[r][s] = k;
+            sum += x.y * k;
+        }
+        sum = xr_warp_sum(sum);
+        if (lane == 0) { row_max[r] = at; row_sum[r] = sum; }
+    }
+    __syncthreads();
+    for (int q0 = 0; q0 < rows * QUADS; q0 += A4_MERGE_THREADS) {
+        const int owned = min(A4_MERGE_THREADS, rows * QUADS - q0), groups = A4_MERGE_THREADS / owned;
+        const int grp = threadIdx.x / owned, e = q0 + threadIdx.x % owned, r = e / QUADS;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (grp < groups) {
+#pragma unroll 4
+            for (int s = grp; s < n_spans; s += groups) {
+                const float4 u = __ldcg(acc + (size_t)s * RB * QUADS + e);
+                const float k = wgt[r][s];
+                v.x += u.x * k; v.y += u.y * k; v.z += u.z * k; v.w += u.w * k;
+            }
+        }
+        __syncthreads();
+        part[threadIdx.x] = v;
+        __syncthreads();
+        if (threadIdx.x < owned) {
+            for (int k = 1; k < groups; k++) {
+                const float4 u = part[k * owned + threadIdx.x];
+                v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+            }
+            a4_out<F32>(a, a.seg_start[seg], kvh, row0 + r, (e % QUADS) * 4, v, row_max[r], row_sum[r]);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Blocks that are resident at once, and a row block's size, for a head size and type.  wide_rows: some request has more than eight packed rows.
+static int a4_rows(int f32, int wide_rows) { return f32 || !wide_rows ? 8 : 16; }
+static int a4_resident(int hs, int f32, int wide_rows) { return (hs <= 128 && !f32 && !wide_rows ? 4 : 2) * xr_sm_count(); }
+static int a4_tile(int hs) { return hs == 64 ? 64 : 32; }
+
+// How a step is cut: row blocks of the longest portion that is taken (at most `most_rows` packed rows), tiles a span, spans of the longest
+// request.  len, pos0: the portions on the HOST; max_kv: the longest key range to be prepared for (0: what the portions say).
+struct A4Plan { int row_blocks, wide, span_tiles, splits; };
+static A4Plan a4_plan(const int* len, const int* pos0, int n_seg, int K, int G, int hs, int f32, int window, int keep, int most_rows, int max_kv) {
+    const int tile = a4_tile(hs);
+    long long rows = 0;
+    for (int s = 0; s < n_seg; s++) {
+        const long long r = (long long)len[s] * G;
+        if (r <= most_rows && r > rows) rows = r;
+    }
+    A4Plan p{0, rows > 8, 1, 1};
+    if (rows < 1) return p;
+    const int rb = a4_rows(f32, p.wide);
+    p.row_blocks = (int)((rows + rb - 1) / rb);
+    long long total = 0, longest = 1;
+    for (int s = 0; s < n_seg; s++) {
+        const long long r = (long long)len[s] * G;
+        if (len[s] < 1 || r > most_rows) continue;
+        // (tiles of the last row block, whose window is the furthest)
+        const long long end = (long long)pos0[s] + len[s];
+        const long long lo = window > 0 && end - len[s] - window + 1 > 0 ? end - len[s] - window + 1 : 0;
+        const long long tiles = (end - 1) / tile - lo / tile + 1 + xr_kept_tiles(keep, (int)lo, tile);
+        total += tiles * K * ((r + rb - 1) / rb);
+        longest = tiles > longest ? tiles : longest;
+    }
+    if (max_kv > 0) {
+        const long long range = window > 0 && window + 16 < max_kv ? window + 16 : max_kv;
+        const long long tiles = (range + tile - 1) / tile + 1 + (window > 0 ? (keep + tile - 1) / tile : 0);
+        longest = tiles > longest ? tiles : longest;
+    }
+    // as many tiles a span as give every resident block one span, a multiple of the warps
+    const long long resident = a4_resident(hs, f32, p.wide);
+    long long span = (total + resident - 1) / resident;
+    span = (span + A4_WARPS - 1) / A4_WARPS * A4_WARPS;
+    const long long least = ((longest + A4_MAX_SPLITS - 1) / A4_MAX_SPLITS + A4_WARPS - 1) / A4_WARPS * A4_WARPS;
+    if (span < least) span = least;
+    if (span < A4_WARPS) span = A4_WARPS;
+    p.span_tiles = (int)span;
+    p.splits = (int)((longest + span - 1) / span);
+    return p;
+}
+
+template <int NG, int NT, bool F32, bool EXTRA>
+static int a4_launch(const A4Args& a, int n_seg, cudaStream_t stream) {
+    using S = A4Shape<NG, NT, F32, EXTRA>;
+    static_assert(A4_WARPS * S::RB * (S::HS + 2) * 4 <= A4_WARPS * A4_STAGES * S::STAGE, "the warps' sums lie in the ring");
+    static bool ready[XR_DEVICES];
+    if (!xr_once_per_device(ready, [] { return xr_allow_smem(k_kv4_attention<NG, NT, F32, EXTRA>, S::SMEM); })) return XR_ERR_LAUNCH;
+    xr_launch((k_kv4_attention<NG, NT, F32, EXTRA>), dim3(a.splits, a.c.K * a.row_blocks, n_seg), dim3(A4_THREADS), S::SMEM, stream, a);
+    if (xr_launch_status() != XR_OK) return XR_ERR_LAUNCH;
+    if (a.splits > 1) xr_launch((k_kv4_merge<NG, S::RB, F32>), dim3(a.c.K * a.row_blocks, n_seg), dim3(A4_MERGE_THREADS), 0, stream, a);
+    return xr_launch_status();
+}
+template <int NG, int NT, bool F32>
+static int a4_launch(const A4Args& a, int n_seg, cudaStream_t stream) {
+    return a.softcap > 0.f || a.bias.table != nullptr ? a4_launch<NG, NT, F32, true>(a, n_seg, stream) : a4_launch<NG, NT, F32, false>(a, n_seg, stream);
+}
+template <int NG>
+static int a4_launch(const A4Args& a, int n_seg, int f32, int wide, cudaStream_t stream) {
+    return f32 ? a4_launch<NG, 1, true>(a, n_seg, stream) : wide ? a4_launch<NG, 2, false>(a, n_seg, stream) : a4_launch<NG, 1, false>(a, n_seg, stream);
+}
+
+// float32 values of scratch that xr_kv4_attention needs for these portions (host arrays len, pos0), 0 if none.
+XR_EXPORT long long xr_kv4_attention_floats(const int* len, const int* pos0, int n_seg, int K, int G, int D, int dtype, int window, int keep, int most_rows,
+                                            int max_kv) {
+    if (n_seg < 1 || K < 1 || G < 1 || D < 1 || D > 256) return 0;
+    const int hs = kv4_held(D), f32 = dtype == XR_F32;
+    const A4Plan p = a4_plan(len, pos0, n_seg, K, G, hs, f32, window, window > 0 ? keep : 0, most_rows, max_kv);
+    if (p.row_blocks < 1 || p.splits < 2) return 0;
+    return (long long)n_seg * K * p.row_blocks * p.splits * a4_rows(f32, p.wide) * (hs + 2);
+}
+
+// q: token t, head h at q + t * q_stride + h * D; out [n][H * D], both of `dtype`.  Portions of at most `most_rows` packed rows (tokens x heads per
+// kv head) are computed, longer ones passed over.  len, pos0: the same lengths and first positions as seg_len and seg_pos0, on the host (they
+// size the grid; what is computed goes by the device's).
+XR_EXPORT int xr_kv4_attention(const void* q, void* out, int dtype, const void* cache, long long n_pages, int layers, int layer, int K, int block, int page_size,
+                               const int* seg_start, const int* seg_len, const int* seg_pos0, const int* block_tables, const int* len, const int* pos0,
+                               float* scratch, long long floats, int* status, long long q_stride, int n_seg, int H, int D, int max_pages, int window,
+                               float scale, const float* sink, float softcap, int keep_first, const float* bias, int bias_len, int most_rows, int max_kv,
+                               cudaStream_t stream) {
+    if (n_seg < 1 || n_seg > 65535 || H < 1 || H % K != 0 || max_pages < 1 || window < 0 || keep_first < 0 || !(scale > 0.f) || !(softcap >= 0.f) ||
+        (bias != nullptr && (bias_len < 1 || softcap > 0.f)) || status == nullptr || most_rows < 1 || max_kv < 0 || q_stride < (long long)H * D ||
+        (dtype != XR_F32 && dtype != XR_BF16) || !kv4_cache_ok(cache, n_pages, layers, layer, K, block, page_size, D) ||
+        (long long)max_pages * page_size > 0x7fffffffLL - 64)
+        return XR_ERR_ARG;
+    const int G = H / K, f32 = dtype == XR_F32, hs = kv4_held(D), keep = window > 0 ? keep_first : 0;
+    const A4Plan p = a4_plan(len, pos0, n_seg, K, G, hs, f32, window, keep, most_rows, max_kv);
+    if (p.row_blocks < 1) return XR_OK;
+    if ((long long)K * p.row_blocks > 65535) return XR_ERR_ARG;
+    const long long items = (long long)n_seg * K * p.row_blocks * p.splits, rb = a4_rows(f32, p.wide);
+    if (p.splits > 1 && (scratch == nullptr || ((uintptr_t)scratch & 15) || floats < items * rb * (hs + 2))) return XR_ERR_ARG;
+    A4Args a{q, out, kv4_cache(cache, n_pages, layers, layer, K, page_size, D), seg_start, seg_len, seg_pos0, block_tables, scratch,
+             scratch + items * rb * hs, status, q_stride, H, G, D, max_pages, window, keep, p.splits, p.span_tiles, p.row_blocks, most_rows,
+             scale, softcap, sink, {bias, bias_len}, 0, 0, -1};
+    a.wide = D % 8 == 0 && q_stride % 8 == 0 && !((uintptr_t)q & 15);
+    a.wide_out = D % 4 == 0 && !((uintptr_t)out & 15);
+    const int tile = a4_tile(hs);
+    if (page_size % tile == 0 && ((page_size / tile) & (page_size / tile - 1)) == 0)
+        for (a.tile_shift = 0; (tile << a.tile_shift) < page_size;) a.tile_shift++;
+    return hs == 64 ? a4_launch<2>(a, n_seg, f32, p.wide, stream) : hs == 128 ? a4_launch<4>(a, n_seg, f32, p.wide, stream) : a4_launch<8>(a, n_seg, f32, p.wide, stream);
+}

@@ -477,7 +477,8 @@ def tc_check_status(device: torch.device) -> None:
         if code != 0:
             ws.status.zero_()
             ws.flags.zero_()                  # a launch that gave up may have left some raised
-            what = {1: "a tcgen05 product", 2: "the bulk-copy decode attention", 3: "the tcgen05 attention", 4: "the tcgen05 attention (shared memory not 1 KB aligned)"}.get(code, "a kernel")
+            what = {1: "a tcgen05 product", 2: "the bulk-copy decode attention", 3: "the tcgen05 attention", 4: "the tcgen05 attention (shared memory not 1 KB aligned)",
+                    5: "the attention over a cache in four bits"}.get(code, "a kernel")
             raise KernelError(f"{what} gave up waiting on a barrier; its output is not valid")
 
 
@@ -733,6 +734,199 @@ def attention_tc(qkv: torch.Tensor, out: torch.Tensor, seg_start, seg_len, seg_p
                                  H, K, hd, max_pages, page_size, window, float(scale), max_seg_len, row_tiles, group[1], group[2],
                                  group[3], _ptr(sink), float(softcap), int(keep_first), _ptr(bias), _bias_len(bias), _stream()), "attention_tc")
     _count()
+
+
+# ---------------------------------------------------------------------------
+# A cache in four bits (csrc/kv4.cuh has the format; csrc/kv4.cu, csrc/attention_kv4.cu)
+KV4_GROUP = 32             # neighbouring elements of a head that share a scale
+
+
+def kv4_held(head_dim: int) -> int:
+    """Elements that a head of `head_dim` is held as."""
+    if not 1 <= head_dim <= 256:
+        raise KernelError(f"a cache in four bits holds heads of 1 to 256 elements, not {head_dim}")
+    return 64 if head_dim <= 64 else 128 if head_dim <= 128 else 256
+
+
+def kv4_block_bytes(head_dim: int, page_size: int) -> int:
+    """Bytes of one page, layer and kv head: codes of keys and values, then their scales."""
+    if page_size < 8 or page_size % 8 or page_size > 65536:
+        raise KernelError(f"a cache in four bits has pages of a multiple of 8 tokens, 8 to 65,536, not {page_size}")
+    hs = kv4_held(head_dim)
+    return page_size * (hs + hs // 8)
+
+
+def kv4_cache(pages: int, layers: int, kv_heads: int, head_dim: int, page_size: int, device) -> torch.Tensor:
+    """A cache in four bits, all zeros: uint8 [pages, layers, kv heads, block]."""
+    return torch.zeros((pages, layers, kv_heads, kv4_block_bytes(head_dim, page_size)), dtype=torch.uint8, device=device)
+
+
+def _on_current(*ts) -> None:
+    if any(t is not None and not t.is_cuda for t in ts):
+        raise KernelError("kernel arguments must lie on the current CUDA device")
+    here = _raw_device() if _raw_device is not None else torch.cuda.current_device()
+    if any(t is not None and t.device.index != here for t in ts):
+        raise KernelError("kernel arguments must lie on the current CUDA device")
+
+
+def _kv4_args(cache: torch.Tensor, layer: int, page_size: int, head_dim: int):
+    """The arguments by which a launcher knows a cache: address, pages, layers, layer, kv heads, block, tokens a page."""
+    if cache.dtype != torch.uint8 or cache.dim() != 4 or not cache.is_contiguous():
+        raise KernelError("a cache in four bits is a contiguous uint8 array [pages, layers, kv heads, block]")
+    if cache.shape[3] != kv4_block_bytes(head_dim, page_size) or not 0 <= layer < cache.shape[1]:
+        raise KernelError(f"this cache has blocks of {cache.shape[3]} bytes and {cache.shape[1]} layers: not one for heads of {head_dim} in pages of "
+                          f"{page_size}, layer {layer}")
+    return cache.data_ptr(), cache.shape[0], cache.shape[1], int(layer), cache.shape[2], cache.shape[3], int(page_size)
+
+
+def _ints(n: int, **ts) -> None:
+    for name, t in ts.items():
+        if t.dtype != torch.int32 or t.numel() < n or not t.is_contiguous():
+            raise KernelError(f"{name}: {n} int32 values, one after another, are wanted")
+
+
+def _tables(block_tables: torch.Tensor):
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or not block_tables.is_contiguous() or block_tables.numel() == 0:
+        raise KernelError("block tables are int32 [requests, pages], one row after another")
+    return block_tables.shape
+
+
+def kv4_store(k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, tok_seg: torch.Tensor, block_tables: torch.Tensor, cache: torch.Tensor, layer: int,
+              page_size: int) -> None:
+    """Quantise rows of keys k [n, kv heads * D] and values v [n, kv heads * Vd] (bfloat16 or float32, strided by rows, as they are to be
+    cached) into the pages: row t is position positions[t] of the request of row tok_seg[t] of the block tables.  `cache`: ``kv4_cache`` for heads
+    of max(D, Vd).  Tokens whose page is not held (an entry below zero or not of this cache, a position beyond the table) are not written; a
+    position may be given once in a call."""
+    K = cache.shape[2] if cache.dim() == 4 else 0
+    n = k.shape[0] if k.dim() == 2 else -1
+    if K < 1 or k.dim() != 2 or v.dim() != 2 or v.shape[0] != n or k.shape[1] % K or v.shape[1] % K or not k.shape[1] or not v.shape[1]:
+        raise KernelError("k and v are [tokens, kv heads * elements], with the cache's kv heads")
+    if k.dtype != v.dtype or k.stride(1) != 1 or v.stride(1) != 1:
+        raise KernelError("k and v have one type, and neighbouring elements lie side by side")
+    n_seg, max_pages = _tables(block_tables)
+    _ints(n, positions=positions, tok_seg=tok_seg)
+    _on_current(k, v, positions, tok_seg, block_tables, cache)
+    D, Vd = k.shape[1] // K, v.shape[1] // K
+    args = _kv4_args(cache, layer, page_size, max(D, Vd))
+    code = dtype_code(k.dtype)
+    if n == 0:
+        return
+    _check(_c.xr_kv4_store(k.data_ptr(), v.data_ptr(), code, max(k.stride(0), K * D), max(v.stride(0), K * Vd), positions.data_ptr(), tok_seg.data_ptr(),
+                           block_tables.data_ptr(), *args, n, D, Vd, n_seg, max_pages, _stream()), "kv4_store")
+    _count()
+
+
+def kv4_read(cache: torch.Tensor, layer: int, page_size: int, block_tables: torch.Tensor, first: torch.Tensor, end: torch.Tensor, out: torch.Tensor,
+             keep_first: int = 0, tables: Optional[torch.Tensor] = None) -> None:
+    """The rows first[r] .. end[r] - 1 of every request r (a row of the block tables), and with `keep_first` its first rows where they lie ahead
+    of those, as the values they are held as: out [pages, 2, kv heads, page_size, D] in bfloat16 (exact) or float32, the requests' pages one after another,
+    each request's kept pages ahead of the others.  Rows of these pages that are not asked for, or whose page is not held, are zeros; pages of
+    `out` behind the last are left as they were.  `tables` (int32, the block tables' shape): receives where a page lies in `out`; entries of
+    pages that are not there are left."""
+    if out.dim() != 5 or out.shape[1] != 2 or out.shape[3] != page_size or not out.is_contiguous() or cache.dim() != 4 or out.shape[2] != cache.shape[2]:
+        raise KernelError("out is [pages, 2, kv heads, page_size, elements], one page after another")
+    n_seg, max_pages = _tables(block_tables)
+    _ints(n_seg, first=first, end=end)
+    if tables is not None and (tables.shape != block_tables.shape or tables.dtype != torch.int32 or not tables.is_contiguous()):
+        raise KernelError("tables has the block tables' shape and type")
+    if keep_first < 0:
+        raise KernelError(f"keep_first {keep_first}")
+    _on_current(cache, block_tables, first, end, out, tables)
+    args = _kv4_args(cache, layer, page_size, out.shape[4])
+    code = dtype_code(out.dtype)
+    if out.shape[0] == 0:
+        return
+    _check(_c.xr_kv4_read(*args, block_tables.data_ptr(), first.data_ptr(), end.data_ptr(), out.data_ptr(), code, _ptr(tables), n_seg, max_pages,
+                          out.shape[4], int(keep_first), out.shape[0], _stream()), "kv4_read")
+    _count()
+
+
+KV4_SHORT_ROWS = 64        # packed rows (tokens x query heads per kv head) up to which a portion attends to the codes themselves
+_KV4_ALL_ROWS = 1 << 30
+
+
+def kv4_pages_read(seg_len, seg_pos0, page_size: int, window: int, keep_first: int) -> int:
+    """Pages that ``kv4_read`` writes for the rows that these portions (numpy, on the host) see."""
+    import numpy as np
+    pos, end = seg_pos0.astype(np.int64), seg_pos0.astype(np.int64) + seg_len
+    first = np.maximum(0, pos - window + 1) if window > 0 else np.zeros_like(pos)
+    kept = np.minimum(-(-keep_first // page_size), first // page_size) if window > 0 else 0
+    return int((kept + (end - 1) // page_size - first // page_size + 1)[seg_len > 0].sum())
+
+
+def attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, layer: int, page_size: int, seg_start: torch.Tensor, seg_len: torch.Tensor,
+                  seg_pos0: torch.Tensor, block_tables: torch.Tensor, heads: int, head_dim: int, scale: float, lengths: tuple, window: int = 0,
+                  sink: Optional[torch.Tensor] = None, softcap: float = 0.0, keep_first: int = 0, bias: Optional[torch.Tensor] = None, max_kv_len: int = 0,
+                  buf=None) -> None:
+    """Causal attention of every token of the step over its request's rows of a cache in four bits, its own row included.  q [n, >= heads *
+    head_dim] (bfloat16 or float32, strided by rows), out [n, heads * head_dim]; portion s is the seg_len[s] rows from seg_start[s] on, at positions
+    seg_pos0[s] .., over row s of the block tables.  `lengths` = (seg_len, seg_pos0) on the host (numpy int32): they size the launches; a call
+    that is captured in a graph may be replayed with other positions (say in `max_kv_len` how long the requests may get, so that the cut suits
+    them) but the same seg_len.  Rows on a page that is not held count as zeros.  Options: see ``attention_simt``.
+    Single tokens, short portions and whatever the prompt kernels do not take attend to the codes; portions of more than KV4_SHORT_ROWS packed rows read the
+    rows they see back into `buf` (``buf(name, shape, dtype)`` gives scratch; None: allocated) and go through the prompt kernels."""
+    K = cache.shape[2] if cache.dim() == 4 else 0
+    if K < 1 or heads < 1 or heads % K:
+        raise KernelError(f"{heads} query heads on {K} kv heads")
+    n_seg, max_pages = _tables(block_tables)
+    _ints(n_seg, seg_start=seg_start, seg_len=seg_len, seg_pos0=seg_pos0)
+    n = out.shape[0]
+    if out.dim() != 2 or out.shape[1] != heads * head_dim or not out.is_contiguous() or q.dim() != 2 or q.shape[0] != n or q.shape[1] < heads * head_dim or \
+            q.stride(1) != 1 or q.dtype != out.dtype:
+        raise KernelError("q and out are rows of the same tokens in one type, out [tokens, heads * elements]")
+    h_len, h_pos = lengths
+    if any(str(a.dtype) != "int32" or a.shape != (n_seg,) or not a.flags["C_CONTIGUOUS"] for a in (h_len, h_pos)):
+        raise KernelError("lengths: two int32 numpy arrays, one value a portion")
+    if int(h_len.sum()) > n or int(h_len.min()) < 0 or int(h_pos.min()) < 0:
+        raise KernelError("lengths: portions that q does not hold, or positions below zero")
+    if window < 0 or keep_first < 0 or not scale > 0 or not softcap >= 0 or (bias is not None and softcap > 0):
+        raise KernelError("window and keep_first are not negative, the scale is positive, a bias goes without a cap")
+    if sink is not None and (sink.dtype != torch.float32 or sink.numel() != heads or not sink.is_contiguous()):
+        raise KernelError("sink: one float32 logit a query head")
+    _check_bias(bias, heads)
+    _on_current(q, out, cache, seg_start, seg_len, seg_pos0, block_tables, sink, bias)
+    args = _kv4_args(cache, layer, page_size, head_dim)
+    code = dtype_code(q.dtype)
+    G = heads // K
+    rows = h_len.astype("int64") * G
+    if buf is None:
+        buf = lambda name, shape, dtype: torch.empty(shape, dtype=dtype, device=out.device)
+    q_stride = max(q.stride(0), heads * head_dim)
+    most = _KV4_ALL_ROWS
+    aligned = q.dtype == torch.bfloat16 and q_stride % 8 == 0 and q.data_ptr() % 16 == 0
+    tc = aligned and attention_tc_supported(q.dtype, heads, K, head_dim, page_size)
+    if aligned and (tc or (head_dim % 16 == 0 and head_dim <= 128 and out.data_ptr() % 16 == 0)):
+        most = KV4_SHORT_ROWS
+    longer = rows > most
+    if longer.any():
+        len_long = h_len * longer
+        pages = kv4_pages_read(len_long, h_pos, page_size, window, keep_first)
+        ints = buf("kv4_portions", (3 * n_seg + block_tables.numel(),), torch.int32)
+        first, end, long_len, tables = ints[:n_seg], ints[n_seg:2 * n_seg], ints[2 * n_seg:3 * n_seg], ints[3 * n_seg:].view(n_seg, max_pages)
+        values = buf("kv4_values", (pages, 2, K, page_size, head_dim), torch.bfloat16)
+        _check(_c.xr_kv4_long(seg_len.data_ptr(), seg_pos0.data_ptr(), first.data_ptr(), end.data_ptr(), long_len.data_ptr(), tables.data_ptr(), n_seg,
+                              max_pages, G, int(window), most, _stream()), "attention_kv4")
+        _check(_c.xr_kv4_read(*args, block_tables.data_ptr(), first.data_ptr(), end.data_ptr(), values.data_ptr(), BF16, tables.data_ptr(), n_seg,
+                              max_pages, head_dim, int(keep_first), pages, _stream()), "attention_kv4")
+        _count(2)
+        half = K * page_size * head_dim
+        longest = int(len_long.max())
+        if tc:
+            attention_tc(q, out, seg_start, long_len, seg_pos0, tables, (values.data_ptr(), pages, 1, 0), heads, K, head_dim, max_pages, page_size, window,
+                         scale, n_seg, longest, row_tiles=long_row_tiles(len_long, G, 128), sink=sink, softcap=softcap, keep_first=keep_first, bias=bias)
+        else:
+            attention_mma(q, q_stride, out, values.data_ptr(), seg_start, long_len, seg_pos0, tables, None, None, 2 * half, half, heads, K, head_dim,
+                          max_pages, page_size, window, scale, n_seg, longest, int((h_pos + len_long).max()), 0, False, True,
+                          row_tiles=long_row_tiles(len_long, G, 64), sink=sink, softcap=softcap, keep_first=keep_first, bias=bias)
+    if not longer.all():
+        floats = int(_c.xr_kv4_attention_floats(h_len.ctypes.data, h_pos.ctypes.data, n_seg, K, G, head_dim, code, int(window), int(keep_first), most,
+                                                int(max_kv_len)))
+        scratch = buf("kv4_spans", (floats,), torch.float32) if floats else None
+        _check(_c.xr_kv4_attention(q.data_ptr(), out.data_ptr(), code, *args, seg_start.data_ptr(), seg_len.data_ptr(), seg_pos0.data_ptr(),
+                                   block_tables.data_ptr(), h_len.ctypes.data, h_pos.ctypes.data, _ptr(scratch), floats, workspace(out.device).status_ptr,
+                                   q_stride, n_seg, heads, head_dim, max_pages, int(window), float(scale), _ptr(sink), float(softcap), int(keep_first),
+                                   _ptr(bias), _bias_len(bias), most, int(max_kv_len), _stream()), "attention_kv4")
+        _count(2 if floats else 1)
 
 
 FLAT_TILE = 128       # the flat array's first key of a portion is a multiple of this
