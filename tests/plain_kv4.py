@@ -97,3 +97,16 @@ def tolerance(out, size, raw, D, dtype):
     d = raw * ((hs + 8) * 2.0 ** -23) + raw * 2.0 ** -21 + 2.0 ** -20
     half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -23
     return (4 * d[..., None] + half) * size + half * out.abs() + 1e-30
+
+
+def quantised_rows(x):
+    """The values that rows x [..., D] are held as, all at once (float64, on x's device)."""
+    D = x.shape[-1]
+    g = torch.nn.functional.pad(x.double(), (0, held(D) - D)).reshape(*x.shape[:-1], -1, 32)
+    hi, lo = g.amax(-1), g.amin(-1)
+    e = torch.where(hi >= -lo, hi, lo)
+    m, ex = torch.frexp(e)
+    s = -torch.ldexp(torch.round(m * 32.0), ex - 5) / 8.0
+    s = torch.where(e.abs() < 2.0 ** -96, torch.zeros_like(s), s)
+    c = torch.round(g / torch.where(s == 0, torch.ones_like(s), s)[..., None]).clamp(-8, 7) * (s != 0)[..., None]
+    return (c * s[..., None]).reshape(*x.shape[:-1], -1)[..., :D]

@@ -94,3 +94,23 @@ def test_pages_that_are_read():
     assert kernels.kv4_pages_read(a(0, 20), a(7, 15), 16, 0, 0) == 3
     assert kernels.kv4_pages_read(a(1), a(100), 16, 10, 20) == 2 + 2           # rows 91 .. 100 lie in pages 5 and 6, the kept in 0 and 1
     assert kernels.kv4_pages_read(a(1), a(40), 16, 20, 33) == 1 + 2            # kept rows that the window's pages hold are not there twice
+
+
+def test_engine_refuses_before_it_looks_for_a_device():
+    from xyntetik_runner_b200.engine.engine import Engine, EngineParams
+    with pytest.raises(ValueError, match="same or int4"):
+        Engine("nowhere", EngineParams(kv="q8_0"))
+    with pytest.raises(ValueError, match="multiple of 8"):
+        Engine("nowhere", EngineParams(kv="int4", page_size=20))
+
+
+def test_bytes_of_a_token():
+    from xyntetik_runner_b200.engine.model import kv_head_bytes
+    from xyntetik_runner_b200.parts.base import KVNeed
+    assert kv_head_bytes(KVNeed(8, 128, four_bits=True), 2, True) == 144 and kv_head_bytes(KVNeed(8, 128, four_bits=True), 2, False) == 512
+    assert kv_head_bytes(KVNeed(1, 576, planes=1), 2, True) == 1152 and kv_head_bytes(KVNeed(1, 40, four_bits=True), 4, True) == 72
+
+
+def test_option():
+    from xyntetik_runner_b200 import cli
+    assert cli.build_parser().parse_args(["-m", "x"]).kv == "same" and cli.build_parser().parse_args(["-m", "x", "--kv", "int4"]).kv == "int4"

@@ -1,0 +1,220 @@
+"""An engine whose cache is in four bits against an engine that keeps rows in the activations' type and whose pages are quantised by the plain form
+between store and attention; steps in graphs and without, cut in every way; generation through the entry points."""
+import json
+import math
+import os
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+import plain_kv4
+
+pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+DENSE = {"kind": "dense", "ff": 64}
+MOE = {"kind": "moe", "router": {"experts": 2, "top": 2}, "expert": {"ff": 64}, "shared": {"ff": 64}}
+
+
+def llama(head_dim=64, heads=8, kv_heads=2, layers=2, window=None):
+    d = {"architectures": ["LlamaForCausalLM"], "hidden_size": 256, "num_hidden_layers": layers, "num_attention_heads": heads,
+         "num_key_value_heads": kv_heads, "head_dim": head_dim, "intermediate_size": 320, "vocab_size": 300, "rms_norm_eps": 1e-5, "rope_theta": 10000.0,
+         "max_position_embeddings": 4096, "tie_word_embeddings": False, "torch_dtype": "bfloat16"}
+    return d
+
+
+def besolix():
+    """Attention with a norm a head, values of another size, a window; the latent layer keeps its rows as they are."""
+    at = dict(heads=4, kv_heads=2, dim=64, vdim=48, scale=0.15, rot={"base": 10000.0, "dims": 32}, mask={"size": 70})
+    la = dict(heads=2, dim=32, rot_dim=16, vdim=32, kv_rank=64, q_rank=48, scale=0.15, rot={"base": 10000.0, "dims": 16}, mask={"size": 90})
+    return {"architecture": "Besolix", "vocab": 300, "width": 128, "norm": {"eps": 1e-5},
+            "layers": [{"type": "attention", "mlp": DENSE, "mixer": at}, {"type": "latent_attention", "mlp": DENSE, "mixer": la},
+                       {"type": "attention", "mlp": DENSE, "mixer": dict(at, dim=128, vdim=128, rot={"base": 10000.0, "dims": 128})}]}
+
+
+def tiny(module, name):
+    import importlib
+    return importlib.import_module("tiny_" + module).CONFIGS[name]
+
+
+def semesun():
+    """Windows with kept first keys, a bias by distance, values that layers share."""
+    import tiny_semesun as t
+    return t.clean(t.model(160, 128, 1e-5, [t.layer(t.attention(4, 2, 64, 64, 0.12, 70, 5, 48, 32, True), DENSE),
+                                            t.layer(t.attention(2, 1, 128, 128, 0.09, 130, 140, 200, 32, True), DENSE),
+                                            t.layer(t.attention(16, 2, 64, 48, 0.15, 33, 1, 20, 32), None),
+                                            t.layer(t.attention(3, 3, 24, 20, 0.2, None, 0, 90, 32), DENSE)]))
+
+
+MODELS = {"llama64": llama, "llama128": lambda: llama(128, 6, 2), "llama100": lambda: llama(100, 3, 1), "mqa": lambda: llama(64, 18, 1),
+          "besolix": besolix, "pitolix": lambda: tiny("pitolix", "mix"), "buzarax": lambda: tiny("buzarax", "mix"), "semesun": semesun,
+          "lilalorn": lambda: tiny("lilalorn", "mix")}
+
+
+def engine(model, dtype, kv, page_size=16, graphs=True, requests=4, max_tokens=2048):
+    from xyntetik_runner_b200 import architectures  # noqa: F401
+    from xyntetik_runner_b200.config import registry
+    from xyntetik_runner_b200.engine.engine import EngineParams, random_engine
+    c = MODELS[model]()
+    arch = registry.resolve(registry.architecture_name(c))
+    return random_engine(arch.config_from_dict(c), 7, EngineParams(dtype=dtype, max_tokens=max_tokens, page_size=page_size, max_requests=requests,
+                                                                   max_request_tokens=512, max_step_tokens=512, cuda_graphs=graphs, kv=kv), std=0.08)
+
+
+STEPS = [  # request -> tokens of each step
+    {"a": 1, "b": 37}, {"a": 5, "b": 1, "c": 90}, {"a": 1, "b": 1, "c": 1}, {"a": 1, "b": 1, "c": 1}, {"a": 1, "b": 1, "c": 1}, {"b": 3, "c": 64}, {"a": 1, "c": 1}]
+
+
+def run(eng, steps=STEPS, vocab=250):
+    from xyntetik_runner_b200.engine.engine import StepEntry
+    rng = np.random.RandomState(3)
+    out = []
+    for st in steps:
+        entries = [StepEntry(r, [int(t) for t in rng.randint(0, vocab, n)], list(range(n))) for r, n in st.items()]
+        out.append(eng.step(entries).clone())
+    eng.check_status()
+    return out
+
+
+def quantise_pages(eng, monkeypatch):
+    """Before every attention of this engine, all rows in its pages become the values that four bits hold (which leaves values that are held already as
+    they are)."""
+    from xyntetik_runner_b200 import kernels
+
+    def behind(fn):
+        def call(*a, **k):
+            for t, g in zip(eng.kv, eng.model.groups):
+                if g.four_bits:
+                    t.copy_(plain_kv4.quantised_rows(t).to(t.dtype))
+            return fn(*a, **k)
+        return call
+    for name in ("attention_simt", "attention_mma", "attention_tc"):
+        monkeypatch.setattr(kernels, name, behind(getattr(kernels, name)))
+
+
+def rows_of(eng, request):
+    return [torch.stack(eng.cached_rows(request, lay.entry)) for lay in eng.model.layers if lay.group >= 0 and eng.model.groups[lay.group].four_bits and lay.writes_cache]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("model", list(MODELS))
+def test_engine_against_quantised_pages(model, dtype, monkeypatch):
+    """Rows: the first layer's are those of the plain form, bit for bit; the others' differ where a rounding ahead of them took a value to the other side of a
+    border between two codes (float32: none to a few in 100,000).  Logits: as near as the arithmetic is where no row differs."""
+    from xyntetik_runner_b200.parts import attention
+    eng = engine(model, dtype, "int4")
+    vocab = min(250, eng.plan.vocab_size)
+    before = attention.counters["kv4"]
+    got = run(eng, vocab=vocab)
+    assert attention.counters["kv4"] > before and any(eng.four_bits)
+    rows = {r: rows_of(eng, r) for r in "abc"}
+    ref = engine(model, dtype, "same", graphs=False)
+    with monkeypatch.context() as m:
+        quantise_pages(ref, m)
+        want = run(ref, vocab=vocab)
+    differ = total = 0
+    for r in "abc":
+        for i, (x, y) in enumerate(zip(rows[r], rows_of(ref, r))):
+            assert x.shape == y.shape and x.abs().max() > 0
+            if i == 0 and model.startswith(("llama", "mqa")):
+                assert torch.equal(x, y)                             # (the first layer's input is the embedding)
+            differ += int((x != y).sum())
+            total += x.numel()
+            assert float((x - y).abs().max()) <= 0.6 * float(y.abs().max())
+    assert differ <= (1e-4 if dtype == "float32" else 0.1) * total, f"{differ} of {total}"
+    for a, b in zip(got, want):
+        scale, off = float(b.abs().max()), float((a - b).abs().max())
+        if dtype == "float32":
+            assert off <= (1e-4 if differ == 0 else 0.02) * scale, f"{off / scale:.3g}"
+        else:
+            # bfloat16 activations differ by their rounding, and a value near a border between two codes may fall on its other side: one step, an eighth of
+            # its group's largest magnitude, 0.31 of the values' size where that is 2.5 of it (32 normal values: 2.2 on average).  A share f of such values is
+            # an error of 0.31 sqrt(f) in keys and in values of every layer, independent of one another; beside it 2^-6 for the roundings
+            # of the products, norms and weights along two to four layers.
+            rel = float((a - b).norm() / b.norm())
+            most = 2.0 ** -6 + 0.31 * math.sqrt(differ / total * 2 * len(rows["a"]))
+            assert off <= 0.1 * scale and rel <= most, f"{rel:.3g} of {most:.3g}, {differ} of {total}"
+
+
+def test_first_layers_rows_are_the_plain_forms():
+    """What four bits hold of the rows that an engine without them keeps."""
+    for dtype in ("float32", "bfloat16"):
+        four, same = engine("llama64", dtype, "int4"), engine("llama64", dtype, "same")
+        run(four), run(same)
+        for r in "abc":
+            for x, y in zip(four.cached_rows(r, 0), same.cached_rows(r, 0)):
+                n = y.shape[0] * y.shape[1]
+                assert torch.equal(x.double().cpu().reshape(n, -1), plain_kv4.quantised(y.reshape(n, -1))[2])
+
+
+@pytest.mark.parametrize("model", ["llama64", "semesun"])
+def test_graphs_and_plain_steps_give_the_same_bits(model):
+    steps = [{"a": 40, "b": 7}] + [{"a": 1, "b": 1}] * 6
+    a, b = engine(model, "bfloat16", "int4", graphs=True), engine(model, "bfloat16", "int4", graphs=False)
+    x, y = run(a, steps), run(b, steps)
+    if a._graph_ok:
+        assert a.graph_replays > 0
+    assert all(torch.equal(p, q) for p, q in zip(x, y))
+
+
+def test_cutting_a_request_changes_little():
+    """A prompt in one portion (read back for the prompt kernel), in portions that attend to the codes, token by token: the same rows in the cache, the same
+    logits within the activations' rounding."""
+    for dtype, tol in (("float32", 1e-4), ("bfloat16", 0.05)):
+        ref = None
+        for cut in ([96], [40, 56], [16] * 6, [5] * 19 + [1], [1] * 96):
+            eng = engine("llama64", dtype, "int4")
+            x = torch.cat(run(eng, [{"a": n} for n in cut]))
+            rows = rows_of(eng, "a")
+            if ref is None:
+                ref = (x, rows)
+            scale = float(ref[0].abs().max())
+            assert float((x - ref[0]).abs().max()) <= tol * scale
+            assert torch.equal(rows[0], ref[1][0])
+
+
+def test_a_window_gives_pages_back_and_reads_zeros():
+    eng = engine("besolix", "bfloat16", "int4")
+    run(eng, [{"a": 120}] + [{"a": 1}] * 60)
+    free = [p.n_free for p in eng.cache.pools]
+    assert max(free) > 0
+    k, v = eng.cached_rows("a", 0)
+    assert k.shape[0] == 180 and not k[:64].any() and k[-70:].abs().amax(dim=(1, 2)).min() > 0
+    eng.end("a")
+    eng.cache.audit()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_generate_and_score(dtype):
+    """Through the runner: many requests in a small pool give every request the tokens that it gets alone; a score."""
+    from xyntetik_runner_b200 import Runner
+    from xyntetik_runner_b200.config import registry
+    c = llama()
+    cfg = registry.resolve(registry.architecture_name(c)).config_from_dict(c)
+    rng = np.random.RandomState(2)
+    prompts = [[int(t) for t in rng.randint(0, 300, n)] for n in (3, 70, 150, 12)]
+    r = Runner(config=cfg, random_seed=3, dtype=dtype, ctx=256, batch=96, parallel=4, kv="int4", page_size=32)
+    together = r.generate(prompts, n=12, ignore_eos=True)
+    assert all(len(x.tokens) == 12 for x in together)
+    if dtype == "float32":
+        for p, x in zip(prompts, together):
+            assert r.generate(p, n=12, ignore_eos=True).tokens == x.tokens
+    lp = r.score(prompts[1])
+    assert len(lp) == 69 and all(np.isfinite(lp))
+    same = Runner(config=cfg, random_seed=3, dtype=dtype, ctx=256, batch=96, parallel=4, page_size=32)
+    assert np.corrcoef(lp, same.score(prompts[1]))[0, 1] > 0.9       # four bits are near what they hold
+    assert r.engine.kv_bytes_per_token() * 3.5 < same.engine.kv_bytes_per_token()
+    assert r.engine.kv_bytes_per_token() == 2 * 2 * 72
+
+
+def test_command_line(tmp_path):
+    path = tmp_path / "m"
+    path.mkdir()
+    (path / "config.json").write_text(json.dumps(llama()))
+    cmd = [sys.executable, "-m", "xyntetik_runner_b200", "-m", str(path), "--random", "5", "-p", "ids:1,5,9", "-n", "5", "--ignore-eos", "-c", "128", "--kv", "int4"]
+    a = subprocess.run(cmd, cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert a.returncode == 0, a.stderr
+    assert a.stdout.startswith("ids:") and len(a.stdout.split("\n")[0].split(",")) == 5

@@ -220,7 +220,7 @@ def test_attention(contexts, T, H, K, D, P, dtype, window, keep, sink, cap, bias
     args, q, held, plain, Ts, starts, pos0 = attention_case(contexts, T, H, K, D, P, dtype, window, keep, sink, cap, bias)
     wide = torch.zeros(q.shape[0], H * D + 24, dtype=dtype, device=DEV)          # q's rows lie in wider ones
     wide[:, :H * D] = q.to(DEV)
-    for rows in (q.to(DEV), wide):
+    for rows in (q.to(DEV), wide, wide[:, :H * D]):
         out = torch.full((q.shape[0] + 3, H * D), 9.0, dtype=dtype, device=DEV)
         kernels.attention_kv4(rows, out[:q.shape[0]], **args)
         kernels.tc_check_status(torch.device(DEV))

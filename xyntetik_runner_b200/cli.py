@@ -4,7 +4,7 @@ Options keep the reference's names and meanings where it has them: -m (here a mo
 config.json and model.safetensors), -p, -f, -n (default 256, -1 = until a stop id), -c, -b, -s (0 is
 refused), --temp (0 = greedy), --top-k, --top-p, --min-p, --repeat-penalty, --ignore-eos, --no-bos,
 --score (teacher-forced log-probabilities of the prompt, the reference's JSON), --parallel, --rope-base, --rope-scale,
---bench-json (extended: --parallel sequences at once and a per-kernel table), -t, -v/--version; -c 0 fits the context
+--kv (same or int4: the cache's type), --bench-json (extended: --parallel sequences at once and a per-kernel table), -t, -v/--version; -c 0 fits the context
 to the free memory.  Where the reference has --gpu off to run its CPU code, --ref runs the plain implementation
 that the tests compare the engine with (greedy only; it is slow and is found only in a source checkout).  Tokenisation is outside the engine: a prompt is either ``ids:1,2,3`` (or a file of
 ids, --prompt-ids) or
@@ -77,6 +77,8 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--no-bos", action="store_true", help="do not prepend the BOS token")
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16",
                     help="bfloat16: serving kernels; float32: everything in true 32 bit")
+    ap.add_argument("--kv", choices=["same", "int4"], default="same",
+                    help="cached keys and values: same (as --dtype), or int4: four bits with a scale per 32 elements, where the mixer can")
     ap.add_argument("--page-size", type=int, default=64, help="tokens per cache page")
     ap.add_argument("--bench-json", action="store_true",
                     help="prefill 512-token prompts (--parallel of them at once), decode -n tokens each with stop ids ignored, "
@@ -181,7 +183,7 @@ def main(argv=None) -> int:
         print("error: --parallel needs N >= 1, --rope-base a positive base, --rope-scale a positive factor", file=sys.stderr)
         return 2
     runner = Runner(args.model, dtype=args.dtype, ctx=args.ctx, batch=args.batch, parallel=args.parallel,
-                    page_size=args.page_size, rope_base=args.rope_base, rope_scale=args.rope_scale)
+                    page_size=args.page_size, rope_base=args.rope_base, rope_scale=args.rope_scale, kv=args.kv)
     plan = runner.engine.plan
     print(f"loaded {args.model} in {time.perf_counter() - t0:.2f} s ({args.dtype})", file=sys.stderr)
     if args.bench_json:

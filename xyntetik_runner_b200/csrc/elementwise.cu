@@ -179,6 +179,18 @@ XR_EXPORT int xr_rmsnorm(const float* x, const int* rows, const float* w, void* 
 // The cache of a layer group is [page][layer][K|V][kv head][token in page][hd];
 // `cache_k` points at this layer's K block of page 0.
 // ---------------------------------------------------------------------------
+// Where token t's K heads go, and how far they lie apart: into its page, or with page_size 0 into rows, one a token, page_stride apart with
+// the heads side by side (another kernel takes them from there).
+template <typename T>
+__device__ __forceinline__ T* xr_store_row(void* cache_k, const int* block_tables, const int* tok_seg, int t, int pos, int max_pages, int page_size,
+                                           long long page_stride, int hd) {
+    if (cache_k == nullptr) return nullptr;
+    if (page_size == 0) return (T*)cache_k + (size_t)t * page_stride;
+    const int page = block_tables[(size_t)tok_seg[t] * max_pages + pos / page_size];
+    return (T*)cache_k + (size_t)page * page_stride + (size_t)(pos % page_size) * hd;
+}
+__device__ __forceinline__ size_t xr_store_step(int page_size, int hd) { return page_size == 0 ? (size_t)hd : (size_t)page_size * hd; }
+
 struct RopeStoreArgs {
     void* qkv;
     const int* positions;
@@ -204,12 +216,8 @@ __global__ void k_rope_store(RopeStoreArgs a) {
     T* row = (T*)a.qkv + (size_t)t * qkv_dim;
     const int pos = a.positions[t];
     const int half = a.rotary_dim >> 1;
-    T* kdst = nullptr;
-    if (a.cache_k != nullptr) {
-        int page = a.block_tables[(size_t)a.tok_seg[t] * a.max_pages + pos / a.page_size];
-        kdst = (T*)a.cache_k + (size_t)page * a.page_stride + (size_t)(pos % a.page_size) * a.hd;
-    }
-    const size_t head_step = (size_t)a.page_size * a.hd;          // between kv heads inside a page
+    T* kdst = xr_store_row<T>(a.cache_k, a.block_tables, a.tok_seg, t, pos, a.max_pages, a.page_size, a.page_stride, a.hd);
+    const size_t head_step = xr_store_step(a.page_size, a.hd);    // between kv heads inside a page
     // rotated pairs of the Q and K heads
     if (half > 0) {
         const int lanes = blockDim.x / half > 0 ? blockDim.x / half : 1;      // heads handled side by side
@@ -256,12 +264,8 @@ k_rope_store_vec(RopeStoreArgs a) {
     __nv_bfloat16* row = (__nv_bfloat16*)a.qkv + (size_t)t * qkv_dim;
     const int pos = a.positions[t];
     const int half = a.rotary_dim >> 1;
-    __nv_bfloat16* kdst = nullptr;
-    if (a.cache_k != nullptr) {
-        int page = a.block_tables[(size_t)a.tok_seg[t] * a.max_pages + pos / a.page_size];
-        kdst = (__nv_bfloat16*)a.cache_k + (size_t)page * a.page_stride + (size_t)(pos % a.page_size) * a.hd;
-    }
-    const size_t head_step = (size_t)a.page_size * a.hd;
+    __nv_bfloat16* kdst = xr_store_row<__nv_bfloat16>(a.cache_k, a.block_tables, a.tok_seg, t, pos, a.max_pages, a.page_size, a.page_stride, a.hd);
+    const size_t head_step = xr_store_step(a.page_size, a.hd);
     for (int j = threadIdx.x; j < half; j += blockDim.x) {
         float ang = (float)pos * a.inv_freq[j];
         rope_cs[j] = cosf(ang) * a.mscale;
@@ -320,7 +324,7 @@ XR_EXPORT int xr_rope_store(void* qkv, int dtype, const int* positions, const in
                             int n, int H, int K, int hd, int rotary_dim, int max_pages, int page_size,
                             int adjacent_pairs, float mscale, cudaStream_t stream) {
     if (n < 1 || H < 1 || K < 1 || hd < 1 || rotary_dim < 0 || rotary_dim > hd || (rotary_dim & 1) ||
-        page_size < 1 || H + 2 * K > 65535)
+        page_size < 0 || H + 2 * K > 65535)
         return XR_ERR_ARG;
     RopeStoreArgs a{qkv, positions, tok_seg, block_tables, inv_freq, cache_k, page_stride, v_offset,
                     n, H, K, hd, rotary_dim, max_pages, page_size, adjacent_pairs ? 1 : 0, mscale};
@@ -434,12 +438,8 @@ k_qk_norm_rope_store(QkNormStoreArgs a) {
             xr_sincos_angle((double)pos * a.freq[j], &cs[half + j], &cs[j]);
             cs[half + j] *= a.mscale; cs[j] *= a.mscale;
         }
-    T* kdst = nullptr;
-    if (a.cache_k != nullptr) {
-        const int page = a.block_tables[(size_t)a.tok_seg[t] * a.max_pages + pos / a.page_size];
-        kdst = (T*)a.cache_k + (size_t)page * a.page_stride + (size_t)(pos % a.page_size) * a.hd;
-    }
-    const size_t head_step = (size_t)a.page_size * a.hd;
+    T* kdst = xr_store_row<T>(a.cache_k, a.block_tables, a.tok_seg, t, pos, a.max_pages, a.page_size, a.page_stride, a.hd);
+    const size_t head_step = xr_store_step(a.page_size, a.hd);
     const float q_factor = a.q_every > 0 ? 1.0f + a.q_coef * logf((float)((pos + 1) / a.q_every) + 1.0f) : 1.0f;
     // A turn by an angle keeps a pair's sum of squares, and cosines and sines times mscale multiply it by mscale^2: the sum of
     // squares of the rotated head is that of the head as it is, the rotated elements weighted by mscale^2.
@@ -584,12 +584,8 @@ k_qk_norm_rope_store_vec(QkNormStoreArgs a) {
         cs[half + j] *= a.mscale; cs[j] *= a.mscale;
     }
     const float rot_weight = a.norm_after ? a.mscale * a.mscale : 1.0f;     // (see k_qk_norm_rope_store)
-    __nv_bfloat16* kdst = nullptr;
-    if (a.cache_k != nullptr) {
-        const int page = a.block_tables[(size_t)a.tok_seg[t] * a.max_pages + pos / a.page_size];
-        kdst = (__nv_bfloat16*)a.cache_k + (size_t)page * a.page_stride + (size_t)(pos % a.page_size) * a.hd;
-    }
-    const size_t head_step = (size_t)a.page_size * a.hd;
+    __nv_bfloat16* kdst = xr_store_row<__nv_bfloat16>(a.cache_k, a.block_tables, a.tok_seg, t, pos, a.max_pages, a.page_size, a.page_stride, a.hd);
+    const size_t head_step = xr_store_step(a.page_size, a.hd);
     const float q_factor = a.q_every > 0 ? 1.0f + a.q_coef * logf((float)((pos + 1) / a.q_every) + 1.0f) : 1.0f;
     const int v_at = (a.H + a.K) * a.D;
     Bf16x8* staged = reinterpret_cast<Bf16x8*>(qk_sm + ((2 * half + 3) & ~3));
@@ -705,7 +701,7 @@ XR_EXPORT int xr_qk_norm_rope_store(const void* in, int dtype, long long ld_in, 
     if (v_mix < 0 || v_mix > 2 || (v_mix != 0 && (v_first == nullptr || cache_k == nullptr || ((uintptr_t)v_first & 15)))) return XR_ERR_ARG;
     if (partial != nullptr && (splits < 1 || D > 256 || cols < (H + K) * D + K * Vd || cols > ld_in)) return XR_ERR_ARG;
     if (n < 1 || H < 1 || K < 1 || D < 1 || Vd < 1 || hd < D || hd < Vd || rotary_dim < 0 || rotary_dim > D || (rotary_dim & 1) ||
-        page_size < 1 || (rotary_dim > 0 && freq == nullptr) || (q_w == nullptr) != (k_w == nullptr) || q_every < 0 ||
+        page_size < 0 || (rotary_dim > 0 && freq == nullptr) || (q_w == nullptr) != (k_w == nullptr) || q_every < 0 ||
         (unit_norm && q_w != nullptr) || (norm_after && !unit_norm))
         return XR_ERR_ARG;
     const int pairs = !((D | hd | ld_in | q_ld | page_stride) & 1) && !(((uintptr_t)in | (uintptr_t)q_out | (uintptr_t)cache_k) & 3);

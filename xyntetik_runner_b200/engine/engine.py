@@ -45,6 +45,10 @@ class EngineParams:
     max_step_tokens: int = 8192        # sizing hint for the step's buffers (they grow if a step brings more)
     cuda_graphs: bool = True           # decode-only steps are captured once per (batch, context bucket) and replayed
     device: str = "cuda:0"
+    kv: str = "same"                   # cached keys and values: "same" (the activations' type), or "int4": four bits where the mixer can (csrc/kv4.cuh)
+
+
+KV_TYPES = ("same", "int4")
 
 
 @dataclass
@@ -130,6 +134,10 @@ class StepContext:
         """(pointer to this layer's K block of page 0, elements between pages, elements from K to V)."""
         return self._eng._cache_layer[lay.entry]
 
+    def cache_four_bits(self, lay: LayerRuntime) -> Optional[torch.Tensor]:
+        """The layer's cache group if it is kept in four bits (``kernels.kv4_cache``; the layer is lay.layer_in_group), else None."""
+        return self._eng.kv[lay.group] if self._eng.four_bits[lay.group] else None
+
     def cache_group(self, lay: LayerRuntime):
         """(pointer to the whole array of the layer's cache group, its pages, its layers, this layer's index)."""
         t = self._eng.kv[lay.group]
@@ -146,6 +154,13 @@ class Engine:
         if p.dtype not in _DTYPES:
             raise ValueError(f"dtype '{p.dtype}': choose bfloat16 or float32")
         self.act_dtype = _DTYPES[p.dtype]
+        if p.kv not in KV_TYPES:
+            raise ValueError(f"kv '{p.kv}': choose same or int4")
+        if p.kv == "int4":
+            try:
+                kernels.kv4_block_bytes(64, p.page_size)
+            except kernels.KernelError as e:
+                raise ValueError(f"kv int4: {e}") from None
         if not torch.cuda.is_available():
             raise RuntimeError("the engine runs on a CUDA device only; none is visible")
         self.device = torch.device(p.device)
@@ -169,14 +184,19 @@ class Engine:
                                   p.max_requests, max_req)
         # device arrays of keys and values: [page][layer in group][K|V (the group's planes)][kv head][token in page][head_dim].  One page
         # more than the pool hands out: the rows that fill a decode step up to a repeating size write there.
+        # Groups in four bits: [page][layer in group][kv head][the bytes of kv4.cuh].
         self.kv: List[torch.Tensor] = []
+        self.four_bits = [p.kv == "int4" and g.four_bits for g in self.model.groups]
         self._filler_page = n_pages
-        for g in self.model.groups:
+        for g, four_bits in zip(self.model.groups, self.four_bits):
+            if four_bits:
+                self.kv.append(kernels.kv4_cache(n_pages + 1, g.n_layers, g.kv_heads, g.head_dim, p.page_size, self.device))
+                continue
             self.kv.append(torch.zeros((n_pages + 1, g.n_layers, g.planes, g.kv_heads, p.page_size, g.head_dim),
                                        dtype=self.act_dtype, device=self.device))
         self._cache_layer: Dict[int, tuple] = {}
         for lay in self.model.layers:
-            if lay.group >= 0:
+            if lay.group >= 0 and not self.four_bits[lay.group]:
                 t = self.kv[lay.group]
                 es = t.element_size()
                 self._cache_layer[lay.entry] = (t.data_ptr() + lay.layer_in_group * t.stride(1) * es,
@@ -255,6 +275,26 @@ class Engine:
         self._open(request)
         self.cache.reserve(request, n_tokens)
         self.cache.commit(request)
+
+    def cached_rows(self, request, entry: int):
+        """(keys, values) that schedule entry `entry` holds of `request`, [tokens, kv heads, head size] in the activations' type: what its
+        queries read.  A cache in four bits is read back as the values it stands for; rows on pages that the window has let go are zeros."""
+        lay = self.model.layers[entry]
+        if lay.group < 0:
+            raise ValueError(f"schedule entry {entry} caches no keys and values")
+        g, P, n = self.model.groups[lay.group], self.params.page_size, self.cache.length(request)
+        if g.planes != 2:
+            raise ValueError(f"schedule entry {entry} caches one row a token, not keys and values")
+        table = torch.from_numpy(self.cache.block_table(lay.group, request)[None, :max(1, -(-n // P))].copy()).to(self.device)
+        if self.four_bits[lay.group]:
+            pages = torch.empty((-(-n // P), 2, g.kv_heads, P, g.head_dim), dtype=self.act_dtype, device=self.device)
+            span = torch.tensor([0, n], dtype=torch.int32, device=self.device)
+            kernels.kv4_read(self.kv[lay.group], lay.layer_in_group, P, table, span[:1], span[1:], pages)
+        else:
+            ids = table[0, :-(-n // P)].long()
+            pages = self.kv[lay.group][ids.clamp(min=0), lay.layer_in_group] * (ids >= 0).view(-1, 1, 1, 1, 1)
+        rows = pages.permute(1, 0, 3, 2, 4).reshape(2, -1, g.kv_heads, g.head_dim)
+        return rows[0, :n], rows[1, :n]
 
     def _open(self, request) -> int:
         slot = self.cache.open(request)
@@ -477,7 +517,7 @@ class Engine:
         return self.model.weight_bytes_per_step()
 
     def kv_bytes_per_token(self) -> int:
-        return self.model.kv_bytes_per_token(2 if self.act_dtype == torch.bfloat16 else 4)
+        return self.model.kv_bytes_per_token(2 if self.act_dtype == torch.bfloat16 else 4, self.params.kv == "int4")
 
 
 def random_engine(config, seed: int, params: EngineParams, std: float = 0.02, norm_jitter: float = 0.01,

@@ -16,6 +16,7 @@ from typing import Dict, List, Optional, Tuple
 
 import torch
 
+from .. import kernels
 from ..cache.pages import GroupSpec
 from ..parts.base import Block, KVNeed, Norm, Part, Runtime, StateNeed
 from ..parts.embedding import Embedding, Head
@@ -74,7 +75,7 @@ class ModelPlan:
                     raise ValueError(f"schedule entry {i}: cache_from must name an earlier entry that owns a cache")
                 a = self.blocks[e.layer].mixer.kv_need()
                 b = self.blocks[self.schedule[e.cache_from].layer].mixer.kv_need()
-                if a is None or b is None or (a.kv_heads, a.head_dim, a.planes) != (b.kv_heads, b.head_dim, b.planes):
+                if a is None or b is None or (a.kv_heads, a.head_dim, a.planes, a.four_bits) != (b.kv_heads, b.head_dim, b.planes, b.four_bits):
                     raise ValueError(f"schedule entry {i}: cannot read the cache of entry {e.cache_from} (geometry differs)")
 
 
@@ -95,6 +96,15 @@ class CacheGroupLayout:
     head_dim: int
     n_layers: int = 0
     planes: int = 2
+    four_bits: bool = False       # every mixer of the group can keep its rows in four bits
+
+
+def kv_head_bytes(need, elem_size: int, four_bits: bool) -> int:
+    """Bytes that a token takes a kv head and layer, by a ``KVNeed`` or a group: in elements of `elem_size` bytes, or with `four_bits` in four bits where the
+    mixer can."""
+    if four_bits and need.four_bits:
+        return kernels.kv4_block_bytes(need.head_dim, 8) // 8
+    return need.planes * need.head_dim * elem_size
 
 
 class LoadedModel:
@@ -110,7 +120,7 @@ class LoadedModel:
         self.groups: List[CacheGroupLayout] = []
         self.layers: List[LayerRuntime] = []
         self.state_needs: List[Tuple[int, StateNeed]] = []
-        keys: Dict[Tuple[int, int, Optional[int], int, int], int] = {}
+        keys: Dict[Tuple[int, int, Optional[int], int, int, bool], int] = {}
         for i, e in enumerate(plan.schedule):
             mixer = plan.blocks[e.layer].mixer
             lay = LayerRuntime(entry=i)
@@ -120,12 +130,12 @@ class LoadedModel:
                     src = self.layers[e.cache_from]
                     lay.group, lay.layer_in_group, lay.writes_cache = src.group, src.layer_in_group, False
                 else:
-                    key = (need.kv_heads, need.head_dim, need.window, need.planes, need.keep_first)
+                    key = (need.kv_heads, need.head_dim, need.window, need.planes, need.keep_first, need.four_bits)
                     if key not in keys:
                         keys[key] = len(self.groups)
                         name = "full" if need.window is None else f"window{need.window}" + (f"+{need.keep_first}" if need.keep_first else "")
                         self.groups.append(CacheGroupLayout(GroupSpec(f"{name}:{need.planes}x{need.kv_heads}x{need.head_dim}", need.window, need.keep_first),
-                                                            need.kv_heads, need.head_dim, planes=need.planes))
+                                                            need.kv_heads, need.head_dim, planes=need.planes, four_bits=need.four_bits))
                     g = keys[key]
                     lay.group, lay.layer_in_group, lay.writes_cache = g, self.groups[g].n_layers, True
                     self.groups[g].n_layers += 1
@@ -134,8 +144,9 @@ class LoadedModel:
                 self.state_needs.append((i, sn))
             self.layers.append(lay)
 
-    def kv_bytes_per_token(self, elem_size: int) -> int:
-        return sum(g.planes * g.kv_heads * g.head_dim * g.n_layers * elem_size for g in self.groups)
+    def kv_bytes_per_token(self, elem_size: int, four_bits: bool = False) -> int:
+        """`four_bits`: the groups that can be are kept in four bits."""
+        return sum(g.kv_heads * g.n_layers * kv_head_bytes(g, elem_size, four_bits) for g in self.groups)
 
     def weight_bytes_per_step(self) -> int:
         """Bytes of weights one step reads: every scheduled block once, the final norm and the head

@@ -17,6 +17,7 @@ import torch
 from .. import kernels
 from ..sampling.sampler import DeviceSampler, SamplingParams
 from .engine import Engine, EngineParams, StepEntry, random_engine
+from .model import kv_head_bytes
 from .scheduler import Request, Scheduler, SchedulerParams, StepPlan
 
 
@@ -110,13 +111,15 @@ class Runner:
                  dtype: str = "bfloat16", ctx: Optional[int] = None, batch: int = 2048, parallel: int = 8,
                  max_tokens: Optional[int] = None, page_size: int = 64, prefill_chunk: Optional[int] = None,
                  device: str = "cuda:0", engine: Optional[Engine] = None, rope_base: Optional[float] = None,
-                 rope_scale: Optional[float] = None):
+                 rope_scale: Optional[float] = None, kv: str = "same"):
         """model: folder with config.json + model.safetensors.  Or `config` (a typed configuration) with
         `random_seed` for seeded random weights.  ctx: longest request (default min(model limit, 4096), the
         reference's -c default, src/model.c:3075; 0: as long as the model allows and the free memory holds, its -c 0).  batch: token budget of a step (-b).  parallel: live
         requests.  max_tokens: tokens the page pool holds (default parallel * ctx).  rope_base: use this
         frequency base instead of the configuration's (--rope-base, src/model.c:282).  rope_scale: force linear
-        position scaling by this factor instead of the configuration's scaling (--rope-scale, src/model.c:324-326)."""
+        position scaling by this factor instead of the configuration's scaling (--rope-scale, src/model.c:324-326).
+        kv: "same" caches keys and values in the activations' type, "int4" in four bits with a scale per 32 elements (--kv; the
+        reference's quantised cache is --kv q8_0); mixers that keep other rows (latent attention) keep them as they are."""
         if engine is None:
             from ..config import registry
             if model is not None:
@@ -130,10 +133,10 @@ class Runner:
                 cfg = arch.override(cfg, rope_base=rope_base, rope_scale=rope_scale)
             model_limit = arch.build_plan(cfg).max_positions        # (parts only, no weights: cheap)
             if ctx == 0:
-                ctx = self._fit_context(arch, cfg, model_limit, parallel, page_size, dtype, device)
+                ctx = self._fit_context(arch, cfg, model_limit, parallel, page_size, dtype, device, kv)
             ctx = ctx or min(model_limit, 4096)
             ep = EngineParams(dtype=dtype, max_tokens=max_tokens or parallel * ctx, page_size=page_size,
-                              max_requests=parallel, max_request_tokens=ctx, max_step_tokens=batch, device=device)
+                              max_requests=parallel, max_request_tokens=ctx, max_step_tokens=batch, device=device, kv=kv)
             if model is not None and (rope_base is not None or rope_scale is not None):
                 from ..weights.loader import FolderSource
                 engine = Engine(params=ep, config=cfg, source=FolderSource(model))
@@ -151,7 +154,7 @@ class Runner:
         self.timing: Dict[str, float] = {}
 
     @staticmethod
-    def _fit_context(arch, cfg, model_limit: int, parallel: int, page_size: int, dtype: str, device: str) -> int:
+    def _fit_context(arch, cfg, model_limit: int, parallel: int, page_size: int, dtype: str, device: str, kv: str = "same") -> int:
         """ctx=0, the reference's auto-fit (-c 0, src/main.c:512): the longest context, up to the model's limit, whose
         keys and values for `parallel` requests fit the device memory that is free now beside the weights (nine
         tenths of it: the step's buffers need room too)."""
@@ -165,10 +168,15 @@ class Runner:
                 n *= int(s_)
             wbytes += n * wdt
         per_token = 0
+        values = 0                                               # what a portion's rows are read back into, a layer at a time
         for e in plan.schedule:
             need = plan.blocks[e.layer].mixer.kv_need()
             if need is not None and e.cache_from is None:
-                per_token += 2 * need.kv_heads * need.head_dim * elem
+                in_four = kv == "int4" and need.four_bits
+                per_token += need.kv_heads * kv_head_bytes(need, elem, True) if in_four else 2 * need.kv_heads * need.head_dim * elem
+                if in_four and elem == 2:
+                    values = max(values, 2 * need.kv_heads * need.head_dim * elem)
+        per_token += values
         free, _ = torch.cuda.mem_get_info(torch.device(device))
         room = int(0.9 * free) - 2 * wbytes                      # (packing a matrix needs a second copy for a moment)
         if per_token == 0:

@@ -165,7 +165,8 @@ def rmsnorm(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, eps: float, row
 def rope_store(qkv: torch.Tensor, positions, tok_seg, block_tables, inv_freq: Optional[torch.Tensor],
                cache_k_ptr: Optional[int], page_stride: int, v_offset: int, H: int, K: int, hd: int,
                rotary_dim: int, max_pages: int, page_size: int, adjacent: bool = False, mscale: float = 1.0) -> None:
-    """Rotate Q in place, rotate K and store K, V into their pages (cache_k_ptr None: store nothing).  Pair j of
+    """Rotate Q in place, rotate K and store K, V into their pages (cache_k_ptr None: store nothing; page_size 0: into rows, token t's K heads
+    at cache_k_ptr + t * page_stride elements, side by side, and its V heads `v_offset` elements further).  Pair j of
     a head is elements (j, j + rotary_dim/2), or (2j, 2j + 1) with `adjacent`; cosines and sines are multiplied
     by `mscale` (src/model.c:3514-3532)."""
     _dev(qkv, positions, tok_seg, block_tables, inv_freq)
@@ -205,7 +206,7 @@ def qk_norm_rope_store(inp: torch.Tensor, q_out: torch.Tensor, positions, tok_se
     """inp [n, >= (H + K) D + K Vd] (rows may be strided): Q heads, K heads (D each), V heads (Vd each).  Every Q and K head is
     RMS-normed with the weight q_w / k_w (float32 [D], shared by the heads; None: no norm), its first `rotary_dim` elements rotated
     (freq: float64 [rotary_dim / 2]); Q goes to q_out [n, *] (head h at column h * hd), K and V into the token's cache rows, every
-    head filled up to `hd` elements with zeros (cache_k_ptr None: nothing is stored).  `unit_norm` (with no weights): every Q
+    head filled up to `hd` elements with zeros (cache_k_ptr None: nothing is stored; page_size 0: into rows, see ``rope_store``).  `unit_norm` (with no weights): every Q
     and K head is divided by its root mean square all the same.  `q_every` > 0: the Q heads of the token at position p are
     multiplied by 1 + q_coef ln(floor((p + 1) / q_every) + 1).  `partial` (float32 [splits][n][inp.shape[1]], with `bias`): the rows are
     still the partial sums of a product cut along K; the kernel sums them (+ bias) into `inp`, every column, before it reads them.
@@ -719,12 +720,14 @@ def attention_tc(qkv: torch.Tensor, out: torch.Tensor, seg_start, seg_len, seg_p
                  max_seg_len: int, row_tiles: int = 0, sink: Optional[torch.Tensor] = None, softcap: float = 0.0,
                  keep_first: int = 0, bias: Optional[torch.Tensor] = None) -> None:
     """Causal attention of the portions with more than 16 packed rows on tcgen05 (S and O in tensor memory).
-    qkv: the step's fused rows (Q heads first); group = (pointer to the cache group's array, pages, layers, layer).
+    qkv: the step's fused rows (Q heads first; rows may be strided); group = (pointer to the cache group's array, pages, layers, layer).
     row_tiles: ``long_row_tiles(lengths, H // K, 128)``, which sizes the grid exactly; 0: every portion gets the blocks
     of the longest.  `sink`: float32 [H]; exp(sink[h]) joins the denominator of head h's softmax once.  `keep_first`, `bias`:
     see ``attention_simt`` (a bias goes without a cap)."""
     _check_bias(bias, H)
-    _dev(qkv, out, seg_start, seg_len, seg_pos0, block_tables, sink)
+    _dev(out, seg_start, seg_len, seg_pos0, block_tables, sink)
+    if not qkv.is_cuda or qkv.stride(1) != 1:
+        raise KernelError("kernel arguments must be CUDA tensors, neighbouring elements of a row side by side")
     assert sink is None or (sink.dtype == torch.float32 and sink.numel() == H)
     n = qkv.shape[0]
     assert qkv.dtype == torch.bfloat16 and out.dtype == torch.bfloat16 and out.shape == (n, H * hd)

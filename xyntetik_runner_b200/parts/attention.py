@@ -36,6 +36,9 @@ nothing else asks for it, for its rotation angles (float64 products of position 
 hold them stay held.  `distance_bias=(name, far)`: a learned table [rows, H] by distance joins the scaled scores, row
 ``DistanceBuckets(rows, far)`` of the distance from query to key.  `value_share` lets layers share values: "first" leaves the
 layer's values of the step's tokens for the layers behind it, "mix" caches (1 - l) v + l v_first, l the number in the tensor `v_mix`.
+
+A cache in four bits (the engine's `kv="int4"`, csrc/kv4.cuh) takes the keys and values as they would have been cached, rounded to the
+activations' type; what every query reads, its own token's row included, are the held values.
 """
 from __future__ import annotations
 
@@ -59,7 +62,7 @@ from .position import DistanceBuckets
 USE_MMA = True
 USE_TC = True
 USE_TMA = os.environ.get("XRB200_NO_TMA_ATTENTION", "0") in ("", "0")
-counters = {"mma": 0, "simt": 0, "tcgen05": 0}
+counters = {"mma": 0, "simt": 0, "tcgen05": 0, "kv4": 0}
 
 
 class GQAAttention(Mixer):
@@ -134,7 +137,7 @@ class GQAAttention(Mixer):
         self.q_norm_w = self.k_norm_w = self.freq64 = None
 
     def kv_need(self):
-        return KVNeed(self.K, self.hd, self.window, keep_first=self.keep_first)
+        return KVNeed(self.K, self.hd, self.window, keep_first=self.keep_first, four_bits=self.scale > 0)
 
     def tensors(self):
         q, k, v, o = (self.prefix + n for n in self.proj)
@@ -236,8 +239,20 @@ class GQAAttention(Mixer):
         n = h.shape[0]
         qkv_dim = (self.H + 2 * self.K) * self.hd
         qkv = ctx.buf("attn_qkv", (n, qkv_dim), ctx.act_dtype)
-        k_ptr, page_stride, v_offset = ctx.cache_layer(lay)
         bt = ctx.block_tables[lay.group]
+        four = ctx.cache_four_bits(lay)
+        page_size = ctx.page_size
+        if four is None:
+            k_ptr, page_stride, v_offset = ctx.cache_layer(lay)
+        elif self.general:
+            # rows of keys and values, which kernels.kv4_store then takes: beside the queries, in their own array
+            rows = ctx.buf("attn_kv_rows", (n, 2 * self.K * self.hd), ctx.act_dtype)
+            k_rows, v_rows = rows[:, :self.K * self.hd], rows[:, self.K * self.hd:]
+            k_ptr, page_stride, v_offset, page_size = rows.data_ptr(), rows.shape[1], self.K * self.hd, 0
+        else:
+            # ... or where the projection left them
+            k_rows, v_rows = qkv[:, self.H * self.hd:(self.H + self.K) * self.hd], qkv[:, (self.H + self.K) * self.hd:]
+            k_ptr, page_stride, v_offset, page_size = k_rows.data_ptr(), qkv_dim, self.K * self.hd, 0
         store_ptr = k_ptr if lay.writes_cache else None
         rot_dim, rot_freq, adjacent, mscale = self.rot
         if self.general:
@@ -255,7 +270,7 @@ class GQAAttention(Mixer):
             coef, every = self.q_temp if self.q_temp is not None else (0.0, 0)
             kernels.qk_norm_rope_store(proj, qkv, ctx.positions, ctx.tok_seg, bt, self.freq64, self.q_norm_w, self.k_norm_w, store_ptr,
                                        page_stride, v_offset, self.H, self.K, self.D, self.Vd, self.hd, rot_dim, ctx.max_pages,
-                                       ctx.page_size, adjacent, self.norm_eps, self.unit_norm, coef, every,
+                                       page_size, adjacent, self.norm_eps, self.unit_norm, coef, every,
                                        partial=None if pend is None else pend.partial, splits=0 if pend is None else pend.splits,
                                        bias=None if pend is None else pend.bias, mscale=mscale, norm_after=self.norm_after,
                                        v_first=v_first, v_lambda=self.v_lambda)
@@ -266,18 +281,26 @@ class GQAAttention(Mixer):
             if pend is not None and lay.writes_cache:
                 # the product was split along K: its finish, the rotation and the page store are one kernel
                 kernels.finish_rope_store(pend.partial, pend.splits, pend.bias, qkv, ctx.positions, ctx.tok_seg, bt,
-                                          rot_freq, store_ptr, page_stride, v_offset, self.H, self.K, self.hd,
+                                          rot_freq, store_ptr if four is None else None, page_stride, v_offset, self.H, self.K, self.hd,
                                           rot_dim, ctx.max_pages, ctx.page_size, adjacent, mscale)
                 pend.release()
             else:
                 if pend is not None:
                     pend.finish()
                 kernels.rope_store(qkv, ctx.positions, ctx.tok_seg, bt, rot_freq, store_ptr, page_stride,
-                                   v_offset, self.H, self.K, self.hd, rot_dim, ctx.max_pages, ctx.page_size, adjacent, mscale)
+                                   v_offset, self.H, self.K, self.hd, rot_dim, ctx.max_pages, page_size, adjacent, mscale)
+        if four is not None and lay.writes_cache:
+            kernels.kv4_store(k_rows, v_rows, ctx.positions, ctx.tok_seg, bt, four, lay.layer_in_group, ctx.page_size)
         o = ctx.buf("attn_out", (n, self.H * self.hd), ctx.act_dtype)
         # Q is read in place from the fused rows (row stride = qkv_dim)
         G = self.H // self.K
-        if USE_MMA and kernels.attention_mma_supported(ctx.act_dtype, self.H, self.K, self.hd):
+        if four is not None:
+            kernels.attention_kv4(qkv[:, :self.H * self.hd], o, four, lay.layer_in_group, ctx.page_size, ctx.seg_start, ctx.seg_len, ctx.seg_pos0, bt, self.H,
+                                  self.hd, self.scale, (ctx.host["seg_len"], ctx.host["seg_pos0"]), window=self.window or 0, sink=self.sink,
+                                  softcap=self.softcap, keep_first=self.keep_first, bias=self.dist_bias, max_kv_len=ctx.max_kv_len if ctx.decode_only else 0,
+                                  buf=ctx.buf)
+            counters["kv4"] += 1
+        elif USE_MMA and kernels.attention_mma_supported(ctx.act_dtype, self.H, self.K, self.hd):
             # (what the portions' lengths say is the same for every layer of the step)
             any_short, any_long, longest, tiles_tc, tiles_rows = ctx.once(("gqa_portions", G), lambda: self._portions(ctx, G))
             splits = ctx.once(("gqa_splits", self.window or 0, self.K),

@@ -59,6 +59,7 @@ class KVNeed:
     window: Optional[int] = None    # None: all keys; w: the last w keys
     planes: int = 2                 # arrays per token: 2 (keys and values), 1 for a mixer that caches one row per token
     keep_first: int = 0             # with a window: a request's first keys that stay visible behind it
+    four_bits: bool = False         # the mixer can also keep them in four bits (csrc/kv4.cuh), if the engine is told to
 
 
 @dataclass(frozen=True)
