@@ -74,11 +74,7 @@ def test_read_refuses(change, message):
     (dict(heads=3), "query heads"), (dict(out=torch.zeros(4, 255)), "rows of the same tokens"), (dict(q=torch.zeros(4, 255)), "rows of the same tokens"),
     (dict(q=torch.zeros(4, 256, dtype=torch.bfloat16)), "rows of the same tokens"), (dict(scale=0.0), "scale"), (dict(scale=math.nan), "scale"),
     (dict(window=-1), "window"), (dict(softcap=-1.0), "window"), (dict(softcap=1.0, bias=torch.zeros(4, 3)), "without a cap|CUDA"),
-    (dict(sink=torch.zeros(3)), "sink"), (dict(lengths=(np.array([2, 2]), np.array([0, 0]))), "int32"),
-    (dict(lengths=(np.array([3, 2], dtype=np.int32), np.array([0, 0], dtype=np.int32))), "does not hold|do not hold|does not|not hold"),
-    (dict(lengths=(np.array([2, 2], dtype=np.int32), np.array([0, -1], dtype=np.int32))), "below zero"),
-    (dict(lengths=(np.array([2], dtype=np.int32), np.array([0], dtype=np.int32))), "one value a portion"),
-    (dict(seg_pos0=torch.zeros(2)), "seg_pos0"), ({}, "current CUDA device")])
+    (dict(sink=torch.zeros(3)), "sink"), (dict(seg_pos0=torch.zeros(2)), "seg_pos0"), ({}, "current CUDA device")])
 def test_attention_refuses(change, message):
     p, i = _parts(), torch.zeros(2, dtype=torch.int32)
     two = np.array([2, 2], dtype=np.int32)
@@ -88,12 +84,22 @@ def test_attention_refuses(change, message):
         kernels.attention_kv4(**{**args, **change})
 
 
-def test_pages_that_are_read():
+def test_what_portions_ask_for():
+    """Pages that are read back, row tiles and scratch, from lengths on the host (the library's part that needs no device)."""
     a = lambda *x: np.array(x, dtype=np.int32)
-    assert kernels.kv4_pages_read(a(1, 20), a(0, 15), 16, 0, 0) == 1 + 3
-    assert kernels.kv4_pages_read(a(0, 20), a(7, 15), 16, 0, 0) == 3
-    assert kernels.kv4_pages_read(a(1), a(100), 16, 10, 20) == 2 + 2           # rows 91 .. 100 lie in pages 5 and 6, the kept in 0 and 1
-    assert kernels.kv4_pages_read(a(1), a(40), 16, 20, 33) == 1 + 2            # kept rows that the window's pages hold are not there twice
+    plan = lambda l, p, window=0, keep=0, most=0, n=100: kernels.kv4_plan((l, p), n, 2, 4, 64, 16, kernels.BF16, window, keep, most).tolist()
+    assert plan(a(1, 20), a(0, 15)) == [0, 2, 0, 1 + 3, 20, 2, 1 + 2, 35]
+    assert plan(a(0, 20), a(7, 15))[:4] == [0, 1, 0, 3]
+    assert plan(a(1), a(100), 10, 20)[3] == 2 + 2           # rows 91 .. 100 lie in pages 5 and 6, the kept in 0 and 1
+    assert plan(a(1), a(40), 20, 33)[3] == 1 + 2            # kept rows that the window's pages hold are not there twice
+    for l, p, n in ((a(-1), a(0), 9), (a(1), a(-1), 9), (a(5, 5), a(0, 0), 9)):
+        with pytest.raises(kernels.KernelError, match="does not hold"):
+            plan(l, p, n=n)
+    for l, p in ((a(1), a(1, 2)), (a(1).astype(np.int64), a(1))):
+        with pytest.raises(kernels.KernelError, match="one value a portion"):
+            plan(l, p)
+    with pytest.raises((BufferError, ValueError), match="contiguous"):
+        plan(np.zeros(8, dtype=np.int32)[::2], np.zeros(8, dtype=np.int32)[::2])
 
 
 def test_engine_refuses_before_it_looks_for_a_device():

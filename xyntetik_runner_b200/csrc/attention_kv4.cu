@@ -25,14 +25,13 @@
 // the tensor cores (q in pieces, p in pieces) give float32's precision.
 #include "kv4.cuh"
 #include "attention_mask.cuh"
+#include <cuda_fp16.h>
 #include <math.h>
 
 #define A4_WARPS 4
 #define A4_THREADS (32 * A4_WARPS)
-#define A4_STAGES 3
-#define A4_PAGES 448                  // block-table entries of a span that are kept in shared memory
-#define A4_SPIN_LIMIT (1u << 22)
 #define A4_LOG2E 1.4426950408889634f
+#define A4_SLACK 8.0f
 
 struct A4Args {
     const void* q; void* out;
@@ -40,7 +39,6 @@ struct A4Args {
     const int* seg_start; const int* seg_len; const int* seg_pos0; const int* block_tables;
     float* part_acc;                  // [n_seg][K * row_blocks][splits][rows][hs]
     float* part_ml;                   // [n_seg][K * row_blocks][splits][rows][2]
-    int* status;
     long long q_stride;
     int H, G, D, max_pages, window, keep, splits, span_tiles, row_blocks, most_rows;
     float scale, softcap;
@@ -75,26 +73,66 @@ __device__ __forceinline__ void a4_out(const A4Args& a, int tok0, int kvh, int r
 }
 
 __device__ __forceinline__ uint32_t a4_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ bool a4_wait(uint64_t* bar, uint32_t parity) {
-    for (uint32_t i = 0; i < A4_SPIN_LIMIT; i++) {
-        uint32_t ok;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(ok) : "r"(a4_smem(bar)), "r"(parity) : "memory");
-        if (ok) return true;
-    }
-    return false;
-}
-__device__ __forceinline__ void a4_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(a4_smem(dst)), "l"(src), "r"(bytes), "r"(a4_smem(bar)) : "memory");
+// 16 bytes from global to shared memory without a register between; `bytes` 0: zeros instead.
+__device__ __forceinline__ void a4_copy(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void a4_mma(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void a4_mma_half(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// d = A B + (c0, c1, c0, c1): what a key's row starts from hangs on its column alone
+__device__ __forceinline__ void a4_mma_from(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %10, %11};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ uint32_t a4_pack_half(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// A word's four pairs of neighbouring codes as float16 numbers: a mantissa of ten bits takes two codes side by side, so that two shifts serve four pairs.
+// Pairs 0 and 2 are 256 + u, pairs 1 and 3 are 16 + u.
+__device__ __forceinline__ void a4_pairs(uint32_t w, uint32_t* p) {
+    const uint32_t l = w * 4u, r = w >> 6;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(p[0]) : "r"(l), "r"(0x003C003Cu), "r"(0x5C005C00u));
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(p[1]) : "r"(l), "r"(0x03C003C0u), "r"(0x4C004C00u));
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(p[2]) : "r"(r), "r"(0x003C003Cu), "r"(0x5C005C00u));
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(p[3]) : "r"(r), "r"(0x03C003C0u), "r"(0x4C004C00u));
+}
+__device__ __forceinline__ uint32_t a4_fma_half(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t a4_mul_half(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ void a4_ldsm4(uint32_t* r, uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+template <int W> __device__ __forceinline__ void a4_lds(uint32_t* r, uint32_t at) {
+    if constexpr (W == 1) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r[0]) : "r"(at));
+    else if constexpr (W == 2) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(at));
+    else {
+#pragma unroll
+        for (int i = 0; i < W; i += 4) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]) : "r"(at + 4 * i));
+    }
+}
+__device__ __forceinline__ uint32_t a4_lds16(uint32_t at) {
+    unsigned short r;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(r) : "r"(at));
+    return r;
 }
 __device__ __forceinline__ uint32_t a4_turn(uint32_t x) {            // transpose of an 8 x 8 matrix of 16-bit numbers over the warp
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
 }
 __device__ __forceinline__ float a4_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
@@ -114,7 +152,7 @@ __device__ __forceinline__ uint32_t a4_piece(float& lo, float& hi) {
 // group of four threads are four neighbouring keys, and so are the places 2t + 1.
 __device__ __forceinline__ int a4_key(int r) { return (r & 8) + 4 * (r & 1) + (((r & 7) >> 1) ^ (r & 1)); }
 
-template <int NG> struct A4Tile { static constexpr int KEYS = NG == 2 ? 64 : 32; };
+template <int NG> struct A4Tile { static constexpr int KEYS = NG <= 4 ? 64 : 32, STAGES = NG == 4 ? 2 : 3; };
 
 // The tiles that the rows of a block see: those of the kept first keys, then those of the window.
 struct A4Walk { int lo, hi, t_lo, kept, n; };
@@ -134,13 +172,13 @@ __device__ __forceinline__ int a4_spans(const A4Args& a, const A4Walk& w) { retu
 // NG: groups of 32 elements a held head (2, 4, 8); NT: eight-row tiles a block; F32: float32 queries and outputs, in pieces (NT 1);
 // EXTRA: a cap or a bias on the scores
 template <int NG, int NT, bool F32, bool EXTRA> struct A4Shape {
-    static constexpr int HS = NG * 32, TK = A4Tile<NG>::KEYS, SUB = TK / 16, KS = 2 * NG, RB = 8 * NT, P = F32 ? 3 : 1;
+    static constexpr int HS = NG * 32, TK = A4Tile<NG>::KEYS, SUB = TK / 16, STAGES = A4Tile<NG>::STAGES, KS = 2 * NG, RB = 8 * NT, P = F32 ? 3 : 1;
     static constexpr int CODES = HS / 2, SCALES = HS / 16;           // bytes of a token's keys (or values)
     static constexpr int STAGE = TK * 2 * (CODES + SCALES);
     static constexpr int VW = NG / 2, MT = 4 * VW;                   // words of a value's row a thread takes; m-tiles of O^T
     static constexpr bool Q_REGS = KS * 2 * NT * P <= 48;            // q's fragments in registers, else in shared memory
-    static constexpr int BLOCKS = NG <= 4 && NT == 1 && !F32 ? 4 : 2;            // blocks an SM (registers, shared memory)
-    static constexpr int SMEM = A4_WARPS * A4_STAGES * (STAGE + 8) + 4 * A4_PAGES + (Q_REGS ? 0 : P * NT * KS * 32 * 8) + 16;
+    static constexpr int BLOCKS = NG <= 4 && NT == 1 && !F32 ? 3 : 2;            // blocks an SM (registers, shared memory)
+    static constexpr int SMEM = A4_WARPS * STAGES * STAGE + (Q_REGS ? 0 : P * NT * KS * 32 * 8) + 16;
 };
 
 template <int NG, int NT, bool F32, bool EXTRA>
@@ -148,13 +186,10 @@ __global__ void __launch_bounds__(A4_THREADS, (A4Shape<NG, NT, F32, EXTRA>::BLOC
 k_kv4_attention(A4Args a) {
     xr_pdl_launch();
     using S = A4Shape<NG, NT, F32, EXTRA>;
-    constexpr int HS = S::HS, TK = S::TK, SUB = S::SUB, KS = S::KS, RB = S::RB, P = S::P, CODES = S::CODES, SCALES = S::SCALES, STAGE = S::STAGE;
+    constexpr int HS = S::HS, TK = S::TK, SUB = S::SUB, STAGES = S::STAGES, KS = S::KS, RB = S::RB, P = S::P, CODES = S::CODES, SCALES = S::SCALES, STAGE = S::STAGE;
     constexpr int VW = S::VW, MT = S::MT;
     extern __shared__ __align__(128) uint8_t smem[];
-    uint64_t* bars = (uint64_t*)(smem + A4_WARPS * A4_STAGES * STAGE);
-    int* gave_up = (int*)(bars + A4_WARPS * A4_STAGES);
-    int* pages = gave_up + 4;
-    uint2* q_sm = (uint2*)(pages + A4_PAGES);                        // [P][NT][KS][32]
+    uint2* q_sm = (uint2*)(smem + A4_WARPS * STAGES * STAGE);                        // [P][NT][KS][32]
     const int seg = blockIdx.z, kvh = blockIdx.y % a.c.K, rb = blockIdx.y / a.c.K, span = blockIdx.x;
     xr_pdl_wait();
     const int L = a.seg_len[seg];
@@ -170,111 +205,148 @@ k_kv4_attention(A4Args a) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int* bt = a.block_tables + (size_t)seg * a.max_pages;
     const int ps = a.c.page_size;
-    const int page0 = (int)((long long)xr_walk_tile(i_begin, walk.kept, walk.t_lo) * TK / ps);
-    for (int i = threadIdx.x; i < A4_PAGES; i += A4_THREADS) {
-        const int pi = page0 + i;
-        pages[i] = pi < a.max_pages && (long long)pi * ps <= walk.hi ? bt[pi] : -1;
-    }
-    if (threadIdx.x < A4_WARPS * A4_STAGES) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(a4_smem(&bars[threadIdx.x])), "r"(1));
-    if (threadIdx.x == 0) *gave_up = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-
-    // q: thread (row g, t) holds the elements that its words of a key hold, 8 NG t ..; k-step 2 w + half: elements 8 w + 4 half ..
-    uint32_t qf[S::Q_REGS ? P : 1][S::Q_REGS ? NT : 1][S::Q_REGS ? KS : 1][2];
-    if (S::Q_REGS || warp == 0) {
+    uint8_t* my_ring = smem + warp * STAGES * STAGE;              // a stage: keys' codes, values' codes, keys' scales, values' scales
+    const uint32_t ring_at = a4_smem(my_ring);
+    const uint8_t* head_run = a.c.base + a.c.layer_at + (long long)kvh * a.c.block();
+    auto page_of = [&](int pi) -> int {
+        const int page = pi < a.max_pages ? __ldg(bt + pi) : -1;
+        return page < a.c.n_pages ? page : -1;
+    };
+    // The page of tile i, where pages hold whole tiles (2^tile_shift of them); asked for a tile ahead of its fetch: one trip to L1 that nobody waits for.
+    auto tiles_page = [&](int i) { return a.tile_shift >= 0 && i < i_end ? page_of(xr_walk_tile(i, walk.kept, walk.t_lo) >> a.tile_shift) : -1; };
+    // The warp fetches tile i of the walk into stage s, 16 bytes a lane at a time; rows on a page that is not held become zeros.
+    auto fetch = [&](int i, int s, int page) {
+        const int tile = xr_walk_tile(i, walk.kept, walk.t_lo);
+        const uint32_t st = ring_at + s * STAGE + 16 * lane;
+        if (a.tile_shift >= 0) {
+            const int in = (tile & ((1 << a.tile_shift) - 1)) * TK;
+            const uint32_t n = page >= 0 ? 16 : 0;
+            const uint8_t* run = head_run + max(page, 0) * a.c.page_bytes;
+            const uint8_t* codes = run + in * CODES + 16 * lane;
+            const uint8_t* scales = run + a.c.scales_at(0) + in * SCALES;
+            const int far = a.c.codes_at(1);
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            const int row = row0 + nt * 8 + g, live = nt * 8 + g < rows;
-            const long long base = live ? (long long)(tok0 + row / a.G) * a.q_stride + (long long)(kvh * a.G + row % a.G) * a.D : 0;
+            for (int e = 0; e < TK * CODES / 512; e++) {
+                a4_copy(st + 512 * e, codes + 512 * e, n);
+                a4_copy(st + TK * CODES + 512 * e, codes + far + 512 * e, n);
+            }
+#pragma unroll
+            for (int e = 0; e < TK * SCALES / 256; e++) {
+                // (half the lanes the keys' scales, half the values')
+                const int b = 16 * (lane & 15) + 256 * e;
+                a4_copy(ring_at + s * STAGE + 2 * TK * CODES + (lane >> 4) * TK * SCALES + b, scales + (lane >> 4) * (ps * SCALES) + b, n);
+            }
+        } else {
+            const long long k0 = (long long)tile * TK;
+            auto piece = [&](uint32_t to, int at, int token, int bytes) {         // the 16 bytes at `at` behind the first token's in a part, `bytes` a token
+                const int r = at / bytes, pi = (int)((k0 + r) / ps), held = page_of(pi);
+                const uint8_t* run = head_run + max(held, 0) * a.c.page_bytes + token;
+                a4_copy(to, run + (k0 + r - (long long)pi * ps) * bytes + at % bytes, held >= 0 ? 16 : 0);
+            };
+#pragma unroll 1
+            for (int b = 16 * lane; b < TK * CODES; b += 512) {
+                piece(ring_at + s * STAGE + b, b, a.c.codes_at(0), CODES);
+                piece(ring_at + s * STAGE + TK * CODES + b, b, a.c.codes_at(1), CODES);
+            }
+#pragma unroll 1
+            for (int b = 16 * (lane & 15); b < TK * SCALES; b += 256)
+                piece(ring_at + s * STAGE + 2 * TK * CODES + (lane >> 4) * TK * SCALES + b, b, a.c.scales_at(lane >> 4), SCALES);
+        }
+    };
+    // (a group of copies a stage, empty ones behind the last tile: the wait counts groups)
+    int next_page;
+    {
+        int first[STAGES];
+#pragma unroll
+        for (int s = 0; s < STAGES; s++) first[s] = tiles_page(i_begin + warp + s * A4_WARPS);
+        next_page = tiles_page(i_begin + warp + STAGES * A4_WARPS);
+#pragma unroll
+        for (int s = 0; s < STAGES; s++) {
+            if (i_begin + warp + s * A4_WARPS < i_end) fetch(i_begin + warp + s * A4_WARPS, s, first[s]);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+    }
+
+    // q.  float32: thread (row g, t) holds the elements that its words of a key hold, 8 NG t ..; k-step 2 w + half: elements 8 w + 4 half ..  bfloat16: thread
+    // (row g, t) holds the elements of word t of every group; k-steps 2 grp and 2 grp + 1.
+    uint32_t qf[S::Q_REGS ? P : 1][S::Q_REGS ? NT : 1][S::Q_REGS ? KS : 1][2];
+    float q_sum[F32 ? 1 : NT][F32 ? 1 : NG][2], q_unit[NT][2];       // of the thread's two columns: what takes a group's bias off; a score's unit
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const int row = row0 + nt * 8 + g, live = nt * 8 + g < rows;
+        const long long base = live ? (long long)(tok0 + row / a.G) * a.q_stride + (long long)(kvh * a.G + row % a.G) * a.D : 0;
+        if constexpr (F32) {
+            q_unit[nt][0] = q_unit[nt][1] = 1.f;
 #pragma unroll
             for (int w = 0; w < NG; w++) {
                 const int d = 8 * (NG * t + w);
-                if constexpr (!F32) {
-                    uint32_t x[4] = {0, 0, 0, 0};
-                    const __nv_bfloat16* src = (const __nv_bfloat16*)a.q + base + d;
-                    if (a.wide) {
-                        if (live && d < a.D) { const uint4 v = *reinterpret_cast<const uint4*>(src); x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
-                    } else {
+                float x[8];
+                const float* src = (const float*)a.q + base + d;
 #pragma unroll
-                        for (int e = 0; e < 8; e++)
-                            if (live && d + e < a.D) x[e >> 1] |= (uint32_t)reinterpret_cast<const unsigned short*>(src)[e] << (16 * (e & 1));
-                    }
+                for (int e = 0; e < 8; e++) x[e] = live && d + e < a.D ? src[e] : 0.f;
+#pragma unroll
+                for (int p = 0; p < 3; p++)
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        if constexpr (S::Q_REGS) { qf[0][nt][2 * w + h][0] = x[2 * h]; qf[0][nt][2 * w + h][1] = x[2 * h + 1]; }
-                        else q_sm[(nt * KS + 2 * w + h) * 32 + lane] = make_uint2(x[2 * h], x[2 * h + 1]);
+                        const uint32_t u = a4_piece(x[4 * h], x[4 * h + 1]), v = a4_piece(x[4 * h + 2], x[4 * h + 3]);
+                        if constexpr (S::Q_REGS) { qf[p][nt][2 * w + h][0] = u; qf[p][nt][2 * w + h][1] = v; }
+                        else if (warp == 0) q_sm[((p * NT + nt) * KS + 2 * w + h) * 32 + lane] = make_uint2(u, v);
                     }
+            }
+        } else {
+            auto word_of = [&](int w, uint32_t* x) {
+                const int d = 32 * w + 8 * t;
+                const __nv_bfloat16* src = (const __nv_bfloat16*)a.q + base + d;
+                x[0] = x[1] = x[2] = x[3] = 0;
+                if (a.wide) {
+                    if (live && d < a.D) { const uint4 v = *reinterpret_cast<const uint4*>(src); x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
                 } else {
-                    float x[8];
-                    const float* src = (const float*)a.q + base + d;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = live && d + e < a.D ? src[e] : 0.f;
-#pragma unroll
-                    for (int p = 0; p < 3; p++)
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const uint32_t u = a4_piece(x[4 * h], x[4 * h + 1]), v = a4_piece(x[4 * h + 2], x[4 * h + 3]);
-                            if constexpr (S::Q_REGS) { qf[p][nt][2 * w + h][0] = u; qf[p][nt][2 * w + h][1] = v; }
-                            else q_sm[((p * NT + nt) * KS + 2 * w + h) * 32 + lane] = make_uint2(u, v);
-                        }
+                    for (int e = 0; e < 8; e++)
+                        if (live && d + e < a.D) x[e >> 1] |= (uint32_t)reinterpret_cast<const unsigned short*>(src)[e] << (16 * (e & 1));
                 }
+            };
+            uint32_t top = 0;                                        // the largest magnitude, by its bits: a NaN is above all others
+#pragma unroll
+            for (int w = 0; w < NG; w++) {
+                uint32_t x[4];
+                word_of(w, x);
+#pragma unroll
+                for (int e = 0; e < 4; e++) top = max(top, max((x[e] << 16) & 0x7fff0000u, x[e] & 0x7fff0000u));
+            }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // The row in float16, times a power of two: largest magnitude in [2^13, 2^14), every element's eight bits whole down to 2^-31 of it.  A row
+            // with an infinity or a NaN has no unit.
+            const int ex = max((int)(top >> 23), 20) - 127;
+            const float up = __int_as_float((127 + 13 - ex) << 23), unit = ex == 128 ? __int_as_float(0x7fc00000) : __int_as_float((127 - 13 + ex) << 23);
+            q_unit[nt][0] = __shfl_sync(0xffffffffu, unit, 8 * t);
+            q_unit[nt][1] = __shfl_sync(0xffffffffu, unit, 8 * t + 4);
+#pragma unroll
+            for (int w = 0; w < NG; w++) {
+                uint32_t x[4];
+                word_of(w, x);
+                uint32_t y[4];
+                float sum = 0.f;                                     // the pairs' biases: 256 + 8 and 16 + 8
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    y[e] = a4_pack_half(__uint_as_float(x[e] << 16) * up, __uint_as_float(x[e] & 0xffff0000u) * up);
+                    const float2 z = __half22float2(*reinterpret_cast<const __half2*>(&y[e]));
+                    sum = fmaf(e & 1 ? -24.f : -264.f, z.x + z.y, sum);
+                }
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if constexpr (S::Q_REGS) { qf[0][nt][2 * w + h][0] = y[2 * h]; qf[0][nt][2 * w + h][1] = y[2 * h + 1]; }
+                    else if (warp == 0) q_sm[(nt * KS + 2 * w + h) * 32 + lane] = make_uint2(y[2 * h], y[2 * h + 1]);
+                }
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                q_sum[nt][w][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
+                q_sum[nt][w][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
             }
         }
     }
-    __syncthreads();
-    uint8_t* my_ring = smem + warp * A4_STAGES * STAGE;              // a stage: keys' codes, values' codes, keys' scales, values' scales
-    uint64_t* my_bars = bars + warp * A4_STAGES;
-    const uint8_t* head_run = a.c.base + a.c.layer_at + (long long)kvh * a.c.block();
-    // Lane 0 fetches tile i of the walk into stage s, a page's piece at a time.  Rows on a page that is not held are rows of zeros.
-    auto page_at = [&](int pi) -> int {
-        const int page = pi - page0 < A4_PAGES && pi >= page0 ? pages[pi - page0] : pi < a.max_pages ? bt[pi] : -1;
-        return page < a.c.n_pages ? page : -1;
-    };
-    auto piece = [&](uint8_t* st, int r, int page, int tok, int len, uint64_t* bar) {
-        const uint8_t* run = head_run + page * a.c.page_bytes;
-#pragma unroll
-        for (int w = 0; w < 2; w++) {
-            a4_copy(st + w * TK * CODES + r * CODES, run + a.c.codes_at(w) + tok * CODES, len * CODES, bar);
-            a4_copy(st + 2 * TK * CODES + w * TK * SCALES + r * SCALES, run + a.c.scales_at(w) + tok * SCALES, len * SCALES, bar);
-        }
-    };
-    auto fetch = [&](int i, int s) {
-        const long long k0 = (long long)xr_walk_tile(i, walk.kept, walk.t_lo) * TK;
-        uint8_t* st = my_ring + s * STAGE;
-        uint64_t* bar = &my_bars[s];
-        if (a.tile_shift >= 0) {
-            // (a page holds 2^tile_shift whole tiles)
-            const int tile = (int)(k0 / TK), page = page_at(tile >> a.tile_shift), tok = (tile & ((1 << a.tile_shift) - 1)) * TK;
-            if (page >= 0) {
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(a4_smem(bar)), "r"(STAGE) : "memory");
-                piece(st, 0, page, tok, TK, bar);
-                return;
-            }
-        }
-        uint32_t bytes = 0;
-        for (int pass = 0; pass < 2; pass++) {
-            for (int r = 0; r < TK;) {
-                const int pi = (int)((k0 + r) / ps), tok = (int)(k0 + r - (long long)pi * ps), len = min(TK - r, ps - tok), page = page_at(pi);
-                if (page >= 0) {
-                    if (pass == 0) bytes += len * 2 * (CODES + SCALES);
-                    else piece(st, r, page, tok, len, bar);
-                } else if (pass == 0) {
-                    for (int w = 0; w < 2; w++)
-                        for (int b = 0; b < len * SCALES; b += 4) *reinterpret_cast<uint32_t*>(st + 2 * TK * CODES + w * TK * SCALES + r * SCALES + b) = 0;
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                }
-                r += len;
-            }
-            // (all bytes are announced before the first copy, so that the barrier's phase cannot end among them)
-            if (pass == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(a4_smem(bar)), "r"(bytes) : "memory");
-        }
-    };
-    if (lane == 0) {
-#pragma unroll
-        for (int s = 0; s < A4_STAGES; s++)
-            if (i_begin + warp + s * A4_WARPS < i_end) fetch(i_begin + warp + s * A4_WARPS, s);
-    }
-    __syncwarp();
+    if (!S::Q_REGS) __syncthreads();
 
     int pos_r[NT][2];                                                // positions of this thread's two columns (rows of q) of each tile
 #pragma unroll
@@ -282,7 +354,13 @@ k_kv4_attention(A4Args a) {
 #pragma unroll
         for (int e = 0; e < 2; e++) pos_r[nt][e] = pos0 + (row0 + min(nt * 8 + 2 * t + e, rows - 1)) / a.G;
     const float sl = a.scale * A4_LOG2E;
+    // (float16 weights: 2^LIFT times larger, so that they are whole numbers of 2^-11 of themselves down to 2^-19 of the largest; at most 2^13)
+    constexpr float LIFT = F32 ? 0.f : 5.f;
+    float unit[NT][2];                                               // what turns a column's scores into exponents of two
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) { unit[nt][0] = EXTRA ? sl : sl * q_unit[nt][0]; unit[nt][1] = EXTRA ? sl : sl * q_unit[nt][1]; }
     float o[NT][MT][4], m[NT][2], l[NT][2];
+    float v_unit = 1.f, v_inv = 1.f, v_most = F32 ? INFINITY : 0.f;  // the sums' unit, its inverse, the largest scale in it
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -291,58 +369,87 @@ k_kv4_attention(A4Args a) {
     }
     const int key_a = a4_key(g);                                     // a subtile's key of row g (row g + 8: 8 further)
     const int place_a = t, place_b = 4 + (t ^ 1);                    // ... of places 2t and 2t + 1
-    const int vgroup = g * VW / 4;
+    // where a thread reads in a stage: keys' codes (bfloat16: the row that it names to ldmatrix; float32: its words) and scales, values' codes and
+    // scales of places 2t and 2t + 1
+    const uint32_t k_at = F32 ? key_a * CODES + 4 * NG * t
+                        : NG == 2 ? (8 * (lane >> 4) + a4_key(lane & 7)) * CODES + 16 * ((lane >> 3) & 1) : a4_key(lane & 7) * CODES + 16 * (lane >> 3);
+    const uint32_t ks_at = 2 * TK * CODES + key_a * SCALES + (F32 ? 2 * (NG * t / 4) : 0);
+    const uint32_t va_at = TK * CODES + place_a * CODES + 4 * VW * g, vb_at = TK * CODES + place_b * CODES + 4 * VW * g;
+    const uint32_t vsa_at = 2 * TK * CODES + TK * SCALES + place_a * SCALES + 2 * (g * VW / 4), vsb_at = vsa_at + (place_b - place_a) * SCALES;
     int stage = 0;
-    uint32_t phase = 0;
-    bool lost = false;
     for (int i = i_begin + warp; i < i_end; i += A4_WARPS) {
         const int k0 = xr_walk_tile(i, walk.kept, walk.t_lo) * TK;
-        const uint8_t* kc = my_ring + stage * STAGE;
-        const uint8_t* vc = kc + TK * CODES;
-        const uint8_t* ks = vc + TK * CODES;
-        const uint8_t* vs = ks + TK * SCALES;
-        if (!__all_sync(0xffffffffu, a4_wait(&my_bars[stage], phase))) { lost = true; break; }
+        const uint32_t st = ring_at + stage * STAGE;
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        __syncwarp();
         float s[SUB][NT][4];
 #pragma unroll
         for (int sub = 0; sub < SUB; sub++) {
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) s[sub][nt][0] = s[sub][nt][1] = s[sub][nt][2] = s[sub][nt][3] = 0.f;
-            const int ka = sub * 16 + key_a, kb = ka + 8;
-            uint32_t wa[NG], wb[NG];
-            if constexpr (NG == 2) {
-                const uint2 x = *reinterpret_cast<const uint2*>(kc + ka * CODES + 8 * t), y = *reinterpret_cast<const uint2*>(kc + kb * CODES + 8 * t);
-                wa[0] = x.x; wa[1] = x.y; wb[0] = y.x; wb[1] = y.y;
-            } else {
+            if constexpr (!F32) {
+                // A group's codes are multiplied as they are, with their bias, from sums that start at what takes it off; the group's scale is a factor on the
+                // result.  All four threads of a key have a word of the same group: ldmatrix deals a 16-byte row's words to them.
+                uint32_t w[2][NG];                                   // word t of every group, of the keys of rows g and g + 8
+                uint32_t sc[2][NG / 2];
+                if constexpr (NG == 2) {
+                    uint32_t r[4];
+                    a4_ldsm4(r, st + k_at + sub * 16 * CODES);
+                    w[0][0] = r[0]; w[0][1] = r[1]; w[1][0] = r[2]; w[1][1] = r[3];
+                } else {
 #pragma unroll
-                for (int c = 0; c < NG / 4; c++) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(kc + ka * CODES + 4 * NG * t + 16 * c), y = *reinterpret_cast<const uint4*>(kc + kb * CODES + 4 * NG * t + 16 * c);
-                    wa[4 * c] = x.x; wa[4 * c + 1] = x.y; wa[4 * c + 2] = x.z; wa[4 * c + 3] = x.w;
-                    wb[4 * c] = y.x; wb[4 * c + 1] = y.y; wb[4 * c + 2] = y.z; wb[4 * c + 3] = y.w;
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int c = 0; c < NG; c += 4) a4_ldsm4(&w[h][c], st + k_at + (sub * 16 + 8 * h) * CODES + 16 * c);
                 }
-            }
 #pragma unroll
-            for (int w0 = 0; w0 < NG; w0 += NG == 2 ? 2 : 4) {
-                // (a thread's words of one group share a scale)
-                const int grp = (NG * t + w0) / 4;
-                uint32_t sa = *reinterpret_cast<const unsigned short*>(ks + ka * SCALES + 2 * grp), sb = *reinterpret_cast<const unsigned short*>(ks + kb * SCALES + 2 * grp);
-                sa |= sa << 16; sb |= sb << 16;
-                const uint32_t ma = kv4_m24(sa), mb = kv4_m24(sb);
+                for (int h = 0; h < 2; h++) a4_lds<NG / 2>(sc[h], st + ks_at + (sub * 16 + 8 * h) * SCALES);
 #pragma unroll
-                for (int w = w0; w < w0 + (NG == 2 ? 2 : 4); w++) {
-                    const uint32_t a0 = kv4_scaled(kv4_pair<0>(wa[w]), sa, ma), a1 = kv4_scaled(kv4_pair<0>(wb[w]), sb, mb);
-                    const uint32_t a2 = kv4_scaled(kv4_pair<1>(wa[w]), sa, ma), a3 = kv4_scaled(kv4_pair<1>(wb[w]), sb, mb);
-                    const uint32_t b0 = kv4_scaled(kv4_pair<2>(wa[w]), sa, ma), b1 = kv4_scaled(kv4_pair<2>(wb[w]), sb, mb);
-                    const uint32_t b2 = kv4_scaled(kv4_pair<3>(wa[w]), sa, ma), b3 = kv4_scaled(kv4_pair<3>(wb[w]), sb, mb);
+                for (int grp = 0; grp < NG; grp++) {
+                    uint32_t pa[4], pb[4];
+                    a4_pairs(w[0][grp], pa);
+                    a4_pairs(w[1][grp], pb);
+                    const float fa = __uint_as_float(grp & 1 ? sc[0][grp >> 1] & 0xffff0000u : sc[0][grp >> 1] << 16);
+                    const float fb = __uint_as_float(grp & 1 ? sc[1][grp >> 1] & 0xffff0000u : sc[1][grp >> 1] << 16);
 #pragma unroll
-                    for (int p = P - 1; p >= 0; p--)
+                    for (int nt = 0; nt < NT; nt++) {
+                        float d[4];
+                        uint2 qa, qb;
+                        if constexpr (S::Q_REGS) { qa = make_uint2(qf[0][nt][2 * grp][0], qf[0][nt][2 * grp][1]); qb = make_uint2(qf[0][nt][2 * grp + 1][0], qf[0][nt][2 * grp + 1][1]); }
+                        else { qa = q_sm[(nt * KS + 2 * grp) * 32 + lane]; qb = q_sm[(nt * KS + 2 * grp + 1) * 32 + lane]; }
+                        a4_mma_from(d, pa[0], pb[0], pa[1], pb[1], qa.x, qa.y, q_sum[nt][grp][0], q_sum[nt][grp][1]);
+                        a4_mma_half(d, pa[2], pb[2], pa[3], pb[3], qb.x, qb.y);
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            uint2 qa, qb;
-                            if constexpr (S::Q_REGS) { qa = make_uint2(qf[p][nt][2 * w][0], qf[p][nt][2 * w][1]); qb = make_uint2(qf[p][nt][2 * w + 1][0], qf[p][nt][2 * w + 1][1]); }
-                            else { qa = q_sm[((p * NT + nt) * KS + 2 * w) * 32 + lane]; qb = q_sm[((p * NT + nt) * KS + 2 * w + 1) * 32 + lane]; }
-                            a4_mma(s[sub][nt], a0, a1, a2, a3, qa.x, qa.y);
-                            a4_mma(s[sub][nt], b0, b1, b2, b3, qb.x, qb.y);
-                        }
+                        for (int e = 0; e < 4; e++) s[sub][nt][e] = grp == 0 ? (e < 2 ? fa : fb) * d[e] : fmaf(e < 2 ? fa : fb, d[e], s[sub][nt][e]);
+                    }
+                }
+            } else {
+                uint32_t wa[NG], wb[NG];
+                a4_lds<NG>(wa, st + k_at + sub * 16 * CODES);
+                a4_lds<NG>(wb, st + k_at + (sub * 16 + 8) * CODES);
+#pragma unroll
+                for (int w0 = 0; w0 < NG; w0 += NG == 2 ? 2 : 4) {
+                    // (a thread's words of one group share a scale)
+                    uint32_t sa = a4_lds16(st + ks_at + sub * 16 * SCALES + w0 / 2), sb = a4_lds16(st + ks_at + (sub * 16 + 8) * SCALES + w0 / 2);
+                    sa *= 0x10001u; sb *= 0x10001u;
+                    const uint32_t ma = kv4_m24(sa), mb = kv4_m24(sb);
+#pragma unroll
+                    for (int w = w0; w < w0 + (NG == 2 ? 2 : 4); w++) {
+                        const uint32_t a0 = kv4_scaled(kv4_pair<0>(wa[w]), sa, ma), a1 = kv4_scaled(kv4_pair<0>(wb[w]), sb, mb);
+                        const uint32_t a2 = kv4_scaled(kv4_pair<1>(wa[w]), sa, ma), a3 = kv4_scaled(kv4_pair<1>(wb[w]), sb, mb);
+                        const uint32_t b0 = kv4_scaled(kv4_pair<2>(wa[w]), sa, ma), b1 = kv4_scaled(kv4_pair<2>(wb[w]), sb, mb);
+                        const uint32_t b2 = kv4_scaled(kv4_pair<3>(wa[w]), sa, ma), b3 = kv4_scaled(kv4_pair<3>(wb[w]), sb, mb);
+#pragma unroll
+                        for (int p = P - 1; p >= 0; p--)
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) {
+                                uint2 qa, qb;
+                                if constexpr (S::Q_REGS) { qa = make_uint2(qf[p][nt][2 * w][0], qf[p][nt][2 * w][1]); qb = make_uint2(qf[p][nt][2 * w + 1][0], qf[p][nt][2 * w + 1][1]); }
+                                else { qa = q_sm[((p * NT + nt) * KS + 2 * w) * 32 + lane]; qb = q_sm[((p * NT + nt) * KS + 2 * w + 1) * 32 + lane]; }
+                                a4_mma(s[sub][nt], a0, a1, a2, a3, qa.x, qa.y);
+                                a4_mma(s[sub][nt], b0, b1, b2, b3, qb.x, qb.y);
+                            }
+                    }
                 }
             }
         }
@@ -356,6 +463,7 @@ k_kv4_attention(A4Args a) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         float& x = s[sub][nt][e];
+                        if (!F32) x *= q_unit[nt][e & 1];
                         if (a.softcap > 0.f) {
                             // c tanh(x scale / c) / scale, through one exponential: tanh(y) = 1 - 2 / (exp(2 y) + 1)
                             const float cap = a.softcap / a.scale, ex = __expf(2.0f * x * (a.scale / a.softcap));
@@ -377,74 +485,66 @@ k_kv4_attention(A4Args a) {
                         if (!xr_sees(key, pos, a.window > 0 ? pos - a.window + 1 : 0, a.keep)) s[sub][nt][e] = -INFINITY;
                     }
         }
-        float off[NT][2], f[NT][2];
+        // The running maximum is followed loosely: weights are exp2(score - m), and m is raised (to the columns' maxima over all lanes) only where a score
+        // is 2^A4_SLACK times above it, or is the first.  Weights up to 2^A4_SLACK change no relative error, and most tiles pay neither for shuffles nor
+        // for another pass over the sums.
         bool grown = false;
+        float mx[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                float mx = fmaxf(s[0][nt][e], s[0][nt][e + 2]);
+                mx[nt][e] = fmaxf(s[0][nt][e], s[0][nt][e + 2]);
 #pragma unroll
-                for (int sub = 1; sub < SUB; sub++) mx = fmaxf(mx, fmaxf(s[sub][nt][e], s[sub][nt][e + 2]));
-#pragma unroll
-                for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-                const float was = m[nt][e];
-                m[nt][e] = fmaxf(was, mx * sl);
-                off[nt][e] = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
-                f[nt][e] = a4_exp2(was - off[nt][e]);
-                grown |= was != m[nt][e];
+                for (int sub = 1; sub < SUB; sub++) mx[nt][e] = fmaxf(mx[nt][e], fmaxf(s[sub][nt][e], s[sub][nt][e + 2]));
+                grown |= mx[nt][e] * unit[nt][e] > m[nt][e] + A4_SLACK;
             }
         if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                l[nt][0] *= f[nt][0]; l[nt][1] *= f[nt][1];
+                float f[2];
 #pragma unroll
-                for (int d = 0; d < MT; d++) { o[nt][d][0] *= f[nt][0]; o[nt][d][1] *= f[nt][1]; o[nt][d][2] *= f[nt][0]; o[nt][d][3] *= f[nt][1]; }
+                for (int e = 0; e < 2; e++) {
+                    float x = mx[nt][e];
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                    const float was = m[nt][e];
+                    m[nt][e] = fmaxf(was, x * unit[nt][e]);
+                    f[e] = was == m[nt][e] ? 1.f : a4_exp2(was - m[nt][e]);            // (both -infinity: no key seen yet)
+                    l[nt][e] *= f[e];
+                }
+#pragma unroll
+                for (int d = 0; d < MT; d++) { o[nt][d][0] *= f[0]; o[nt][d][1] *= f[1]; o[nt][d][2] *= f[0]; o[nt][d][3] *= f[1]; }
             }
         }
+        float off[NT][2];
 #pragma unroll
-        for (int sub = 0; sub < SUB; sub++) {
-            uint32_t pb[P][NT][2];
+        for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                float x[4];
+            for (int e = 0; e < 2; e++) off[nt][e] = m[nt][e] == -INFINITY ? 0.f : m[nt][e] - LIFT;
+        // the values' scales: of places 2t, 2t + 1, 2t + 8, 2t + 9 of every subtile
+        uint32_t sv[SUB][4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) { x[e] = a4_exp2(fmaf(s[sub][nt][e], sl, -off[nt][e & 1])); l[nt][e & 1] += x[e]; }
+        for (int sub = 0; sub < SUB; sub++)
 #pragma unroll
-                for (int p = 0; p < P; p++) {
-                    pb[p][nt][0] = a4_turn(P == 1 ? a4_pack(x[0], x[1]) : a4_piece(x[0], x[1]));
-                    pb[p][nt][1] = a4_turn(P == 1 ? a4_pack(x[2], x[3]) : a4_piece(x[2], x[3]));
-                }
-            }
-            const int k1 = sub * 16 + place_a, k2 = sub * 16 + place_b;              // places 2t, 2t + 1; 8 further: 2t + 8, 2t + 9
-            uint32_t w[4][VW];
+            for (int c = 0; c < 4; c++) sv[sub][c] = a4_lds16(st + (c & 1 ? vsb_at : vsa_at) + (sub * 16 + 8 * (c >> 1)) * SCALES);
+        if (edge) {
+            // What lies behind the last key or ahead of the window may be anything, scales that are no numbers too: no row sees it.
+            const bool several = first_pos != last_pos;
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const uint8_t* src = vc + ((c & 1 ? k2 : k1) + 8 * (c >> 1)) * CODES + 4 * VW * g;
-                if constexpr (VW == 1) w[c][0] = *reinterpret_cast<const uint32_t*>(src);
-                else if constexpr (VW == 2) { const uint2 x = *reinterpret_cast<const uint2*>(src); w[c][0] = x.x; w[c][1] = x.y; }
-                else { const uint4 x = *reinterpret_cast<const uint4*>(src); w[c][0] = x.x; w[c][1] = x.y; w[c][2] = x.z; w[c][3] = x.w; }
-            }
-            uint32_t sv[4];
-#pragma unroll
-            for (int c = 0; c < 4; c++) sv[c] = *reinterpret_cast<const unsigned short*>(vs + ((c & 1 ? k2 : k1) + 8 * (c >> 1)) * SCALES + 2 * vgroup);
-            if (edge) {
-                // What lies behind the last key or ahead of the window may be anything, scales that are no numbers too: no row sees it.
+            for (int sub = 0; sub < SUB; sub++) {
                 uint32_t none = 0;
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    const int at = (c & 1 ? k2 : k1) + 8 * (c >> 1), key = k0 + at;
-                    if (!xr_sees(key, walk.hi, walk.lo, a.keep)) sv[c] = 0;
-                    if ((sv[c] & 0x7f80) == 0x7f80) none |= 1u << (at & 15);
+                    const int at = (c & 1 ? place_b : place_a) + 8 * (c >> 1);
+                    if (!xr_sees(k0 + sub * 16 + at, walk.hi, walk.lo, a.keep)) sv[sub][c] = 0;
+                    if (several && (sv[sub][c] & 0x7f80) == 0x7f80) { none |= 1u << at; sv[sub][c] = 0; }
                 }
-                if (first_pos != last_pos && __any_sync(0xffffffffu, none != 0)) {
-                    // A value that is no number, and rows of several positions, some of which may not see it: it is left out of the
-                    // products, and the elements of its group become NaN for the rows that do see it.
+                if (__any_sync(0xffffffffu, none != 0)) {
+                    // A value that is no number, and rows of several positions, some of which may not see it: it is left out of the products, and the
+                    // elements of its group become NaN for the rows that do see it.
                     none |= __shfl_xor_sync(0xffffffffu, none, 1);
                     none |= __shfl_xor_sync(0xffffffffu, none, 2);
-#pragma unroll
-                    for (int c = 0; c < 4; c++)
-                        if ((sv[c] & 0x7f80) == 0x7f80) sv[c] = 0;
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -459,38 +559,97 @@ k_kv4_attention(A4Args a) {
                         }
                 }
             }
-            const uint32_t s0 = sv[0] | (sv[1] << 16), s1 = sv[2] | (sv[3] << 16), m0 = kv4_m24(s0), m1 = kv4_m24(s1);
+        }
+        // bfloat16 queries: values are multiplied in float16, in units of v_unit, a power of two: scales within 2^-20 .. 248 units make values that are exact.  The
+        // unit is chosen by the first tile with values that are not zero (2^6 times its largest scale), and again where a scale outgrows it.
+        uint32_t v_scale[F32 ? 1 : SUB][2];                            // pairs of scales in float16
+        if constexpr (!F32) {
+            float vs[SUB][4], top = 0.f;
 #pragma unroll
-            for (int j = 0; j < VW; j++) {
-                // the halves of two keys' words side by side: pair i of them is element 2i (low halves) or 2i + 1 of both keys
-                const uint32_t lo0 = __byte_perm(w[0][j], w[1][j], 0x5410), hi0 = __byte_perm(w[0][j], w[1][j], 0x7632);
-                const uint32_t lo1 = __byte_perm(w[2][j], w[3][j], 0x5410), hi1 = __byte_perm(w[2][j], w[3][j], 0x7632);
-#define A4_VALUES(I)                                                                                                                              \
-                {                                                                                                                                 \
-                    const uint32_t a0 = kv4_scaled(kv4_pair<I>(lo0), s0, m0), a1 = kv4_scaled(kv4_pair<I>(hi0), s0, m0);                          \
-                    const uint32_t a2 = kv4_scaled(kv4_pair<I>(lo1), s1, m1), a3 = kv4_scaled(kv4_pair<I>(hi1), s1, m1);                          \
-                    _Pragma("unroll") for (int p = P - 1; p >= 0; p--)                                                                            \
-                        _Pragma("unroll") for (int nt = 0; nt < NT; nt++) a4_mma(o[nt][4 * j + I], a0, a1, a2, a3, pb[p][nt][0], pb[p][nt][1]);   \
+            for (int sub = 0; sub < SUB; sub++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) { vs[sub][c] = __uint_as_float(sv[sub][c] << 16) * v_inv; top = fmaxf(top, fabsf(vs[sub][c])); }
+            if (__any_sync(0xffffffffu, top > v_most)) {
+                top = xr_warp_max(top);
+                const float grow = __int_as_float(((int)(__float_as_uint(top) >> 23) + 6) << 23), less = __int_as_float((254 - (int)(__float_as_uint(top) >> 23) - 6) << 23);
+                v_unit *= grow; v_inv *= less; v_most = 248.f;
+#pragma unroll
+                for (int sub = 0; sub < SUB; sub++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) vs[sub][c] *= less;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int d = 0; d < MT; d++) { o[nt][d][0] *= less; o[nt][d][1] *= less; o[nt][d][2] *= less; o[nt][d][3] *= less; }
+            }
+#pragma unroll
+            for (int sub = 0; sub < SUB; sub++) { v_scale[sub][0] = a4_pack_half(vs[sub][0], vs[sub][1]); v_scale[sub][1] = a4_pack_half(vs[sub][2], vs[sub][3]); }
+        }
+#pragma unroll
+        for (int sub = 0; sub < SUB; sub++) {
+            uint32_t pb[P][NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) { x[e] = a4_exp2(fmaf(s[sub][nt][e], unit[nt][e & 1], -off[nt][e & 1])); l[nt][e & 1] += x[e]; }
+#pragma unroll
+                for (int p = 0; p < P; p++) {
+                    pb[p][nt][0] = a4_turn(F32 ? a4_piece(x[0], x[1]) : a4_pack_half(x[0], x[1]));
+                    pb[p][nt][1] = a4_turn(F32 ? a4_piece(x[2], x[3]) : a4_pack_half(x[2], x[3]));
                 }
-                A4_VALUES(0) A4_VALUES(1) A4_VALUES(2) A4_VALUES(3)
+            }
+            uint32_t w[4][VW];
+#pragma unroll
+            for (int c = 0; c < 4; c++) a4_lds<VW>(w[c], st + (c & 1 ? vb_at : va_at) + (sub * 16 + 8 * (c >> 1)) * CODES);
+            if constexpr (!F32) {
+                const uint32_t s0 = v_scale[sub][0], s1 = v_scale[sub][1];
+                // -264 s and -24 s (11 and 7 bits: exact)
+                const uint32_t m0[2] = {a4_mul_half(s0, 0xDC20DC20u), a4_mul_half(s0, 0xCE00CE00u)}, m1[2] = {a4_mul_half(s1, 0xDC20DC20u), a4_mul_half(s1, 0xCE00CE00u)};
+#pragma unroll
+                for (int j = 0; j < VW; j++) {
+                    // the halves of two keys' words side by side: pair i of them is element 2i (low halves) or 2i + 1 of both keys
+                    uint32_t lo0[4], hi0[4], lo1[4], hi1[4];
+                    a4_pairs(__byte_perm(w[0][j], w[1][j], 0x5410), lo0);
+                    a4_pairs(__byte_perm(w[0][j], w[1][j], 0x7632), hi0);
+                    a4_pairs(__byte_perm(w[2][j], w[3][j], 0x5410), lo1);
+                    a4_pairs(__byte_perm(w[2][j], w[3][j], 0x7632), hi1);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t a0 = a4_fma_half(lo0[i], s0, m0[i & 1]), a1 = a4_fma_half(hi0[i], s0, m0[i & 1]);
+                        const uint32_t a2 = a4_fma_half(lo1[i], s1, m1[i & 1]), a3 = a4_fma_half(hi1[i], s1, m1[i & 1]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) a4_mma_half(o[nt][4 * j + i], a0, a1, a2, a3, pb[0][nt][0], pb[0][nt][1]);
+                    }
+                }
+            } else {
+                const uint32_t s0 = sv[sub][1] * 65536u + sv[sub][0], s1 = sv[sub][3] * 65536u + sv[sub][2], m0 = kv4_m24(s0), m1 = kv4_m24(s1);
+#pragma unroll
+                for (int j = 0; j < VW; j++) {
+                    const uint32_t lo0 = __byte_perm(w[0][j], w[1][j], 0x5410), hi0 = __byte_perm(w[0][j], w[1][j], 0x7632);
+                    const uint32_t lo1 = __byte_perm(w[2][j], w[3][j], 0x5410), hi1 = __byte_perm(w[2][j], w[3][j], 0x7632);
+#define A4_VALUES(I)                                                                                                                              \
+                    {                                                                                                                             \
+                        const uint32_t a0 = kv4_scaled(kv4_pair<I>(lo0), s0, m0), a1 = kv4_scaled(kv4_pair<I>(hi0), s0, m0);                      \
+                        const uint32_t a2 = kv4_scaled(kv4_pair<I>(lo1), s1, m1), a3 = kv4_scaled(kv4_pair<I>(hi1), s1, m1);                      \
+                        _Pragma("unroll") for (int p = P - 1; p >= 0; p--)                                                                        \
+                            _Pragma("unroll") for (int nt = 0; nt < NT; nt++) a4_mma(o[nt][4 * j + I], a0, a1, a2, a3, pb[p][nt][0], pb[p][nt][1]); \
+                    }
+                    A4_VALUES(0) A4_VALUES(1) A4_VALUES(2) A4_VALUES(3)
 #undef A4_VALUES
+                }
             }
         }
         __syncwarp();
-        if (lane == 0 && i + A4_STAGES * A4_WARPS < i_end) fetch(i + A4_STAGES * A4_WARPS, stage);
-        if (++stage == A4_STAGES) { stage = 0; phase ^= 1; }
-    }
-    if (lost && lane == 0) {
-        // a copy did not arrive: what is still in flight is waited for (within the same limit) before the block may end
-        *gave_up = 1;
-        for (int s = 1; s < A4_STAGES; s++) {
-            if (++stage == A4_STAGES) { stage = 0; phase ^= 1; }
-            a4_wait(&my_bars[stage], phase);
+        if (i + STAGES * A4_WARPS < i_end) {
+            fetch(i + STAGES * A4_WARPS, stage, next_page);
+            next_page = tiles_page(i + (STAGES + 1) * A4_WARPS);
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (++stage == STAGES) stage = 0;
     }
     // the warps' sums meet in the ring's memory: [warp][row][HS], then [warp][row] (maximum, sum)
     __syncthreads();
-    if (threadIdx.x == 0 && *gave_up) atomicExch(a.status, 5);
     float* acc_s = reinterpret_cast<float*>(smem);
     float* ml_s = acc_s + A4_WARPS * RB * HS;
 #pragma unroll
@@ -504,10 +663,10 @@ k_kv4_attention(A4Args a) {
             float* dst = acc_s + (warp * RB + r) * HS + 8 * VW * g;
 #pragma unroll
             for (int j = 0; j < VW; j++) {
-                *reinterpret_cast<float4*>(dst + 8 * j) = make_float4(o[nt][4 * j][e], o[nt][4 * j][e + 2], o[nt][4 * j + 1][e], o[nt][4 * j + 1][e + 2]);
-                *reinterpret_cast<float4*>(dst + 8 * j + 4) = make_float4(o[nt][4 * j + 2][e], o[nt][4 * j + 2][e + 2], o[nt][4 * j + 3][e], o[nt][4 * j + 3][e + 2]);
+                *reinterpret_cast<float4*>(dst + 8 * j) = make_float4(o[nt][4 * j][e] * v_unit, o[nt][4 * j][e + 2] * v_unit, o[nt][4 * j + 1][e] * v_unit, o[nt][4 * j + 1][e + 2] * v_unit);
+                *reinterpret_cast<float4*>(dst + 8 * j + 4) = make_float4(o[nt][4 * j + 2][e] * v_unit, o[nt][4 * j + 2][e + 2] * v_unit, o[nt][4 * j + 3][e] * v_unit, o[nt][4 * j + 3][e + 2] * v_unit);
             }
-            if (g == 0) { ml_s[(warp * RB + r) * 2] = m[nt][e]; ml_s[(warp * RB + r) * 2 + 1] = sum; }
+            if (g == 0) { ml_s[(warp * RB + r) * 2] = m[nt][e] - LIFT; ml_s[(warp * RB + r) * 2 + 1] = sum; }
         }
     __syncthreads();
     const size_t item = ((size_t)seg * gridDim.y + blockIdx.y) * a.splits + span;
@@ -540,6 +699,8 @@ k_kv4_attention(A4Args a) {
 // ---------------------------------------------------------------------------------------------
 #define A4_MERGE_THREADS 512
 #define A4_MAX_SPLITS 256
+#define A4_START 1.5
+#define A4_MERGE 1.3
 template <int NG, int RB, bool F32>
 __global__ void __launch_bounds__(A4_MERGE_THREADS)
 k_kv4_merge(A4Args a) {
@@ -604,8 +765,8 @@ k_kv4_merge(A4Args a) {
 // ---------------------------------------------------------------------------------------------
 // Blocks that are resident at once, and a row block's size, for a head size and type.  wide_rows: some request has more than eight packed rows.
 static int a4_rows(int f32, int wide_rows) { return f32 || !wide_rows ? 8 : 16; }
-static int a4_resident(int hs, int f32, int wide_rows) { return (hs <= 128 && !f32 && !wide_rows ? 4 : 2) * xr_sm_count(); }
-static int a4_tile(int hs) { return hs == 64 ? 64 : 32; }
+static int a4_resident(int hs, int f32, int wide_rows) { return (hs <= 128 && !f32 && !wide_rows ? 3 : 2) * xr_sm_count(); }
+static int a4_tile(int hs) { return hs <= 128 ? 64 : 32; }
 
 // How a step is cut: row blocks of the longest portion that is taken (at most `most_rows` packed rows), tiles a span, spans of the longest
 // request.  len, pos0: the portions on the HOST; max_kv: the longest key range to be prepared for (0: what the portions say).
@@ -621,38 +782,56 @@ static A4Plan a4_plan(const int* len, const int* pos0, int n_seg, int K, int G, 
     if (rows < 1) return p;
     const int rb = a4_rows(f32, p.wide);
     p.row_blocks = (int)((rows + rb - 1) / rb);
-    long long total = 0, longest = 1;
-    for (int s = 0; s < n_seg; s++) {
-        const long long r = (long long)len[s] * G;
-        if (len[s] < 1 || r > most_rows) continue;
-        // (tiles of the last row block, whose window is the furthest)
-        const long long end = (long long)pos0[s] + len[s];
-        const long long lo = window > 0 && end - len[s] - window + 1 > 0 ? end - len[s] - window + 1 : 0;
-        const long long tiles = (end - 1) / tile - lo / tile + 1 + xr_kept_tiles(keep, (int)lo, tile);
-        total += tiles * K * ((r + rb - 1) / rb);
-        longest = tiles > longest ? tiles : longest;
-    }
+    long long longest = 1, lone = 0;
+    const long long resident = a4_resident(hs, f32, p.wide);
+    // (tiles of a portion's last row block, whose window is the furthest)
+    auto tiles_of = [&](int s) {
+        const long long end = (long long)pos0[s] + len[s], lo = window > 0 && end - len[s] - window + 1 > 0 ? end - len[s] - window + 1 : 0;
+        return (end - 1) / tile - lo / tile + 1 + xr_kept_tiles(keep, (int)lo, tile);
+    };
+    auto taken = [&](int s) { return len[s] >= 1 && (long long)len[s] * G <= most_rows; };
+    for (int s = 0; s < n_seg; s++)
+        if (taken(s)) {
+            const long long t = tiles_of(s);
+            longest = t > longest ? t : longest;
+            lone += K * (((long long)len[s] * G + rb - 1) / rb);
+        }
     if (max_kv > 0) {
         const long long range = window > 0 && window + 16 < max_kv ? window + 16 : max_kv;
-        const long long tiles = (range + tile - 1) / tile + 1 + (window > 0 ? (keep + tile - 1) / tile : 0);
-        longest = tiles > longest ? tiles : longest;
+        const long long t = (range + tile - 1) / tile + 1 + (window > 0 ? (keep + tile - 1) / tile : 0);
+        longest = t > longest ? t : longest;
     }
-    // as many tiles a span as give every resident block one span, a multiple of the warps
-    const long long resident = a4_resident(hs, f32, p.wide);
-    long long span = (total + resident - 1) / resident;
-    span = (span + A4_WARPS - 1) / A4_WARPS * A4_WARPS;
-    const long long least = ((longest + A4_MAX_SPLITS - 1) / A4_MAX_SPLITS + A4_WARPS - 1) / A4_WARPS * A4_WARPS;
-    if (span < least) span = least;
-    if (span < A4_WARPS) span = A4_WARPS;
-    p.span_tiles = (int)span;
-    p.splits = (int)((longest + span - 1) / span);
+    // Tiles a warp of a span takes: the number whose last block is done first, in the time of a tile (a warp's, all others at work).  Up to `resident` blocks
+    // run at once; blocks of one length go in rounds, blocks of many lengths as slots fall free, half a block of which is idle at the end.  A block
+    // costs A4_START beside its tiles (its first tiles are on their way), combining spans A4_MERGE.
+    const long long most = (longest + A4_WARPS - 1) / A4_WARPS, least = (longest + A4_MAX_SPLITS * A4_WARPS - 1) / (A4_MAX_SPLITS * A4_WARPS);
+    long long best = most;
+    double best_cost = -1.0;
+    for (long long n = most; n >= least && n >= 1; n = n > 48 ? n - n / 24 : n - 1) {
+        long long blocks = 0;
+        double tiles = 0.0;
+        for (int s = 0; s < n_seg; s++)
+            if (taken(s)) {
+                const long long of = K * (((long long)len[s] * G + rb - 1) / rb), t = tiles_of(s);
+                blocks += of * ((t + n * A4_WARPS - 1) / (n * A4_WARPS));
+                tiles += (double)of * t;
+            }
+        const double work = tiles / A4_WARPS + A4_START * blocks;
+        const bool alike = tiles > 0.85 * (double)blocks * n * A4_WARPS;
+        double cost = blocks <= resident ? n + A4_START : alike ? (double)((blocks + resident - 1) / resident) * (n + A4_START) : work / resident + 0.5 * (n + A4_START);
+        if (n < most) cost += A4_MERGE;
+        if (best_cost < 0.0 || cost < best_cost) { best_cost = cost; best = n; }
+        if (work / resident > 1.5 * best_cost) break;
+    }
+    p.span_tiles = (int)(best * A4_WARPS);
+    p.splits = (int)((longest + p.span_tiles - 1) / p.span_tiles);
     return p;
 }
 
 template <int NG, int NT, bool F32, bool EXTRA>
 static int a4_launch(const A4Args& a, int n_seg, cudaStream_t stream) {
     using S = A4Shape<NG, NT, F32, EXTRA>;
-    static_assert(A4_WARPS * S::RB * (S::HS + 2) * 4 <= A4_WARPS * A4_STAGES * S::STAGE, "the warps' sums lie in the ring");
+    static_assert(A4_WARPS * S::RB * (S::HS + 2) * 4 <= A4_WARPS * S::STAGES * S::STAGE, "the warps' sums lie in the ring");
     static bool ready[XR_DEVICES];
     if (!xr_once_per_device(ready, [] { return xr_allow_smem(k_kv4_attention<NG, NT, F32, EXTRA>, S::SMEM); })) return XR_ERR_LAUNCH;
     xr_launch((k_kv4_attention<NG, NT, F32, EXTRA>), dim3(a.splits, a.c.K * a.row_blocks, n_seg), dim3(A4_THREADS), S::SMEM, stream, a);
@@ -669,14 +848,36 @@ static int a4_launch(const A4Args& a, int n_seg, int f32, int wide, cudaStream_t
     return f32 ? a4_launch<NG, 1, true>(a, n_seg, stream) : wide ? a4_launch<NG, 2, false>(a, n_seg, stream) : a4_launch<NG, 1, false>(a, n_seg, stream);
 }
 
-// float32 values of scratch that xr_kv4_attention needs for these portions (host arrays len, pos0), 0 if none.
-XR_EXPORT long long xr_kv4_attention_floats(const int* len, const int* pos0, int n_seg, int K, int G, int D, int dtype, int window, int keep, int most_rows,
-                                            int max_kv) {
-    if (n_seg < 1 || K < 1 || G < 1 || D < 1 || D > 256) return 0;
-    const int hs = kv4_held(D), f32 = dtype == XR_F32;
-    const A4Plan p = a4_plan(len, pos0, n_seg, K, G, hs, f32, window, window > 0 ? keep : 0, most_rows, max_kv);
-    if (p.row_blocks < 1 || p.splits < 2) return 0;
-    return (long long)n_seg * K * p.row_blocks * p.splits * a4_rows(f32, p.wide) * (hs + 2);
+// What a step's portions ask for, from their lengths and first positions on the HOST: said[0] portions of 1 to `most_rows` packed rows, [1] longer ones,
+// [2] float32 values of scratch that xr_kv4_attention needs for the short ones; of the longer ones [3] the pages that xr_kv4_read writes for
+// them, [4] the most tokens, [5], [6] the row tiles of 128 and 64 packed rows, [7] the furthest end.  n: tokens of the step.
+XR_EXPORT int xr_kv4_plan(const int* len, const int* pos0, int n_seg, int n, int K, int G, int D, int page_size, int dtype, int window, int keep_first,
+                          int most_rows, int max_kv, long long* said) {
+    if (n_seg < 1 || n < 0 || K < 1 || G < 1 || D < 1 || D > 256 || page_size < 1 || window < 0 || keep_first < 0 || most_rows < 0) return XR_ERR_ARG;
+    long long tokens = 0;
+    for (int i = 0; i < 8; i++) said[i] = 0;
+    for (int s = 0; s < n_seg; s++) {
+        const long long l = len[s], p = pos0[s], rows = l * G;
+        if (l < 0 || p < 0) return XR_ERR_ARG;
+        tokens += l;
+        if (l == 0) continue;
+        if (rows <= most_rows) { said[0]++; continue; }
+        said[1]++;
+        const long long first = window > 0 && p - window + 1 > 0 ? p - window + 1 : 0, from = first / page_size;
+        const long long kept = ((long long)keep_first + page_size - 1) / page_size;
+        said[3] += (window > 0 ? (kept < from ? kept : from) : 0) + (p + l - 1) / page_size - from + 1;
+        if (l > said[4]) said[4] = l;
+        said[5] += (rows + 127) / 128;
+        said[6] += (rows + 63) / 64;
+        if (p + l > said[7]) said[7] = p + l;
+    }
+    if (tokens > n) return XR_ERR_ARG;
+    if (said[0] > 0) {
+        const int hs = kv4_held(D), f32 = dtype == XR_F32;
+        const A4Plan p = a4_plan(len, pos0, n_seg, K, G, hs, f32, window, window > 0 ? keep_first : 0, most_rows, max_kv);
+        if (p.splits > 1) said[2] = (long long)n_seg * K * p.row_blocks * p.splits * a4_rows(f32, p.wide) * (hs + 2);
+    }
+    return XR_OK;
 }
 
 // q: token t, head h at q + t * q_stride + h * D; out [n][H * D], both of `dtype`.  Portions of at most `most_rows` packed rows (tokens x heads per
@@ -684,11 +885,11 @@ XR_EXPORT long long xr_kv4_attention_floats(const int* len, const int* pos0, int
 // size the grid; what is computed goes by the device's).
 XR_EXPORT int xr_kv4_attention(const void* q, void* out, int dtype, const void* cache, long long n_pages, int layers, int layer, int K, int block, int page_size,
                                const int* seg_start, const int* seg_len, const int* seg_pos0, const int* block_tables, const int* len, const int* pos0,
-                               float* scratch, long long floats, int* status, long long q_stride, int n_seg, int H, int D, int max_pages, int window,
+                               float* scratch, long long floats, long long q_stride, int n_seg, int H, int D, int max_pages, int window,
                                float scale, const float* sink, float softcap, int keep_first, const float* bias, int bias_len, int most_rows, int max_kv,
                                cudaStream_t stream) {
     if (n_seg < 1 || n_seg > 65535 || H < 1 || H % K != 0 || max_pages < 1 || window < 0 || keep_first < 0 || !(scale > 0.f) || !(softcap >= 0.f) ||
-        (bias != nullptr && (bias_len < 1 || softcap > 0.f)) || status == nullptr || most_rows < 1 || max_kv < 0 || q_stride < (long long)H * D ||
+        (bias != nullptr && (bias_len < 1 || softcap > 0.f)) || most_rows < 1 || max_kv < 0 || q_stride < (long long)H * D ||
         (dtype != XR_F32 && dtype != XR_BF16) || !kv4_cache_ok(cache, n_pages, layers, layer, K, block, page_size, D) ||
         (long long)max_pages * page_size > 0x7fffffffLL - 64)
         return XR_ERR_ARG;
@@ -699,7 +900,7 @@ XR_EXPORT int xr_kv4_attention(const void* q, void* out, int dtype, const void* 
     const long long items = (long long)n_seg * K * p.row_blocks * p.splits, rb = a4_rows(f32, p.wide);
     if (p.splits > 1 && (scratch == nullptr || ((uintptr_t)scratch & 15) || floats < items * rb * (hs + 2))) return XR_ERR_ARG;
     A4Args a{q, out, kv4_cache(cache, n_pages, layers, layer, K, page_size, D), seg_start, seg_len, seg_pos0, block_tables, scratch,
-             scratch + items * rb * hs, status, q_stride, H, G, D, max_pages, window, keep, p.splits, p.span_tiles, p.row_blocks, most_rows,
+             scratch + items * rb * hs, q_stride, H, G, D, max_pages, window, keep, p.splits, p.span_tiles, p.row_blocks, most_rows,
              scale, softcap, sink, {bias, bias_len}, 0, 0, -1};
     a.wide = D % 8 == 0 && q_stride % 8 == 0 && !((uintptr_t)q & 15);
     a.wide_out = D % 4 == 0 && !((uintptr_t)out & 15);

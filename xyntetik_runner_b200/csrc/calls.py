@@ -13,14 +13,21 @@ from __future__ import annotations
 
 from .signatures import LONG, SIGNATURES
 
-_TYPES = {"p": "void*", "i": "int", "l": "long long", "f": "float", "u": "unsigned", "U": "unsigned long long", "o": "int*"}
+_TYPES = {"p": "void*", "i": "int", "l": "long long", "f": "float", "u": "unsigned", "U": "unsigned long long", "o": "int*", "b": "void*"}
 _READ = {"p": "xr_pointer", "i": "(int)PyLong_AsLong", "l": "PyLong_AsLongLong", "f": "(float)PyFloat_AsDouble", "u": "(unsigned)PyLong_AsUnsignedLong",
-         "U": "PyLong_AsUnsignedLongLong"}
+         "U": "PyLong_AsUnsignedLongLong", "b": "xr_buffer"}
 
 _HEAD = """#define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <dlfcn.h>
 static inline void* xr_pointer(PyObject* o) { return o == Py_None ? nullptr : (void*)PyLong_AsUnsignedLongLong(o); }
+static inline void* xr_buffer(PyObject* o) {
+    Py_buffer view;                                  // (the caller holds the object while the launcher runs)
+    if (PyObject_GetBuffer(o, &view, PyBUF_SIMPLE) != 0) return nullptr;
+    void* at = view.buf;
+    PyBuffer_Release(&view);
+    return at;
+}
 """
 
 

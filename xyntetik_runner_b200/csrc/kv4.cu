@@ -16,7 +16,12 @@ struct Kv4StoreArgs {
     Kv4Cache c;
     int n, D, Vd, n_seg, max_pages;
     int wide;                            // rows, heads and addresses allow 16-byte loads
+    int word_shift;                      // log2 of the words of a held head
 };
+
+// A maximum and a minimum that keep a NaN.
+__device__ __forceinline__ float kv4_max(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float kv4_min(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 
 // s of a group from its largest and smallest element (kv4.cuh)
 __device__ __forceinline__ float kv4_scale_of(float hi, float lo) {
@@ -29,87 +34,102 @@ __device__ __forceinline__ float kv4_scale_of(float hi, float lo) {
     return -0.125f * __int_as_float(b);
 }
 
-template <typename T>
-__device__ __forceinline__ void kv4_load8(const T* src, int live, bool wide, float* x) {
-    if (wide && live == 8) {
-        if constexpr (sizeof(T) == 2) {
-            const uint4 r = *reinterpret_cast<const uint4*>(src);
-            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+// Eight elements in two steps, so that a thread's loads are all on their way before the first is used.
+template <typename T> struct Kv4Row8;
+template <> struct Kv4Row8<__nv_bfloat16> {
+    uint4 r;
+    __device__ __forceinline__ void load(const __nv_bfloat16* src, int live, bool wide) {
+        r = make_uint4(0, 0, 0, 0);
+        if (wide) { if (live > 0) r = *reinterpret_cast<const uint4*>(src); return; }
+        uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-        } else {
-            const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
-            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-        }
-        return;
+        for (int i = 0; i < 8; i++)
+            if (i < live) w[i >> 1] |= (uint32_t)reinterpret_cast<const unsigned short*>(src)[i] << (16 * (i & 1));
+        r = make_uint4(w[0], w[1], w[2], w[3]);
     }
+    __device__ __forceinline__ void get(float* x) const {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = i < live ? xr_to_f32<T>(src[i]) : 0.f;
+        for (int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    }
+};
+template <> struct Kv4Row8<float> {
+    float4 p, q;
+    __device__ __forceinline__ void load(const float* src, int live, bool wide) {
+        p = q = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (wide) { if (live > 0) { p = reinterpret_cast<const float4*>(src)[0]; q = reinterpret_cast<const float4*>(src)[1]; } return; }
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = i < live ? src[i] : 0.f;
+        p = make_float4(x[0], x[1], x[2], x[3]); q = make_float4(x[4], x[5], x[6], x[7]);
+    }
+    __device__ __forceinline__ void get(float* x) const { x[0] = p.x; x[1] = p.y; x[2] = p.z; x[3] = p.w; x[4] = q.x; x[5] = q.y; x[6] = q.z; x[7] = q.w; }
+};
+
+// The word of eight elements with scale s (finite, not zero).  The codes hang on x / s rounded to the nearest whole number, and quotients of exactly n + 1/2 are
+// common (x has eight bits, s five), so the quotient has to be the correctly rounded one: r the correctly rounded 1 / s, q = x r, and q + (x - q s) r
+// with fused operations is it (Markstein, IBM J. Res. Dev. 34, 1990).  Codes come out of the low bits of 1.5 2^23 + 8 + c; the constant's bits, shifted
+// and added up like the codes', are taken off at the end.
+__device__ __forceinline__ uint32_t kv4_word(const float* x, float s) {
+    const float r = __frcp_rn(s);
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float q = x[i] * r, c = fmaf(fmaf(-q, s, x[i]), r, q);
+        word += __float_as_uint(fminf(fmaxf(c, -8.f), 7.f) + 12582920.f) << (4 * (i >> 1) + 16 * (i & 1));
+    }
+    return word - 0x4B400000u * 0x11111111u;
 }
 
+// grid (tokens, 256 words of a token)
 template <typename T>
 __global__ void __launch_bounds__(256)
 k_kv4_store(Kv4StoreArgs a) {
     xr_pdl_launch();
-    xr_pdl_wait();
-    const int words = a.c.hs >> 3;
-    const long long at = (long long)blockIdx.x * 256 + threadIdx.x, total = (long long)a.n * 2 * a.c.K * words;
-    const bool live = at < total;
-    // (groups are whole: a head's words are a multiple of four, and so are the threads behind the last one)
-    const int w = (int)(at % words);
-    const long long head = live ? at / words : 0;
-    const int t = (int)(head / (2 * a.c.K)), r = (int)(head % (2 * a.c.K)), plane = r >= a.c.K, kvh = r - plane * a.c.K;
-    const int pos = a.positions[t], seg = a.tok_seg[t];
-    const int pi = pos / a.c.page_size;
-    int page = -1;
-    if (live && pos >= 0 && seg >= 0 && seg < a.n_seg && pi < a.max_pages) page = a.block_tables[(size_t)seg * a.max_pages + pi];
-    if (page >= a.c.n_pages) page = -1;                    // (a token whose page is not held is not written)
-    const int D = plane ? a.Vd : a.D;
-    float x[8];
+    const int words = 1 << a.word_shift, per = 2 * a.c.K << a.word_shift;       // words of a head; of a token
+    const int u = blockIdx.y * 256 + threadIdx.x, t = blockIdx.x;
+    // (groups are whole: a token's words are a multiple of four)
+    const bool live = u < per;
+    const int w = u & (words - 1), r = u >> a.word_shift, plane = r >= a.c.K, kvh = r - (plane ? a.c.K : 0), D = plane ? a.Vd : a.D;
     const T* src = plane ? (const T*)a.v + (long long)t * a.v_stride + (long long)kvh * D + 8 * w : (const T*)a.k + (long long)t * a.k_stride + (long long)kvh * D + 8 * w;
-    kv4_load8<T>(src, page >= 0 ? min(8, max(0, D - 8 * w)) : 0, a.wide, x);
+    xr_pdl_wait();
+    Kv4Row8<T> row;
+    row.load(src, live ? min(8, max(0, D - 8 * w)) : 0, a.wide);
+    const int pos = a.positions[t], seg = a.tok_seg[t];
+    const int pi = pos / a.c.page_size, tok = pos - pi * a.c.page_size;
+    int page = -1;
+    if (pos >= 0 && seg >= 0 && seg < a.n_seg && pi < a.max_pages) page = a.block_tables[(size_t)seg * a.max_pages + pi];
+    float x[8];
+    row.get(x);
     float hi = x[0], lo = x[0];
-    bool none = !(fabsf(x[0]) <= 3.402823466e38f);
 #pragma unroll
-    for (int i = 1; i < 8; i++) { hi = fmaxf(hi, x[i]); lo = fminf(lo, x[i]); none |= !(fabsf(x[i]) <= 3.402823466e38f); }
-    // (maximum and minimum pass a NaN over: it is looked for apart, and an infinity with it)
-    if (none) hi = INFINITY;
+    for (int i = 1; i < 8; i++) { hi = kv4_max(hi, x[i]); lo = kv4_min(lo, x[i]); }
 #pragma unroll
     for (int o = 1; o <= 2; o <<= 1) {
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = kv4_max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        lo = kv4_min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
     }
-    if (page < 0) return;
+    if (!live || page < 0 || page >= a.c.n_pages) return;  // (a token whose page is not held is not written)
     const float s = kv4_scale_of(hi, lo);
-    uint32_t word = 0x88888888u;                           // c = 0 everywhere
-    if (s != 0.f && s == s) {
-        word = 0;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            // a true division: x has eight bits (or 24), s five, and halves between two codes occur; a product with 1 / s may land on their other side
-            const int c = (int)fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -8.f), 7.f);
-            word |= (uint32_t)(c + 8) << (4 * (i >> 1) + 16 * (i & 1));
-        }
-    }
+    const uint32_t word = s != 0.f && s == s ? kv4_word(x, s) : 0x88888888u;       // (c = 0 everywhere)
     uint8_t* run = const_cast<uint8_t*>(a.c.run(page, kvh));
-    const int tok = pos % a.c.page_size;
-    reinterpret_cast<uint32_t*>(run + a.c.codes_at(plane))[(long long)tok * words + w] = word;
-    if ((w & 3) == 0) reinterpret_cast<__nv_bfloat16*>(run + a.c.scales_at(plane))[(long long)tok * (words >> 2) + (w >> 2)] = __float2bfloat16_rn(s);
+    reinterpret_cast<uint32_t*>(run + a.c.codes_at(plane))[(tok << a.word_shift) + w] = word;
+    if ((w & 3) == 0) reinterpret_cast<__nv_bfloat16*>(run + a.c.scales_at(plane))[((tok << a.word_shift) + w) >> 2] = __float2bfloat16_rn(s);
 }
 
 XR_EXPORT int xr_kv4_store(const void* k, const void* v, int dtype, long long k_stride, long long v_stride, const int* positions, const int* tok_seg,
                            const int* block_tables, void* cache, long long n_pages, int layers, int layer, int K, int block, int page_size, int n, int D,
                            int Vd, int n_seg, int max_pages, cudaStream_t stream) {
-    if (n < 1 || Vd < 1 || Vd > 256 || n_seg < 1 || max_pages < 1 || k_stride < (long long)K * D || v_stride < (long long)K * Vd ||
+    if (n < 1 || Vd < 1 || Vd > 256 || n_seg < 1 || max_pages < 1 || K > 16384 || k_stride < (long long)K * D || v_stride < (long long)K * Vd ||
         !kv4_cache_ok(cache, n_pages, layers, layer, K, block, page_size, D > Vd ? D : Vd) || D < 1)
         return XR_ERR_ARG;
     Kv4StoreArgs a{k, v, k_stride, v_stride, positions, tok_seg, block_tables, kv4_cache(cache, n_pages, layers, layer, K, page_size, D > Vd ? D : Vd),
                    n, D, Vd, n_seg, max_pages, 0};
     a.wide = !(((uintptr_t)k | (uintptr_t)v) & 15) && D % 8 == 0 && Vd % 8 == 0 && k_stride % 8 == 0 && v_stride % 8 == 0;
-    const long long blocks = ((long long)n * 2 * K * (a.c.hs >> 3) + 255) / 256;
-    if (blocks > 0x7fffffffLL) return XR_ERR_ARG;
-    if (dtype == XR_F32) xr_launch((k_kv4_store<float>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
-    else if (dtype == XR_BF16) xr_launch((k_kv4_store<__nv_bfloat16>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    a.word_shift = a.c.hs == 64 ? 3 : a.c.hs == 128 ? 4 : 5;
+    const dim3 grid(n, (unsigned)(((2LL * K << a.word_shift) + 255) / 256));
+    if (dtype == XR_F32) xr_launch((k_kv4_store<float>), grid, dim3(256), 0, stream, a);
+    else if (dtype == XR_BF16) xr_launch((k_kv4_store<__nv_bfloat16>), grid, dim3(256), 0, stream, a);
     else return XR_ERR_ARG;
     return xr_launch_status();
 }
@@ -140,13 +160,31 @@ __device__ __forceinline__ void kv4_pages_of(const Kv4ReadArgs& a, int seg, int&
     count = f < e ? (e - 1) / P - from + 1 : 0;
 }
 
+__device__ __forceinline__ void kv4_values(uint32_t word, uint32_t s, uint32_t* v) {
+    const uint32_t s2 = s * 0x10001u, m = kv4_m24(s2);
+    v[0] = kv4_scaled(kv4_pair<0>(word), s2, m); v[1] = kv4_scaled(kv4_pair<1>(word), s2, m);
+    v[2] = kv4_scaled(kv4_pair<2>(word), s2, m); v[3] = kv4_scaled(kv4_pair<3>(word), s2, m);
+}
+// A word's eight values to a 16-byte border.
 template <typename T>
+__device__ __forceinline__ void kv4_eight(uint32_t word, uint32_t s, T* to) {
+    uint32_t v[4];
+    kv4_values(word, s, v);
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
+    else {
+        reinterpret_cast<uint4*>(to)[0] = make_uint4(v[0] << 16, v[0] & 0xffff0000u, v[1] << 16, v[1] & 0xffff0000u);
+        reinterpret_cast<uint4*>(to)[1] = make_uint4(v[2] << 16, v[2] & 0xffff0000u, v[3] << 16, v[3] & 0xffff0000u);
+    }
+}
+
+// WS: log2 of a held head's words where a head is held as it is (D is 8 << WS, on 16-byte borders); 0: any head.
+template <typename T, int WS>
 __global__ void __launch_bounds__(256)
 k_kv4_read(Kv4ReadArgs a) {
     xr_pdl_launch();
-    __shared__ int found[4];
+    __shared__ int found[2];
     xr_pdl_wait();
-    const int j = blockIdx.x, kvh = blockIdx.y;
+    const int j = blockIdx.x;
     if (threadIdx.x < 32) {
         int before = 0;
         bool done = false;
@@ -159,9 +197,12 @@ k_kv4_read(Kv4ReadArgs a) {
             for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, sum, o); if (threadIdx.x >= o) sum += u; }
             const int at = before + sum - kept - count;                  // this request's first page of the output
             const bool mine = seg < a.n_seg && j >= at && j < at + kept + count;
-            if (mine) { const int i = j - at; found[0] = seg; found[1] = i < kept ? i : from + i - kept; }
+            if (mine) {
+                const int i = j - at, pi = i < kept ? i : from + i - kept;
+                found[0] = seg; found[1] = pi;
+                if (blockIdx.y == 0 && a.tables != nullptr) a.tables[(size_t)seg * a.max_pages + pi] = j;
+            }
             done = __ballot_sync(0xffffffffu, mine) != 0;
-            if (kvh == 0 && a.tables != nullptr && mine) a.tables[(size_t)seg * a.max_pages + (j - at < kept ? j - at : from + j - at - kept)] = j;
             before += __shfl_sync(0xffffffffu, sum, 31);
         }
         if (!done && threadIdx.x == 0) found[0] = -1;
@@ -169,40 +210,67 @@ k_kv4_read(Kv4ReadArgs a) {
     __syncthreads();
     const int seg = found[0];
     if (seg < 0) return;                                                 // (more pages of output than the requests take: left as they were)
-    const int pi = found[1], P = a.c.page_size, words = a.c.hs >> 3, used = (a.D + 7) >> 3;
-    const int first = a.first[seg], end = a.end[seg];
+    const int pi = found[1], P = a.c.page_size, first = a.first[seg], end = a.end[seg];
     int page = a.block_tables[(size_t)seg * a.max_pages + pi];
     if (page >= a.c.n_pages) page = -1;
-    const uint8_t* run = a.c.run(max(page, 0), kvh);
-    T* dst = (T*)a.out + ((size_t)j * 2 * a.c.K + kvh) * P * a.D;
+    const int words = a.c.hs >> 3, used = (a.D + 7) >> 3, p0 = pi * P;
     const size_t plane_step = (size_t)a.c.K * P * a.D;
-    const int per_plane = P * used;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < 2 * per_plane; i += 256) {
-        const int plane = i >= per_plane, u = i - plane * per_plane, tok = u / used, w = u - tok * used;
-        const int p = pi * P + tok;
-        const bool seen = page >= 0 && p < end && (p >= first || p < a.keep);
-        uint32_t word = 0, s = 0;
-        if (seen) {
-            word = __ldg(reinterpret_cast<const uint32_t*>(run + a.c.codes_at(plane)) + tok * words + w);
-            s = __ldg(reinterpret_cast<const unsigned short*>(run + a.c.scales_at(plane)) + tok * (words >> 2) + (w >> 2));
-        }
-        const uint32_t s2 = s | (s << 16), m = kv4_m24(s2);
-        const uint32_t v[4] = {kv4_scaled(kv4_pair<0>(word), s2, m), kv4_scaled(kv4_pair<1>(word), s2, m), kv4_scaled(kv4_pair<2>(word), s2, m),
-                               kv4_scaled(kv4_pair<3>(word), s2, m)};
-        T* to = dst + plane * plane_step + (size_t)tok * a.D + 8 * w;
-        if (a.wide) {
-            if constexpr (sizeof(T) == 2) *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
-            else {
-                reinterpret_cast<uint4*>(to)[0] = make_uint4(v[0] << 16, v[0] & 0xffff0000u, v[1] << 16, v[1] & 0xffff0000u);
-                reinterpret_cast<uint4*>(to)[1] = make_uint4(v[2] << 16, v[2] & 0xffff0000u, v[3] << 16, v[3] & 0xffff0000u);
-            }
-        } else {
+    // what of the page is asked for: tokens a0 .. a1 - 1, and the first `kept`
+    const int a0 = max(first - p0, 0), a1 = page >= 0 ? min(end - p0, P) : 0, kept = page >= 0 ? min(a.keep - p0, a1) : 0;
+    for (int kvh = blockIdx.y; kvh < a.c.K; kvh += gridDim.y) {
+        const uint8_t* run = a.c.run(max(page, 0), kvh);
+        T* dst = (T*)a.out + ((size_t)j * 2 * a.c.K + kvh) * P * a.D;
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (8 * w + e < a.D) to[e] = xr_from_f32<T>(__uint_as_float(e & 1 ? v[e >> 1] & 0xffff0000u : v[e >> 1] << 16));
+        for (int plane = 0; plane < 2; plane++) {
+            const uint32_t* codes = reinterpret_cast<const uint32_t*>(run + a.c.codes_at(plane));
+            const unsigned short* scales = reinterpret_cast<const unsigned short*>(run + a.c.scales_at(plane));
+            T* to = dst + plane * plane_step;
+            if constexpr (WS > 0) {
+                // four words a thread, their loads side by side
+                constexpr int N = 4;
+                for (int i0 = threadIdx.x; i0 < P << WS; i0 += N * 256) {
+                    uint32_t word[N], s[N];
+#pragma unroll
+                    for (int e = 0; e < N; e++) {
+                        const int i = i0 + e * 256, tok = i >> WS;
+                        word[e] = s[e] = 0;
+                        if (tok < a1 && (tok >= a0 || tok < kept)) { word[e] = __ldg(codes + i); s[e] = __ldg(scales + (i >> 2)); }
+                    }
+#pragma unroll
+                    for (int e = 0; e < N; e++) {
+                        const int i = i0 + e * 256;
+                        if (i >= P << WS) break;
+                        kv4_eight<T>(word[e], s[e], to + 8 * (size_t)i);
+                    }
+                }
+            } else {
+                for (int i = threadIdx.x; i < P * used; i += 256) {
+                    const int tok = i / used, w = i - tok * used;
+                    uint32_t word = 0, s = 0;
+                    if (tok < a1 && (tok >= a0 || tok < kept)) { word = __ldg(codes + tok * words + w); s = __ldg(scales + tok * (words >> 2) + (w >> 2)); }
+                    if (a.wide) { kv4_eight<T>(word, s, to + (size_t)tok * a.D + 8 * w); continue; }
+                    uint32_t v[4];
+                    kv4_values(word, s, v);
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (8 * w + e < a.D) to[(size_t)tok * a.D + 8 * w + e] = xr_from_f32<T>(__uint_as_float(e & 1 ? v[e >> 1] & 0xffff0000u : v[e >> 1] << 16));
+                }
+            }
         }
     }
+}
+
+template <typename T>
+static void kv4_launch_read(const Kv4ReadArgs& a, cudaStream_t stream) {
+    // A block takes one page and as many of its kv heads as leave six blocks an SM: what a block works out about its page costs more than a head's values.
+    const long long want = 6LL * xr_sm_count();
+    const int heads = (int)(a.out_pages * (long long)a.c.K / want < 1 ? 1 : a.out_pages * (long long)a.c.K / want > a.c.K ? a.c.K : a.out_pages * (long long)a.c.K / want);
+    const dim3 grid(a.out_pages, (a.c.K + heads - 1) / heads);
+    const bool whole = a.wide && a.D == a.c.hs;
+    if (whole && a.D == 64) xr_launch((k_kv4_read<T, 3>), grid, dim3(256), 0, stream, a);
+    else if (whole && a.D == 128) xr_launch((k_kv4_read<T, 4>), grid, dim3(256), 0, stream, a);
+    else if (whole) xr_launch((k_kv4_read<T, 5>), grid, dim3(256), 0, stream, a);
+    else xr_launch((k_kv4_read<T, 0>), grid, dim3(256), 0, stream, a);
 }
 
 XR_EXPORT int xr_kv4_read(const void* cache, long long n_pages, int layers, int layer, int K, int block, int page_size, const int* block_tables,
@@ -213,8 +281,8 @@ XR_EXPORT int xr_kv4_read(const void* cache, long long n_pages, int layers, int 
         return XR_ERR_ARG;
     Kv4ReadArgs a{kv4_cache(cache, n_pages, layers, layer, K, page_size, D), first, end, block_tables, out, tables, n_seg, max_pages, D, keep, out_pages, 0};
     a.wide = D % 8 == 0 && !((uintptr_t)out & 15);
-    if (dtype == XR_F32) xr_launch((k_kv4_read<float>), dim3(out_pages, K), dim3(256), 0, stream, a);
-    else if (dtype == XR_BF16) xr_launch((k_kv4_read<__nv_bfloat16>), dim3(out_pages, K), dim3(256), 0, stream, a);
+    if (dtype == XR_F32) kv4_launch_read<float>(a, stream);
+    else if (dtype == XR_BF16) kv4_launch_read<__nv_bfloat16>(a, stream);
     else return XR_ERR_ARG;
     return xr_launch_status();
 }

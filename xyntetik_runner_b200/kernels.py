@@ -8,8 +8,10 @@ the first call raises.
 from __future__ import annotations
 
 import ctypes
+from array import array
 from typing import Optional
 
+import numpy as np
 import torch
 
 from .csrc import build as _build
@@ -55,7 +57,23 @@ class _Calls:
 class _CtypesCalls:
     def __init__(self, L: ctypes.CDLL):
         for name, letters in SIGNATURES.items():
-            setattr(self, name, self._setting(getattr(L, name), letters.index("o")) if "o" in letters else getattr(L, name))
+            fn = getattr(L, name)
+            if "b" in letters:
+                fn = self._reading(fn, [i for i, c in enumerate(letters) if c == "b"])
+            setattr(self, name, self._setting(fn, letters.index("o")) if "o" in letters else fn)
+
+    @staticmethod
+    def _reading(fn, at):
+        def call(*args):
+            args, kept = list(args), []
+            for i in at:
+                view = memoryview(args[i])
+                if not view.c_contiguous:
+                    raise BufferError("ndarray is not C-contiguous")
+                kept.append(np.asarray(view))
+                args[i] = kept[-1].ctypes.data
+            return fn(*args)
+        return call
 
     @staticmethod
     def _setting(fn, at: int):
@@ -74,7 +92,7 @@ def library_file() -> str:
 
 
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float, "u": ctypes.c_uint, "U": ctypes.c_ulonglong,
-           "o": ctypes.POINTER(ctypes.c_int)}
+           "o": ctypes.POINTER(ctypes.c_int), "b": ctypes.c_void_p}
 
 
 def _declare(L: ctypes.CDLL) -> None:
@@ -478,8 +496,7 @@ def tc_check_status(device: torch.device) -> None:
         if code != 0:
             ws.status.zero_()
             ws.flags.zero_()                  # a launch that gave up may have left some raised
-            what = {1: "a tcgen05 product", 2: "the bulk-copy decode attention", 3: "the tcgen05 attention", 4: "the tcgen05 attention (shared memory not 1 KB aligned)",
-                    5: "the attention over a cache in four bits"}.get(code, "a kernel")
+            what = {1: "a tcgen05 product", 2: "the bulk-copy decode attention", 3: "the tcgen05 attention", 4: "the tcgen05 attention (shared memory not 1 KB aligned)"}.get(code, "a kernel")
             raise KernelError(f"{what} gave up waiting on a barrier; its output is not valid")
 
 
@@ -764,32 +781,46 @@ def kv4_cache(pages: int, layers: int, kv_heads: int, head_dim: int, page_size: 
     return torch.zeros((pages, layers, kv_heads, kv4_block_bytes(head_dim, page_size)), dtype=torch.uint8, device=device)
 
 
+_I32, _U8 = torch.int32, torch.uint8
+
+
+def _here() -> int:
+    return _raw_device() if _raw_device is not None else torch.cuda.current_device()
+
+
 def _on_current(*ts) -> None:
-    if any(t is not None and not t.is_cuda for t in ts):
-        raise KernelError("kernel arguments must lie on the current CUDA device")
-    here = _raw_device() if _raw_device is not None else torch.cuda.current_device()
-    if any(t is not None and t.device.index != here for t in ts):
-        raise KernelError("kernel arguments must lie on the current CUDA device")
+    """All tensors lie on the current device: a launch goes to its stream."""
+    here = None
+    for t in ts:
+        if t is None:
+            continue
+        at = t.get_device()
+        if at != here:
+            if at < 0 or here is not None or at != _here():
+                raise KernelError("kernel arguments must lie on the current CUDA device")
+            here = at
 
 
 def _kv4_args(cache: torch.Tensor, layer: int, page_size: int, head_dim: int):
     """The arguments by which a launcher knows a cache: address, pages, layers, layer, kv heads, block, tokens a page."""
-    if cache.dtype != torch.uint8 or cache.dim() != 4 or not cache.is_contiguous():
+    if cache.dtype is not _U8 or cache.ndim != 4 or not cache.is_contiguous():
         raise KernelError("a cache in four bits is a contiguous uint8 array [pages, layers, kv heads, block]")
-    if cache.shape[3] != kv4_block_bytes(head_dim, page_size) or not 0 <= layer < cache.shape[1]:
-        raise KernelError(f"this cache has blocks of {cache.shape[3]} bytes and {cache.shape[1]} layers: not one for heads of {head_dim} in pages of "
-                          f"{page_size}, layer {layer}")
-    return cache.data_ptr(), cache.shape[0], cache.shape[1], int(layer), cache.shape[2], cache.shape[3], int(page_size)
+    pages, layers, K, block = cache.shape
+    if block != kv4_block_bytes(head_dim, page_size) or not 0 <= layer < layers:
+        raise KernelError(f"this cache has blocks of {block} bytes and {layers} layers: not one for heads of {head_dim} in pages of {page_size}, "
+                          f"layer {layer}")
+    return cache.data_ptr(), pages, layers, layer, K, block, page_size
 
 
-def _ints(n: int, **ts) -> None:
-    for name, t in ts.items():
-        if t.dtype != torch.int32 or t.numel() < n or not t.is_contiguous():
-            raise KernelError(f"{name}: {n} int32 values, one after another, are wanted")
+def _ints(t: torch.Tensor, n: int, name: str) -> int:
+    """The address of `n` int32 values."""
+    if t.dtype is not _I32 or t.numel() < n or not t.is_contiguous():
+        raise KernelError(f"{name}: {n} int32 values, one after another, are wanted")
+    return t.data_ptr()
 
 
 def _tables(block_tables: torch.Tensor):
-    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or not block_tables.is_contiguous() or block_tables.numel() == 0:
+    if block_tables.dtype is not _I32 or block_tables.ndim != 2 or not block_tables.is_contiguous() or block_tables.numel() == 0:
         raise KernelError("block tables are int32 [requests, pages], one row after another")
     return block_tables.shape
 
@@ -800,22 +831,24 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, tok_seg
     cached) into the pages: row t is position positions[t] of the request of row tok_seg[t] of the block tables.  `cache`: ``kv4_cache`` for heads
     of max(D, Vd).  Tokens whose page is not held (an entry below zero or not of this cache, a position beyond the table) are not written; a
     position may be given once in a call."""
-    K = cache.shape[2] if cache.dim() == 4 else 0
-    n = k.shape[0] if k.dim() == 2 else -1
-    if K < 1 or k.dim() != 2 or v.dim() != 2 or v.shape[0] != n or k.shape[1] % K or v.shape[1] % K or not k.shape[1] or not v.shape[1]:
+    K = cache.shape[2] if cache.ndim == 4 else 0
+    (n, kd), (n_v, vd) = (k.shape, v.shape) if k.ndim == 2 and v.ndim == 2 else ((0, 0), (0, 0))
+    if K < 1 or n_v != n or kd < 1 or vd < 1 or kd % K or vd % K:
         raise KernelError("k and v are [tokens, kv heads * elements], with the cache's kv heads")
-    if k.dtype != v.dtype or k.stride(1) != 1 or v.stride(1) != 1:
+    (k_row, k_one), (v_row, v_one) = k.stride(), v.stride()
+    if k.dtype is not v.dtype or (k_one != 1 and kd > 1) or (v_one != 1 and vd > 1):
         raise KernelError("k and v have one type, and neighbouring elements lie side by side")
     n_seg, max_pages = _tables(block_tables)
-    _ints(n, positions=positions, tok_seg=tok_seg)
+    at_pos, at_seg = _ints(positions, n, "positions"), _ints(tok_seg, n, "tok_seg")
     _on_current(k, v, positions, tok_seg, block_tables, cache)
-    D, Vd = k.shape[1] // K, v.shape[1] // K
+    D, Vd = kd // K, vd // K
     args = _kv4_args(cache, layer, page_size, max(D, Vd))
     code = dtype_code(k.dtype)
     if n == 0:
         return
-    _check(_c.xr_kv4_store(k.data_ptr(), v.data_ptr(), code, max(k.stride(0), K * D), max(v.stride(0), K * Vd), positions.data_ptr(), tok_seg.data_ptr(),
-                           block_tables.data_ptr(), *args, n, D, Vd, n_seg, max_pages, _stream()), "kv4_store")
+    # (one row has no stride: torch may say anything)
+    _check(_c.xr_kv4_store(k.data_ptr(), v.data_ptr(), code, k_row if n > 1 else kd, v_row if n > 1 else vd, at_pos, at_seg, block_tables.data_ptr(), *args, n, D,
+                           Vd, n_seg, max_pages, _stream()), "kv4_store")
     _count()
 
 
@@ -826,21 +859,22 @@ def kv4_read(cache: torch.Tensor, layer: int, page_size: int, block_tables: torc
     each request's kept pages ahead of the others.  Rows of these pages that are not asked for, or whose page is not held, are zeros; pages of
     `out` behind the last are left as they were.  `tables` (int32, the block tables' shape): receives where a page lies in `out`; entries of
     pages that are not there are left."""
-    if out.dim() != 5 or out.shape[1] != 2 or out.shape[3] != page_size or not out.is_contiguous() or cache.dim() != 4 or out.shape[2] != cache.shape[2]:
+    pages, two, K, page, D = out.shape if out.ndim == 5 else (0, 0, 0, 0, 0)
+    if two != 2 or page != page_size or not out.is_contiguous() or cache.ndim != 4 or K != cache.shape[2]:
         raise KernelError("out is [pages, 2, kv heads, page_size, elements], one page after another")
     n_seg, max_pages = _tables(block_tables)
-    _ints(n_seg, first=first, end=end)
+    at_first, at_end = _ints(first, n_seg, "first"), _ints(end, n_seg, "end")
     if tables is not None and (tables.shape != block_tables.shape or tables.dtype != torch.int32 or not tables.is_contiguous()):
         raise KernelError("tables has the block tables' shape and type")
     if keep_first < 0:
         raise KernelError(f"keep_first {keep_first}")
     _on_current(cache, block_tables, first, end, out, tables)
-    args = _kv4_args(cache, layer, page_size, out.shape[4])
+    args = _kv4_args(cache, layer, page_size, D)
     code = dtype_code(out.dtype)
-    if out.shape[0] == 0:
+    if pages == 0:
         return
-    _check(_c.xr_kv4_read(*args, block_tables.data_ptr(), first.data_ptr(), end.data_ptr(), out.data_ptr(), code, _ptr(tables), n_seg, max_pages,
-                          out.shape[4], int(keep_first), out.shape[0], _stream()), "kv4_read")
+    _check(_c.xr_kv4_read(*args, block_tables.data_ptr(), at_first, at_end, out.data_ptr(), code, _ptr(tables), n_seg, max_pages, D, keep_first, pages,
+                          _stream()), "kv4_read")
     _count()
 
 
@@ -848,13 +882,22 @@ KV4_SHORT_ROWS = 64        # packed rows (tokens x query heads per kv head) up t
 _KV4_ALL_ROWS = 1 << 30
 
 
-def kv4_pages_read(seg_len, seg_pos0, page_size: int, window: int, keep_first: int) -> int:
-    """Pages that ``kv4_read`` writes for the rows that these portions (numpy, on the host) see."""
-    import numpy as np
-    pos, end = seg_pos0.astype(np.int64), seg_pos0.astype(np.int64) + seg_len
-    first = np.maximum(0, pos - window + 1) if window > 0 else np.zeros_like(pos)
-    kept = np.minimum(-(-keep_first // page_size), first // page_size) if window > 0 else 0
-    return int((kept + (end - 1) // page_size - first // page_size + 1)[seg_len > 0].sum())
+# what xr_kv4_plan says of a step's portions, in this order
+_PLAN = ("short", "long", "floats", "pages", "longest", "tiles_128", "tiles_64", "end")
+
+
+def kv4_plan(lengths: tuple, n: int, kv_heads: int, group: int, head_dim: int, page_size: int, code: int, window: int, keep_first: int, most_rows: int,
+             max_kv_len: int = 0):
+    """What the portions `lengths` = (tokens, first positions) ask for, on the host: how many are short (at most `most_rows` packed rows) and how many longer;
+    floats of scratch for the short ones; of the longer ones the pages that their rows are read back into, the tokens of the longest, their row
+    tiles of 128 and 64 rows, and the end of the furthest.  Raises where they do not fit `n` tokens."""
+    h_len, h_pos = lengths
+    if h_len.dtype.char != "i" or h_pos.dtype.char != "i" or h_len.ndim != 1 or h_len.shape != h_pos.shape:
+        raise KernelError("lengths: two int32 numpy arrays, one value a portion")
+    said = array("q", (0,) * len(_PLAN))
+    if _c.xr_kv4_plan(h_len, h_pos, h_len.size, n, kv_heads, group, head_dim, page_size, code, window, keep_first, most_rows, max_kv_len, said) != 0:
+        raise KernelError("lengths: portions that q does not hold, or positions below zero")
+    return said
 
 
 def attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, layer: int, page_size: int, seg_start: torch.Tensor, seg_len: torch.Tensor,
@@ -868,69 +911,61 @@ def attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, layer
     them) but the same seg_len.  Rows on a page that is not held count as zeros.  Options: see ``attention_simt``.
     Single tokens, short portions and whatever the prompt kernels do not take attend to the codes; portions of more than KV4_SHORT_ROWS packed rows read the
     rows they see back into `buf` (``buf(name, shape, dtype)`` gives scratch; None: allocated) and go through the prompt kernels."""
-    K = cache.shape[2] if cache.dim() == 4 else 0
+    K = cache.shape[2] if cache.ndim == 4 else 0
     if K < 1 or heads < 1 or heads % K:
         raise KernelError(f"{heads} query heads on {K} kv heads")
     n_seg, max_pages = _tables(block_tables)
-    _ints(n_seg, seg_start=seg_start, seg_len=seg_len, seg_pos0=seg_pos0)
-    n = out.shape[0]
-    if out.dim() != 2 or out.shape[1] != heads * head_dim or not out.is_contiguous() or q.dim() != 2 or q.shape[0] != n or q.shape[1] < heads * head_dim or \
-            q.stride(1) != 1 or q.dtype != out.dtype:
+    at_start, at_len, at_pos = _ints(seg_start, n_seg, "seg_start"), _ints(seg_len, n_seg, "seg_len"), _ints(seg_pos0, n_seg, "seg_pos0")
+    cols, dtype = heads * head_dim, q.dtype
+    (n, width), (n_out, out_cols) = (q.shape, out.shape) if q.ndim == 2 and out.ndim == 2 else ((0, 0), (1, 0))
+    q_row, q_one = q.stride() if q.ndim == 2 else (0, 0)
+    if n != n_out or out_cols != cols or width < cols or (q_one != 1 and cols > 1) or out.dtype is not dtype or not out.is_contiguous():
         raise KernelError("q and out are rows of the same tokens in one type, out [tokens, heads * elements]")
-    h_len, h_pos = lengths
-    if any(str(a.dtype) != "int32" or a.shape != (n_seg,) or not a.flags["C_CONTIGUOUS"] for a in (h_len, h_pos)):
-        raise KernelError("lengths: two int32 numpy arrays, one value a portion")
-    if int(h_len.sum()) > n or int(h_len.min()) < 0 or int(h_pos.min()) < 0:
-        raise KernelError("lengths: portions that q does not hold, or positions below zero")
+    if n < 2:
+        q_row = cols                       # (one row has no stride: torch may say anything)
     if window < 0 or keep_first < 0 or not scale > 0 or not softcap >= 0 or (bias is not None and softcap > 0):
         raise KernelError("window and keep_first are not negative, the scale is positive, a bias goes without a cap")
-    if sink is not None and (sink.dtype != torch.float32 or sink.numel() != heads or not sink.is_contiguous()):
+    if sink is not None and (sink.dtype is not torch.float32 or sink.numel() != heads or not sink.is_contiguous()):
         raise KernelError("sink: one float32 logit a query head")
-    _check_bias(bias, heads)
+    if bias is not None:
+        _check_bias(bias, heads)
     _on_current(q, out, cache, seg_start, seg_len, seg_pos0, block_tables, sink, bias)
     args = _kv4_args(cache, layer, page_size, head_dim)
-    code = dtype_code(q.dtype)
+    code = dtype_code(dtype)
     G = heads // K
-    rows = h_len.astype("int64") * G
-    if buf is None:
-        buf = lambda name, shape, dtype: torch.empty(shape, dtype=dtype, device=out.device)
-    q_stride = max(q.stride(0), heads * head_dim)
-    most = _KV4_ALL_ROWS
-    aligned = q.dtype == torch.bfloat16 and q_stride % 8 == 0 and q.data_ptr() % 16 == 0
-    tc = aligned and attention_tc_supported(q.dtype, heads, K, head_dim, page_size)
-    if aligned and (tc or (head_dim % 16 == 0 and head_dim <= 128 and out.data_ptr() % 16 == 0)):
-        most = KV4_SHORT_ROWS
-    longer = rows > most
-    if longer.any():
-        len_long = h_len * longer
-        pages = kv4_pages_read(len_long, h_pos, page_size, window, keep_first)
-        ints = buf("kv4_portions", (3 * n_seg + block_tables.numel(),), torch.int32)
-        first, end, long_len, tables = ints[:n_seg], ints[n_seg:2 * n_seg], ints[2 * n_seg:3 * n_seg], ints[3 * n_seg:].view(n_seg, max_pages)
-        values = buf("kv4_values", (pages, 2, K, page_size, head_dim), torch.bfloat16)
-        _check(_c.xr_kv4_long(seg_len.data_ptr(), seg_pos0.data_ptr(), first.data_ptr(), end.data_ptr(), long_len.data_ptr(), tables.data_ptr(), n_seg,
-                              max_pages, G, int(window), most, _stream()), "attention_kv4")
-        _check(_c.xr_kv4_read(*args, block_tables.data_ptr(), first.data_ptr(), end.data_ptr(), values.data_ptr(), BF16, tables.data_ptr(), n_seg,
-                              max_pages, head_dim, int(keep_first), pages, _stream()), "attention_kv4")
+    if lengths[0].size != n_seg:
+        raise KernelError("lengths: two int32 numpy arrays, one value a portion")
+    # portions that the prompt kernels take: bfloat16 on 16-byte borders, head sizes that one of them has
+    aligned = code == BF16 and q_row % 8 == 0 and q.data_ptr() % 16 == 0 and head_dim % 16 == 0 and head_dim <= 128 and out.data_ptr() % 16 == 0
+    most = KV4_SHORT_ROWS if aligned else _KV4_ALL_ROWS
+    short, long, floats, pages, longest, tiles_128, tiles_64, end = kv4_plan(lengths, n, K, G, head_dim, page_size, code, window, keep_first, most, max_kv_len)
+    if long:
+        def scratch(name, shape, dt):
+            return torch.empty(shape, dtype=dt, device=out.device) if buf is None else buf(name, shape, dt)
+        ints = scratch("kv4_portions", (3 * n_seg + n_seg * max_pages,), _I32)
+        first, last, long_len, tables = ints[:n_seg], ints[n_seg:2 * n_seg], ints[2 * n_seg:3 * n_seg], ints[3 * n_seg:].view(n_seg, max_pages)
+        values = scratch("kv4_values", (pages, 2, K, page_size, head_dim), torch.bfloat16)
+        _check(_c.xr_kv4_long(at_len, at_pos, first.data_ptr(), last.data_ptr(), long_len.data_ptr(), tables.data_ptr(), n_seg, max_pages, G, window, most,
+                              _stream()), "attention_kv4")
+        _check(_c.xr_kv4_read(*args, block_tables.data_ptr(), first.data_ptr(), last.data_ptr(), values.data_ptr(), BF16, tables.data_ptr(), n_seg, max_pages,
+                              head_dim, keep_first, pages, _stream()), "attention_kv4")
         _count(2)
         half = K * page_size * head_dim
-        longest = int(len_long.max())
-        if tc:
+        if attention_tc_supported(dtype, heads, K, head_dim, page_size):
             attention_tc(q, out, seg_start, long_len, seg_pos0, tables, (values.data_ptr(), pages, 1, 0), heads, K, head_dim, max_pages, page_size, window,
-                         scale, n_seg, longest, row_tiles=long_row_tiles(len_long, G, 128), sink=sink, softcap=softcap, keep_first=keep_first, bias=bias)
+                         scale, n_seg, longest, row_tiles=tiles_128, sink=sink, softcap=softcap, keep_first=keep_first, bias=bias)
         else:
-            attention_mma(q, q_stride, out, values.data_ptr(), seg_start, long_len, seg_pos0, tables, None, None, 2 * half, half, heads, K, head_dim,
-                          max_pages, page_size, window, scale, n_seg, longest, int((h_pos + len_long).max()), 0, False, True,
-                          row_tiles=long_row_tiles(len_long, G, 64), sink=sink, softcap=softcap, keep_first=keep_first, bias=bias)
-    if not longer.all():
-        floats = int(_c.xr_kv4_attention_floats(h_len.ctypes.data, h_pos.ctypes.data, n_seg, K, G, head_dim, code, int(window), int(keep_first), most,
-                                                int(max_kv_len)))
-        scratch = buf("kv4_spans", (floats,), torch.float32) if floats else None
-        _check(_c.xr_kv4_attention(q.data_ptr(), out.data_ptr(), code, *args, seg_start.data_ptr(), seg_len.data_ptr(), seg_pos0.data_ptr(),
-                                   block_tables.data_ptr(), h_len.ctypes.data, h_pos.ctypes.data, _ptr(scratch), floats, workspace(out.device).status_ptr,
-                                   q_stride, n_seg, heads, head_dim, max_pages, int(window), float(scale), _ptr(sink), float(softcap), int(keep_first),
-                                   _ptr(bias), _bias_len(bias), most, int(max_kv_len), _stream()), "attention_kv4")
+            attention_mma(q, q_row, out, values.data_ptr(), seg_start, long_len, seg_pos0, tables, None, None, 2 * half, half, heads, K, head_dim, max_pages,
+                          page_size, window, scale, n_seg, longest, end, 0, False, True, row_tiles=tiles_64, sink=sink, softcap=softcap,
+                          keep_first=keep_first, bias=bias)
+    if short:
+        spans = None
+        if floats:
+            spans = torch.empty(floats, dtype=torch.float32, device=out.device) if buf is None else buf("kv4_spans", (floats,), torch.float32)
+        _check(_c.xr_kv4_attention(q.data_ptr(), out.data_ptr(), code, *args, at_start, at_len, at_pos, block_tables.data_ptr(), lengths[0], lengths[1],
+                                   _ptr(spans), floats, q_row, n_seg, heads, head_dim, max_pages, window, scale, _ptr(sink),
+                                   softcap, keep_first, _ptr(bias), _bias_len(bias), most, max_kv_len, _stream()), "attention_kv4")
         _count(2 if floats else 1)
-
 
 FLAT_TILE = 128       # the flat array's first key of a portion is a multiple of this
 
