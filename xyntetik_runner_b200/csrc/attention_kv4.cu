@@ -32,6 +32,7 @@
 #define A4_THREADS (32 * A4_WARPS)
 #define A4_LOG2E 1.4426950408889634f
 #define A4_SLACK 8.0f
+#define A4_CLUSTER 8                  // most spans that a cluster combines (the portable cluster size)
 
 struct A4Args {
     const void* q; void* out;
@@ -45,6 +46,7 @@ struct A4Args {
     const float* sink;
     XrBias bias;
     int wide, wide_out;               // 16-byte loads of q; four neighbouring outputs at once
+    int clustered;                    // a request's spans are the blocks of a cluster, which combines them
     int tile_shift;                   // pages of 2^tile_shift whole tiles (-1: pages of other sizes)
 };
 
@@ -76,6 +78,26 @@ __device__ __forceinline__ uint32_t a4_smem(const void* p) { return (uint32_t)__
 // 16 bytes from global to shared memory without a register between; `bytes` 0: zeros instead.
 __device__ __forceinline__ void a4_copy(uint32_t dst, const void* src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// Shared memory of another block of the cluster, and the cluster's barrier.
+__device__ __forceinline__ uint32_t a4_of_rank(const void* mine, uint32_t rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(a4_smem(mine)), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ float4 a4_far4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 a4_far2(uint32_t at) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void a4_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void a4_mma(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -200,7 +222,10 @@ k_kv4_attention(A4Args a) {
     const int first_pos = pos0 + row0 / a.G, last_pos = pos0 + (row0 + rows - 1) / a.G;
     const A4Walk walk = a4_walk(first_pos, last_pos, a.window, a.keep, TK);
     const int n_spans = a4_spans(a, walk);
-    if (span >= n_spans) return;
+    if (span >= n_spans) {
+        if (a.clustered) { a4_cluster_sync(); a4_cluster_sync(); }       // (nothing to do, but the cluster's barriers count every block)
+        return;
+    }
     const int i_begin = span * a.span_tiles, i_end = span == n_spans - 1 ? walk.n : i_begin + a.span_tiles;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int* bt = a.block_tables + (size_t)seg * a.max_pages;
@@ -686,10 +711,45 @@ k_kv4_attention(A4Args a) {
             sum += ml_s[(w * RB + r) * 2 + 1] * k;
         }
         if (n_spans == 1) a4_out<F32>(a, tok0, kvh, row0 + r, d, v, at, sum);
-        else {
+        else if (a.clustered) {
+            // the block's own sums, where its first warp's were (this thread alone reads them), and behind all others (maximum, sum)
+            *reinterpret_cast<float4*>(acc_s + r * HS + d) = v;
+            if (d == 0) *reinterpret_cast<float2*>(ml_s + (A4_WARPS * RB + r) * 2) = make_float2(mm, sum);
+        } else {
             *reinterpret_cast<float4*>(a.part_acc + (item * RB + r) * HS + d) = v;
             if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (item * RB + r) * 2) = make_float2(mm, sum);
         }
+    }
+    if (a.clustered) {
+        // Every block of the cluster finishes a share of the rows' quadruples out of all blocks' shared memory, in ascending order of spans.
+        a4_cluster_sync();
+        if (n_spans > 1)
+            for (int q = span + threadIdx.x * n_spans; q < rows * (HS / 4); q += A4_THREADS * n_spans) {
+                const int r = q / (HS / 4), d = (q % (HS / 4)) * 4;
+                float2 ml[A4_CLUSTER];
+                float4 acc[A4_CLUSTER];
+#pragma unroll
+                for (int s = 0; s < A4_CLUSTER; s++) {
+                    const uint32_t rank = min(s, n_spans - 1);       // (clamped: no load is conditional)
+                    ml[s] = a4_far2(a4_of_rank(ml_s + (A4_WARPS * RB + r) * 2, rank));
+                    acc[s] = a4_far4(a4_of_rank(acc_s + r * HS + d, rank));
+                }
+                float mm = -INFINITY;
+#pragma unroll
+                for (int s = 0; s < A4_CLUSTER; s++) mm = fmaxf(mm, ml[s].x);
+                const float at = mm == -INFINITY ? 0.f : mm;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                float sum = 0.f;
+#pragma unroll
+                for (int s = 0; s < A4_CLUSTER; s++) {
+                    if (s >= n_spans) break;
+                    const float k = a4_exp2(ml[s].x - at);
+                    v.x += acc[s].x * k; v.y += acc[s].y * k; v.z += acc[s].z * k; v.w += acc[s].w * k;
+                    sum += ml[s].y * k;
+                }
+                a4_out<F32>(a, tok0, kvh, row0 + r, d, v, at, sum);
+            }
+        a4_cluster_sync();                                           // (nobody leaves while another reads its memory)
     }
 }
 
@@ -700,6 +760,7 @@ k_kv4_attention(A4Args a) {
 #define A4_MERGE_THREADS 512
 #define A4_MAX_SPLITS 256
 #define A4_START 1.5
+#define A4_MEET 0.5
 #define A4_MERGE 1.3
 template <int NG, int RB, bool F32>
 __global__ void __launch_bounds__(A4_MERGE_THREADS)
@@ -770,7 +831,7 @@ static int a4_tile(int hs) { return hs <= 128 ? 64 : 32; }
 
 // How a step is cut: row blocks of the longest portion that is taken (at most `most_rows` packed rows), tiles a span, spans of the longest
 // request.  len, pos0: the portions on the HOST; max_kv: the longest key range to be prepared for (0: what the portions say).
-struct A4Plan { int row_blocks, wide, span_tiles, splits; };
+struct A4Plan { int row_blocks, wide, span_tiles, splits, clustered; };
 static A4Plan a4_plan(const int* len, const int* pos0, int n_seg, int K, int G, int hs, int f32, int window, int keep, int most_rows, int max_kv) {
     const int tile = a4_tile(hs);
     long long rows = 0;
@@ -778,63 +839,83 @@ static A4Plan a4_plan(const int* len, const int* pos0, int n_seg, int K, int G, 
         const long long r = (long long)len[s] * G;
         if (r <= most_rows && r > rows) rows = r;
     }
-    A4Plan p{0, rows > 8, 1, 1};
+    A4Plan p{0, rows > 8, A4_WARPS, 1, 0};
     if (rows < 1) return p;
     const int rb = a4_rows(f32, p.wide);
     p.row_blocks = (int)((rows + rb - 1) / rb);
-    long long longest = 1, lone = 0;
     const long long resident = a4_resident(hs, f32, p.wide);
-    // (tiles of a portion's last row block, whose window is the furthest)
-    auto tiles_of = [&](int s) {
-        const long long end = (long long)pos0[s] + len[s], lo = window > 0 && end - len[s] - window + 1 > 0 ? end - len[s] - window + 1 : 0;
-        return (end - 1) / tile - lo / tile + 1 + xr_kept_tiles(keep, (int)lo, tile);
+    auto tiles_of = [&](int s) {                                     // (of the last row block, whose window is the furthest)
+        const int end = pos0[s] + len[s], lo = window > 0 ? (end - len[s] - window + 1 > 0 ? end - len[s] - window + 1 : 0) : 0;
+        return (end - 1) / tile - lo / tile + 1 + xr_kept_tiles(keep, lo, tile);
     };
     auto taken = [&](int s) { return len[s] >= 1 && (long long)len[s] * G <= most_rows; };
+    int longest = 1;
+    for (int s = 0; s < n_seg; s++)
+        if (taken(s)) { const int t = tiles_of(s); longest = t > longest ? t : longest; }
+    // blocks by the tiles that they would have whole, in at most 32 classes (each taken for its upper end)
+    constexpr int CLASSES = 32;
+    long long of[CLASSES] = {};
+    double tiles = 0.0;
     for (int s = 0; s < n_seg; s++)
         if (taken(s)) {
-            const long long t = tiles_of(s);
-            longest = t > longest ? t : longest;
-            lone += K * (((long long)len[s] * G + rb - 1) / rb);
+            const int t = tiles_of(s);
+            const long long blocks = K * (((long long)len[s] * G + rb - 1) / rb);
+            of[((long long)t * CLASSES - 1) / longest] += blocks;
+            tiles += (double)blocks * t;
         }
-    if (max_kv > 0) {
-        const long long range = window > 0 && window + 16 < max_kv ? window + 16 : max_kv;
-        const long long t = (range + tile - 1) / tile + 1 + (window > 0 ? (keep + tile - 1) / tile : 0);
-        longest = t > longest ? t : longest;
-    }
     // Tiles a warp of a span takes: the number whose last block is done first, in the time of a tile (a warp's, all others at work).  Up to `resident` blocks
     // run at once; blocks of one length go in rounds, blocks of many lengths as slots fall free, half a block of which is idle at the end.  A block
-    // costs A4_START beside its tiles (its first tiles are on their way), combining spans A4_MERGE.
-    const long long most = (longest + A4_WARPS - 1) / A4_WARPS, least = (longest + A4_MAX_SPLITS * A4_WARPS - 1) / (A4_MAX_SPLITS * A4_WARPS);
-    long long best = most;
+    // costs A4_START beside its tiles (its first tiles are on their way), combining spans A4_MEET inside a cluster and A4_MERGE in a kernel of its own.
+    const int most = (longest + A4_WARPS - 1) / A4_WARPS, least = (longest + A4_MAX_SPLITS * A4_WARPS - 1) / (A4_MAX_SPLITS * A4_WARPS);
+    int best = most;
     double best_cost = -1.0;
-    for (long long n = most; n >= least && n >= 1; n = n > 48 ? n - n / 24 : n - 1) {
+    for (int n = most; n >= least && n >= 1; n = n > 48 ? n - n / 24 : n - 1) {
+        const int span = n * A4_WARPS;
         long long blocks = 0;
-        double tiles = 0.0;
-        for (int s = 0; s < n_seg; s++)
-            if (taken(s)) {
-                const long long of = K * (((long long)len[s] * G + rb - 1) / rb), t = tiles_of(s);
-                blocks += of * ((t + n * A4_WARPS - 1) / (n * A4_WARPS));
-                tiles += (double)of * t;
-            }
+        for (int c = 0; c < CLASSES; c++)
+            if (of[c]) blocks += of[c] * (((long long)(c + 1) * longest / CLASSES + span - 1) / span);
+        const int splits = (longest + span - 1) / span;
         const double work = tiles / A4_WARPS + A4_START * blocks;
-        const bool alike = tiles > 0.85 * (double)blocks * n * A4_WARPS;
+        const bool alike = tiles > 0.85 * (double)blocks * span;
         double cost = blocks <= resident ? n + A4_START : alike ? (double)((blocks + resident - 1) / resident) * (n + A4_START) : work / resident + 0.5 * (n + A4_START);
-        if (n < most) cost += A4_MERGE;
-        if (best_cost < 0.0 || cost < best_cost) { best_cost = cost; best = n; }
+        const bool meet = splits <= A4_CLUSTER && blocks + 8LL * (splits - 1) <= resident;
+        if (splits > 1) cost += meet ? A4_MEET : A4_MERGE;
+        if (best_cost < 0.0 || cost < best_cost) { best_cost = cost; best = n; p.clustered = splits > 1 && meet; }
         if (work / resident > 1.5 * best_cost) break;
     }
-    p.span_tiles = (int)(best * A4_WARPS);
-    p.splits = (int)((longest + p.span_tiles - 1) / p.span_tiles);
+    p.span_tiles = best * A4_WARPS;
+    if (max_kv > 0) {
+        // (a captured launch may meet requests up to this length; beyond the grid's spans the last one takes the rest)
+        const long long range = window > 0 && window + 16 < max_kv ? window + 16 : max_kv;
+        const long long t = (range + tile - 1) / tile + 1 + (window > 0 ? (keep + tile - 1) / tile : 0);
+        const long long more = best * (long long)A4_WARPS * (p.clustered ? A4_CLUSTER : A4_MAX_SPLITS);
+        longest = (int)(t > longest ? (t < more ? t : (more > longest ? more : longest)) : longest);
+    }
+    p.splits = (longest + p.span_tiles - 1) / p.span_tiles;
     return p;
 }
 
 template <int NG, int NT, bool F32, bool EXTRA>
 static int a4_launch(const A4Args& a, int n_seg, cudaStream_t stream) {
     using S = A4Shape<NG, NT, F32, EXTRA>;
-    static_assert(A4_WARPS * S::RB * (S::HS + 2) * 4 <= A4_WARPS * S::STAGES * S::STAGE, "the warps' sums lie in the ring");
+    static_assert((A4_WARPS * S::RB * (S::HS + 2) + 2 * S::RB) * 4 <= A4_WARPS * S::STAGES * S::STAGE, "the warps' sums lie in the ring");
     static bool ready[XR_DEVICES];
     if (!xr_once_per_device(ready, [] { return xr_allow_smem(k_kv4_attention<NG, NT, F32, EXTRA>, S::SMEM); })) return XR_ERR_LAUNCH;
-    xr_launch((k_kv4_attention<NG, NT, F32, EXTRA>), dim3(a.splits, a.c.K * a.row_blocks, n_seg), dim3(A4_THREADS), S::SMEM, stream, a);
+    const dim3 grid(a.splits, a.c.K * a.row_blocks, n_seg);
+    if (a.clustered) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = grid; cfg.blockDim = dim3(A4_THREADS); cfg.dynamicSmemBytes = S::SMEM; cfg.stream = stream;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = a.splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = xr_pdl_enabled() ? 2 : 1;
+        cudaLaunchKernelEx(&cfg, k_kv4_attention<NG, NT, F32, EXTRA>, a);
+        return xr_launch_status();
+    }
+    xr_launch((k_kv4_attention<NG, NT, F32, EXTRA>), grid, dim3(A4_THREADS), S::SMEM, stream, a);
     if (xr_launch_status() != XR_OK) return XR_ERR_LAUNCH;
     if (a.splits > 1) xr_launch((k_kv4_merge<NG, S::RB, F32>), dim3(a.c.K * a.row_blocks, n_seg), dim3(A4_MERGE_THREADS), 0, stream, a);
     return xr_launch_status();
@@ -850,12 +931,13 @@ static int a4_launch(const A4Args& a, int n_seg, int f32, int wide, cudaStream_t
 
 // What a step's portions ask for, from their lengths and first positions on the HOST: said[0] portions of 1 to `most_rows` packed rows, [1] longer ones,
 // [2] float32 values of scratch that xr_kv4_attention needs for the short ones; of the longer ones [3] the pages that xr_kv4_read writes for
-// them, [4] the most tokens, [5], [6] the row tiles of 128 and 64 packed rows, [7] the furthest end.  n: tokens of the step.
+// them, [4] the most tokens, [5], [6] the row tiles of 128 and 64 packed rows, [7] the furthest end; [8] .. [12] how the short ones are cut, as
+// xr_kv4_attention takes it.  n: tokens of the step.
 XR_EXPORT int xr_kv4_plan(const int* len, const int* pos0, int n_seg, int n, int K, int G, int D, int page_size, int dtype, int window, int keep_first,
                           int most_rows, int max_kv, long long* said) {
     if (n_seg < 1 || n < 0 || K < 1 || G < 1 || D < 1 || D > 256 || page_size < 1 || window < 0 || keep_first < 0 || most_rows < 0) return XR_ERR_ARG;
     long long tokens = 0;
-    for (int i = 0; i < 8; i++) said[i] = 0;
+    for (int i = 0; i < 13; i++) said[i] = 0;
     for (int s = 0; s < n_seg; s++) {
         const long long l = len[s], p = pos0[s], rows = l * G;
         if (l < 0 || p < 0) return XR_ERR_ARG;
@@ -875,37 +957,37 @@ XR_EXPORT int xr_kv4_plan(const int* len, const int* pos0, int n_seg, int n, int
     if (said[0] > 0) {
         const int hs = kv4_held(D), f32 = dtype == XR_F32;
         const A4Plan p = a4_plan(len, pos0, n_seg, K, G, hs, f32, window, window > 0 ? keep_first : 0, most_rows, max_kv);
-        if (p.splits > 1) said[2] = (long long)n_seg * K * p.row_blocks * p.splits * a4_rows(f32, p.wide) * (hs + 2);
+        said[8] = p.row_blocks; said[9] = p.wide; said[10] = p.span_tiles; said[11] = p.splits; said[12] = p.clustered;
+        if (p.splits > 1 && !p.clustered) said[2] = (long long)n_seg * K * p.row_blocks * p.splits * a4_rows(f32, p.wide) * (hs + 2);
     }
     return XR_OK;
 }
 
 // q: token t, head h at q + t * q_stride + h * D; out [n][H * D], both of `dtype`.  Portions of at most `most_rows` packed rows (tokens x heads per
-// kv head) are computed, longer ones passed over.  len, pos0: the same lengths and first positions as seg_len and seg_pos0, on the host (they
-// size the grid; what is computed goes by the device's).
+// kv head) are computed, longer ones passed over.  row_blocks, wide, span_tiles, splits, clustered: xr_kv4_plan's answer for the portions' lengths on the
+// host (they cut the work; what is computed goes by seg_len and seg_pos0 on the device, of at most row_blocks row blocks).
 XR_EXPORT int xr_kv4_attention(const void* q, void* out, int dtype, const void* cache, long long n_pages, int layers, int layer, int K, int block, int page_size,
-                               const int* seg_start, const int* seg_len, const int* seg_pos0, const int* block_tables, const int* len, const int* pos0,
-                               float* scratch, long long floats, long long q_stride, int n_seg, int H, int D, int max_pages, int window,
-                               float scale, const float* sink, float softcap, int keep_first, const float* bias, int bias_len, int most_rows, int max_kv,
-                               cudaStream_t stream) {
-    if (n_seg < 1 || n_seg > 65535 || H < 1 || H % K != 0 || max_pages < 1 || window < 0 || keep_first < 0 || !(scale > 0.f) || !(softcap >= 0.f) ||
-        (bias != nullptr && (bias_len < 1 || softcap > 0.f)) || most_rows < 1 || max_kv < 0 || q_stride < (long long)H * D ||
-        (dtype != XR_F32 && dtype != XR_BF16) || !kv4_cache_ok(cache, n_pages, layers, layer, K, block, page_size, D) ||
-        (long long)max_pages * page_size > 0x7fffffffLL - 64)
+                               const int* seg_start, const int* seg_len, const int* seg_pos0, const int* block_tables, float* scratch, long long floats,
+                               long long q_stride, int n_seg, int H, int D, int max_pages, int window, float scale, const float* sink, float softcap,
+                               int keep_first, const float* bias, int bias_len, int most_rows, int row_blocks, int wide, int span_tiles, int splits,
+                               int clustered, cudaStream_t stream) {
+    if (n_seg < 1 || n_seg > 65535 || H < 1 || K < 1 || H % K != 0 || max_pages < 1 || window < 0 || keep_first < 0 || !(scale > 0.f) || !(softcap >= 0.f) ||
+        (bias != nullptr && (bias_len < 1 || softcap > 0.f)) || most_rows < 1 || q_stride < (long long)H * D || (dtype != XR_F32 && dtype != XR_BF16) ||
+        !kv4_cache_ok(cache, n_pages, layers, layer, K, block, page_size, D) || (long long)max_pages * page_size > 0x7fffffffLL - 64 || row_blocks < 1 ||
+        span_tiles < 1 || splits < 1 || splits > A4_MAX_SPLITS || (clustered && splits > A4_CLUSTER) || (long long)K * row_blocks > 65535)
         return XR_ERR_ARG;
     const int G = H / K, f32 = dtype == XR_F32, hs = kv4_held(D), keep = window > 0 ? keep_first : 0;
-    const A4Plan p = a4_plan(len, pos0, n_seg, K, G, hs, f32, window, keep, most_rows, max_kv);
-    if (p.row_blocks < 1) return XR_OK;
-    if ((long long)K * p.row_blocks > 65535) return XR_ERR_ARG;
-    const long long items = (long long)n_seg * K * p.row_blocks * p.splits, rb = a4_rows(f32, p.wide);
-    if (p.splits > 1 && (scratch == nullptr || ((uintptr_t)scratch & 15) || floats < items * rb * (hs + 2))) return XR_ERR_ARG;
+    const bool spans = splits > 1 && !clustered;
+    const long long items = spans ? (long long)n_seg * K * row_blocks * splits : 0, rb = a4_rows(f32, wide);
+    if (spans && (scratch == nullptr || ((uintptr_t)scratch & 15) || floats < items * rb * (hs + 2))) return XR_ERR_ARG;
     A4Args a{q, out, kv4_cache(cache, n_pages, layers, layer, K, page_size, D), seg_start, seg_len, seg_pos0, block_tables, scratch,
-             scratch + items * rb * hs, q_stride, H, G, D, max_pages, window, keep, p.splits, p.span_tiles, p.row_blocks, most_rows,
-             scale, softcap, sink, {bias, bias_len}, 0, 0, -1};
-    a.wide = D % 8 == 0 && q_stride % 8 == 0 && !((uintptr_t)q & 15);
+             spans ? scratch + items * rb * hs : nullptr, q_stride, H, G, D, max_pages, window, keep, splits, span_tiles, row_blocks, most_rows,
+             scale, softcap, sink, {bias, bias_len}, 0, 0, clustered && splits > 1, -1};
+    const int lot = f32 ? 4 : 8;                                     // elements of 16 bytes
+    a.wide = D % 8 == 0 && q_stride % lot == 0 && !((uintptr_t)q & 15);
     a.wide_out = D % 4 == 0 && !((uintptr_t)out & 15);
     const int tile = a4_tile(hs);
     if (page_size % tile == 0 && ((page_size / tile) & (page_size / tile - 1)) == 0)
         for (a.tile_shift = 0; (tile << a.tile_shift) < page_size;) a.tile_shift++;
-    return hs == 64 ? a4_launch<2>(a, n_seg, f32, p.wide, stream) : hs == 128 ? a4_launch<4>(a, n_seg, f32, p.wide, stream) : a4_launch<8>(a, n_seg, f32, p.wide, stream);
+    return hs == 64 ? a4_launch<2>(a, n_seg, f32, wide, stream) : hs == 128 ? a4_launch<4>(a, n_seg, f32, wide, stream) : a4_launch<8>(a, n_seg, f32, wide, stream);
 }

@@ -57,7 +57,11 @@ template <> struct Kv4Row8<float> {
     float4 p, q;
     __device__ __forceinline__ void load(const float* src, int live, bool wide) {
         p = q = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (wide) { if (live > 0) { p = reinterpret_cast<const float4*>(src)[0]; q = reinterpret_cast<const float4*>(src)[1]; } return; }
+        if (wide) {                                        // (a head ends with a whole or half a word)
+            if (live > 0) p = reinterpret_cast<const float4*>(src)[0];
+            if (live > 4) q = reinterpret_cast<const float4*>(src)[1];
+            return;
+        }
         float x[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] = i < live ? src[i] : 0.f;
@@ -125,7 +129,8 @@ XR_EXPORT int xr_kv4_store(const void* k, const void* v, int dtype, long long k_
         return XR_ERR_ARG;
     Kv4StoreArgs a{k, v, k_stride, v_stride, positions, tok_seg, block_tables, kv4_cache(cache, n_pages, layers, layer, K, page_size, D > Vd ? D : Vd),
                    n, D, Vd, n_seg, max_pages, 0};
-    a.wide = !(((uintptr_t)k | (uintptr_t)v) & 15) && D % 8 == 0 && Vd % 8 == 0 && k_stride % 8 == 0 && v_stride % 8 == 0;
+    const int even = dtype == XR_F32 ? 4 : 8;              // elements of 16 bytes
+    a.wide = !(((uintptr_t)k | (uintptr_t)v) & 15) && D % even == 0 && Vd % even == 0 && k_stride % even == 0 && v_stride % even == 0;
     a.word_shift = a.c.hs == 64 ? 3 : a.c.hs == 128 ? 4 : 5;
     const dim3 grid(n, (unsigned)(((2LL * K << a.word_shift) + 255) / 256));
     if (dtype == XR_F32) xr_launch((k_kv4_store<float>), grid, dim3(256), 0, stream, a);
@@ -248,7 +253,7 @@ k_kv4_read(Kv4ReadArgs a) {
                     const int tok = i / used, w = i - tok * used;
                     uint32_t word = 0, s = 0;
                     if (tok < a1 && (tok >= a0 || tok < kept)) { word = __ldg(codes + tok * words + w); s = __ldg(scales + tok * (words >> 2) + (w >> 2)); }
-                    if (a.wide) { kv4_eight<T>(word, s, to + (size_t)tok * a.D + 8 * w); continue; }
+                    if (a.wide && 8 * w + 8 <= a.D) { kv4_eight<T>(word, s, to + (size_t)tok * a.D + 8 * w); continue; }
                     uint32_t v[4];
                     kv4_values(word, s, v);
 #pragma unroll
@@ -280,7 +285,7 @@ XR_EXPORT int xr_kv4_read(const void* cache, long long n_pages, int layers, int 
         (long long)max_pages * page_size > 0x7fffffffLL)
         return XR_ERR_ARG;
     Kv4ReadArgs a{kv4_cache(cache, n_pages, layers, layer, K, page_size, D), first, end, block_tables, out, tables, n_seg, max_pages, D, keep, out_pages, 0};
-    a.wide = D % 8 == 0 && !((uintptr_t)out & 15);
+    a.wide = D % (dtype == XR_F32 ? 4 : 8) == 0 && !((uintptr_t)out & 15);
     if (dtype == XR_F32) kv4_launch_read<float>(a, stream);
     else if (dtype == XR_BF16) kv4_launch_read<__nv_bfloat16>(a, stream);
     else return XR_ERR_ARG;

@@ -883,14 +883,14 @@ _KV4_ALL_ROWS = 1 << 30
 
 
 # what xr_kv4_plan says of a step's portions, in this order
-_PLAN = ("short", "long", "floats", "pages", "longest", "tiles_128", "tiles_64", "end")
+_PLAN = ("short", "long", "floats", "pages", "longest", "tiles_128", "tiles_64", "end", "row_blocks", "wide", "span_tiles", "splits", "clustered")
 
 
 def kv4_plan(lengths: tuple, n: int, kv_heads: int, group: int, head_dim: int, page_size: int, code: int, window: int, keep_first: int, most_rows: int,
              max_kv_len: int = 0):
     """What the portions `lengths` = (tokens, first positions) ask for, on the host: how many are short (at most `most_rows` packed rows) and how many longer;
     floats of scratch for the short ones; of the longer ones the pages that their rows are read back into, the tokens of the longest, their row
-    tiles of 128 and 64 rows, and the end of the furthest.  Raises where they do not fit `n` tokens."""
+    tiles of 128 and 64 rows, and the end of the furthest; then how the short ones are cut, as the launcher takes it.  Raises where they do not fit `n` tokens."""
     h_len, h_pos = lengths
     if h_len.dtype.char != "i" or h_pos.dtype.char != "i" or h_len.ndim != 1 or h_len.shape != h_pos.shape:
         raise KernelError("lengths: two int32 numpy arrays, one value a portion")
@@ -938,7 +938,7 @@ def attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, layer
     # portions that the prompt kernels take: bfloat16 on 16-byte borders, head sizes that one of them has
     aligned = code == BF16 and q_row % 8 == 0 and q.data_ptr() % 16 == 0 and head_dim % 16 == 0 and head_dim <= 128 and out.data_ptr() % 16 == 0
     most = KV4_SHORT_ROWS if aligned else _KV4_ALL_ROWS
-    short, long, floats, pages, longest, tiles_128, tiles_64, end = kv4_plan(lengths, n, K, G, head_dim, page_size, code, window, keep_first, most, max_kv_len)
+    short, long, floats, pages, longest, tiles_128, tiles_64, end, *cut = kv4_plan(lengths, n, K, G, head_dim, page_size, code, window, keep_first, most, max_kv_len)
     if long:
         def scratch(name, shape, dt):
             return torch.empty(shape, dtype=dt, device=out.device) if buf is None else buf(name, shape, dt)
@@ -962,9 +962,9 @@ def attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, layer
         spans = None
         if floats:
             spans = torch.empty(floats, dtype=torch.float32, device=out.device) if buf is None else buf("kv4_spans", (floats,), torch.float32)
-        _check(_c.xr_kv4_attention(q.data_ptr(), out.data_ptr(), code, *args, at_start, at_len, at_pos, block_tables.data_ptr(), lengths[0], lengths[1],
-                                   _ptr(spans), floats, q_row, n_seg, heads, head_dim, max_pages, window, scale, _ptr(sink),
-                                   softcap, keep_first, _ptr(bias), _bias_len(bias), most, max_kv_len, _stream()), "attention_kv4")
+        _check(_c.xr_kv4_attention(q.data_ptr(), out.data_ptr(), code, *args, at_start, at_len, at_pos, block_tables.data_ptr(), _ptr(spans),
+                                   floats, q_row, n_seg, heads, head_dim, max_pages, window, scale, _ptr(sink),
+                                   softcap, keep_first, _ptr(bias), _bias_len(bias), most, *cut, _stream()), "attention_kv4")
         _count(2 if floats else 1)
 
 FLAT_TILE = 128       # the flat array's first key of a portion is a multiple of this
