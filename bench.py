@@ -334,6 +334,7 @@ def main() -> int:
     ap.add_argument("--skip-kernels", action="store_true", help="leave the per-kernel table out of the line")
     ap.add_argument("--decode-only", action="store_true", help="time the decode step only (for profiling a small run)")
     ap.add_argument("--prefill-only", action="store_true", help="time the 2,048-token prefill only (for profiling a small run)")
+    ap.add_argument("--kv", choices=["same", "int4"], default="same", help="cached keys and values: as the activations, or four bits (named in config)")
     ap.add_argument("--no-graphs", action="store_true", help="launch every kernel of a decode step one by one")
     ap.add_argument("--shape", choices=sorted(SHAPES), default=None, help="layer sizes (default llama-3-8b)")
     ap.add_argument("--workload", choices=["decode", "mixed"], default="decode",
@@ -399,9 +400,13 @@ def main() -> int:
     t_load = time.perf_counter()
     eng = random_engine(cfg, seed, EngineParams(dtype="bfloat16", max_tokens=max_b * ctx_len, page_size=64, max_requests=max_b,
                                                 max_request_tokens=ctx_len, max_step_tokens=2048,
-                                                cuda_graphs=not args.no_graphs))
-    for kv in eng.kv:                      # keys and values of an imagined earlier context
-        kv.normal_(0.0, 1.0)
+                                                cuda_graphs=not args.no_graphs, kv=args.kv))
+    for kv, four_bits in zip(eng.kv, eng.four_bits):       # keys and values of an imagined earlier context
+        if four_bits:
+            kv.random_(0, 256)
+            kv.view(torch.bfloat16)[..., kv.shape[3] * 8 // 9 // 2:] = 0.25      # (the scales, behind eight ninths of a block)
+        else:
+            kv.normal_(0.0, 1.0)
     torch.cuda.synchronize()
     load_s = time.perf_counter() - t_load
     rng = np.random.RandomState(0)
@@ -543,7 +548,7 @@ def main() -> int:
         "vs_baseline": None, "dtype": "bf16", "data": f"synthetic (random weights seed {seed}, random token ids, random cached keys/values)",
         "config": {"model": shape + "-shape", "layers": cfg.num_hidden_layers, "layers_of_model": full_layers,
                    "hidden": d, "heads": H, "kv_heads": Kh, "head_dim": hd, "intermediate": F, "vocab": V,
-                   "global_batch": args.batch, "seq_len": ctx_len, "page_size": 64, "parallelism": "single-gpu",
+                   "global_batch": args.batch, "seq_len": ctx_len, "page_size": 64, **({"kv": args.kv} if args.kv != "same" else {}), "parallelism": "single-gpu",
                    "l2": "step inputs (weights) exceed L2", "peaks": pk["source"], "timing": f"median of {R} regions of {K} steps"},
         "e2e": {"value": e2e["tok_s"], "unit": "tok/s", "h2d_bytes_per_step": int(e2e["h2d"]), "d2h_bytes_per_step": 4 * args.batch,
                 "ms_per_step": e2e["ms"], "valid": e2e["valid"], "context_mid": e2e["context_mid"],

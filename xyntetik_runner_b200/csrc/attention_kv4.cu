@@ -46,6 +46,7 @@ struct A4Args {
     const float* sink;
     XrBias bias;
     int wide, wide_out;               // 16-byte loads of q; four neighbouring outputs at once
+    int early;                        // what earlier steps left, and the step's description, are at rest
     int clustered;                    // a request's spans are the blocks of a cluster, which combines them
     int tile_shift;                   // pages of 2^tile_shift whole tiles (-1: pages of other sizes)
 };
@@ -213,7 +214,8 @@ k_kv4_attention(A4Args a) {
     extern __shared__ __align__(128) uint8_t smem[];
     uint2* q_sm = (uint2*)(smem + A4_WARPS * STAGES * STAGE);                        // [P][NT][KS][32]
     const int seg = blockIdx.z, kvh = blockIdx.y % a.c.K, rb = blockIdx.y / a.c.K, span = blockIdx.x;
-    xr_pdl_wait();
+    // (a.early: portions, block tables and the rows of earlier steps are at rest, so that tiles of such rows set out before the kernel ahead is complete)
+    if (!a.early) xr_pdl_wait();
     const int L = a.seg_len[seg];
     const long long rows_all = (long long)L * a.G;
     if (L < 1 || rows_all > a.most_rows || (long long)rb * RB >= rows_all) return;
@@ -285,11 +287,15 @@ k_kv4_attention(A4Args a) {
 #pragma unroll
         for (int s = 0; s < STAGES; s++) first[s] = tiles_page(i_begin + warp + s * A4_WARPS);
         next_page = tiles_page(i_begin + warp + STAGES * A4_WARPS);
+        // (this step's own rows are stored by a kernel ahead; the span's last tile is the furthest)
+        const bool old_rows = ((long long)xr_walk_tile(i_end - 1, walk.kept, walk.t_lo) + 1) * TK <= pos0;
+        if (a.early && !old_rows) xr_pdl_wait();
 #pragma unroll
         for (int s = 0; s < STAGES; s++) {
             if (i_begin + warp + s * A4_WARPS < i_end) fetch(i_begin + warp + s * A4_WARPS, s, first[s]);
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
+        if (a.early && old_rows) xr_pdl_wait();
     }
 
     // q.  float32: thread (row g, t) holds the elements that its words of a key hold, 8 NG t ..; k-step 2 w + half: elements 8 w + 4 half ..  bfloat16: thread
@@ -965,12 +971,13 @@ XR_EXPORT int xr_kv4_plan(const int* len, const int* pos0, int n_seg, int n, int
 
 // q: token t, head h at q + t * q_stride + h * D; out [n][H * D], both of `dtype`.  Portions of at most `most_rows` packed rows (tokens x heads per
 // kv head) are computed, longer ones passed over.  row_blocks, wide, span_tiles, splits, clustered: xr_kv4_plan's answer for the portions' lengths on the
-// host (they cut the work; what is computed goes by seg_len and seg_pos0 on the device, of at most row_blocks row blocks).
+// host (they cut the work; what is computed goes by seg_len and seg_pos0 on the device, of at most row_blocks row blocks).  early: nothing that is still
+// running writes the portions, the block tables or rows before a portion's first.
 XR_EXPORT int xr_kv4_attention(const void* q, void* out, int dtype, const void* cache, long long n_pages, int layers, int layer, int K, int block, int page_size,
                                const int* seg_start, const int* seg_len, const int* seg_pos0, const int* block_tables, float* scratch, long long floats,
                                long long q_stride, int n_seg, int H, int D, int max_pages, int window, float scale, const float* sink, float softcap,
-                               int keep_first, const float* bias, int bias_len, int most_rows, int row_blocks, int wide, int span_tiles, int splits,
-                               int clustered, cudaStream_t stream) {
+                               int keep_first, const float* bias, int bias_len, int most_rows, int early, int row_blocks, int wide, int span_tiles,
+                               int splits, int clustered, cudaStream_t stream) {
     if (n_seg < 1 || n_seg > 65535 || H < 1 || K < 1 || H % K != 0 || max_pages < 1 || window < 0 || keep_first < 0 || !(scale > 0.f) || !(softcap >= 0.f) ||
         (bias != nullptr && (bias_len < 1 || softcap > 0.f)) || most_rows < 1 || q_stride < (long long)H * D || (dtype != XR_F32 && dtype != XR_BF16) ||
         !kv4_cache_ok(cache, n_pages, layers, layer, K, block, page_size, D) || (long long)max_pages * page_size > 0x7fffffffLL - 64 || row_blocks < 1 ||
@@ -982,7 +989,7 @@ XR_EXPORT int xr_kv4_attention(const void* q, void* out, int dtype, const void* 
     if (spans && (scratch == nullptr || ((uintptr_t)scratch & 15) || floats < items * rb * (hs + 2))) return XR_ERR_ARG;
     A4Args a{q, out, kv4_cache(cache, n_pages, layers, layer, K, page_size, D), seg_start, seg_len, seg_pos0, block_tables, scratch,
              spans ? scratch + items * rb * hs : nullptr, q_stride, H, G, D, max_pages, window, keep, splits, span_tiles, row_blocks, most_rows,
-             scale, softcap, sink, {bias, bias_len}, 0, 0, clustered && splits > 1, -1};
+             scale, softcap, sink, {bias, bias_len}, 0, 0, early, clustered && splits > 1, -1};
     const int lot = f32 ? 4 : 8;                                     // elements of 16 bytes
     a.wide = D % 8 == 0 && q_stride % lot == 0 && !((uintptr_t)q & 15);
     a.wide_out = D % 4 == 0 && !((uintptr_t)out & 15);

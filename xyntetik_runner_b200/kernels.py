@@ -903,14 +903,16 @@ def kv4_plan(lengths: tuple, n: int, kv_heads: int, group: int, head_dim: int, p
 def attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, layer: int, page_size: int, seg_start: torch.Tensor, seg_len: torch.Tensor,
                   seg_pos0: torch.Tensor, block_tables: torch.Tensor, heads: int, head_dim: int, scale: float, lengths: tuple, window: int = 0,
                   sink: Optional[torch.Tensor] = None, softcap: float = 0.0, keep_first: int = 0, bias: Optional[torch.Tensor] = None, max_kv_len: int = 0,
-                  buf=None) -> None:
+                  buf=None, early: bool = False) -> None:
     """Causal attention of every token of the step over its request's rows of a cache in four bits, its own row included.  q [n, >= heads *
     head_dim] (bfloat16 or float32, strided by rows), out [n, heads * head_dim]; portion s is the seg_len[s] rows from seg_start[s] on, at positions
     seg_pos0[s] .., over row s of the block tables.  `lengths` = (seg_len, seg_pos0) on the host (numpy int32): they size the launches; a call
     that is captured in a graph may be replayed with other positions (say in `max_kv_len` how long the requests may get, so that the cut suits
     them) but the same seg_len.  Rows on a page that is not held count as zeros.  Options: see ``attention_simt``.
     Single tokens, short portions and whatever the prompt kernels do not take attend to the codes; portions of more than KV4_SHORT_ROWS packed rows read the
-    rows they see back into `buf` (``buf(name, shape, dtype)`` gives scratch; None: allocated) and go through the prompt kernels."""
+    rows they see back into `buf` (``buf(name, shape, dtype)`` gives scratch; None: allocated) and go through the prompt kernels.  `early`: the caller says that
+    nothing still running writes the portions, the block tables or rows ahead of a portion's first (an engine's step); they may then be read before
+    the kernel ahead in the stream is complete."""
     K = cache.shape[2] if cache.ndim == 4 else 0
     if K < 1 or heads < 1 or heads % K:
         raise KernelError(f"{heads} query heads on {K} kv heads")
@@ -964,7 +966,7 @@ def attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, layer
             spans = torch.empty(floats, dtype=torch.float32, device=out.device) if buf is None else buf("kv4_spans", (floats,), torch.float32)
         _check(_c.xr_kv4_attention(q.data_ptr(), out.data_ptr(), code, *args, at_start, at_len, at_pos, block_tables.data_ptr(), _ptr(spans),
                                    floats, q_row, n_seg, heads, head_dim, max_pages, window, scale, _ptr(sink),
-                                   softcap, keep_first, _ptr(bias), _bias_len(bias), most, *cut, _stream()), "attention_kv4")
+                                   softcap, keep_first, _ptr(bias), _bias_len(bias), most, int(early), *cut, _stream()), "attention_kv4")
         _count(2 if floats else 1)
 
 FLAT_TILE = 128       # the flat array's first key of a portion is a multiple of this

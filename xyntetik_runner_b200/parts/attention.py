@@ -298,7 +298,7 @@ class GQAAttention(Mixer):
             kernels.attention_kv4(qkv[:, :self.H * self.hd], o, four, lay.layer_in_group, ctx.page_size, ctx.seg_start, ctx.seg_len, ctx.seg_pos0, bt, self.H,
                                   self.hd, self.scale, (ctx.host["seg_len"], ctx.host["seg_pos0"]), window=self.window or 0, sink=self.sink,
                                   softcap=self.softcap, keep_first=self.keep_first, bias=self.dist_bias, max_kv_len=ctx.max_kv_len if ctx.decode_only else 0,
-                                  buf=ctx.buf)
+                                  buf=ctx.buf, early=True)
             counters["kv4"] += 1
         elif USE_MMA and kernels.attention_mma_supported(ctx.act_dtype, self.H, self.K, self.hd):
             # (what the portions' lengths say is the same for every layer of the step)
