@@ -102,6 +102,21 @@ def test_what_portions_ask_for():
         plan(np.zeros(8, dtype=np.int32)[::2], np.zeros(8, dtype=np.int32)[::2])
 
 
+@pytest.mark.parametrize("lens,K,G,D,cut", [
+    ([60] * 70, 40, 1, 64, "whole"), ([64], 1, 4, 128, "whole"), ([640], 1, 4, 128, "cluster"), ([640], 8, 4, 64, "cluster"), ([8192] * 8, 8, 4, 128, "cluster"),
+    ([20000], 1, 8, 128, "spans"), ([131072], 8, 4, 128, "spans")])
+def test_how_requests_are_cut(lens, K, G, D, cut):
+    """Whole, in spans that a cluster combines, in spans with scratch and a second kernel; every tile belongs to a span, with requests as long as is announced too."""
+    n = np.array(lens, dtype=np.int32)
+    for most in (0, 3 * max(lens)):
+        said = dict(zip(kernels._PLAN, kernels.kv4_plan((np.ones_like(n), n - 1), len(lens), K, G, D, 64, kernels.BF16, 0, 0, 1 << 30, most)))
+        assert said["short"] == len(lens) and said["long"] == 0 and said["row_blocks"] == 1
+        if most == 0:
+            assert ("whole" if said["splits"] == 1 else "cluster" if said["clustered"] else "spans") == cut
+        assert (said["floats"] > 0) == (said["splits"] > 1 and not said["clustered"]) and (not said["clustered"] or said["splits"] <= 8)
+        assert said["splits"] * said["span_tiles"] * 64 >= max(lens)
+
+
 def test_engine_refuses_before_it_looks_for_a_device():
     from xyntetik_runner_b200.engine.engine import Engine, EngineParams
     with pytest.raises(ValueError, match="same or int4"):

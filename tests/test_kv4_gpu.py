@@ -226,3 +226,200 @@ def test_attention(contexts, T, H, K, D, P, dtype, window, keep, sink, cap, bias
         kernels.tc_check_status(torch.device(DEV))
         check(out, q, held, plain, Ts, starts, pos0, H, D, dtype)
         assert torch.all(out[q.shape[0]:] == 9.0)
+
+
+def run_case(case, **change):
+    from xyntetik_runner_b200 import kernels
+    args, q, held, plain, Ts, starts, pos0 = attention_case(*case)
+    H, D, dtype = case[2], case[4], case[6]
+    args.update(change)
+    out = torch.full((q.shape[0], H * D), 9.0, dtype=dtype, device=DEV)
+    kernels.attention_kv4(q.to(DEV), out, **args)
+    kernels.tc_check_status(torch.device(DEV))
+    return out, args, q, held, plain, Ts, starts, pos0
+
+
+@pytest.mark.parametrize("case", [
+    ([640], 1, 4, 1, 128, 64, BF16, 0, 0, 1, 0, 0), ([2500], 1, 4, 1, 128, 64, BF16, 0, 0, 1, 0, 0), ([9000, 300], 1, 2, 1, 64, 64, BF16, 0, 0, 0, 0, 0),
+    ([20000], 1, 8, 1, 128, 64, BF16, 0, 0, 0, 0, 0), ([6000], 2, 2, 1, 256, 16, F32, 0, 0, 1, 0, 0), ([5000] * 2, 1, 16, 8, 64, 24, BF16, 3000, 40, 0, 0, 0),
+    ([60] * 70, 1, 40, 40, 64, 16, BF16, 0, 0, 0, 0, 0)])
+def test_requests_that_are_cut(case):
+    """One block a request, spans that meet in a cluster, spans that a second kernel combines (test_kv4_cpu.py: which are which)."""
+    out, args, q, held, plain, Ts, starts, pos0 = run_case(case)
+    check(out, q, held, plain, Ts, starts, pos0, case[2], case[4], case[6])
+
+
+def test_empty_portions():
+    """Portions of no tokens beside others, and a call without any token."""
+    from xyntetik_runner_b200 import kernels
+    case = ([50, 7, 90], [1, 0, 3], 4, 2, 64, 16, BF16, 0, 0, 0, 0, 0)
+    out, args, q, held, plain, Ts, starts, pos0 = run_case(case)
+    check(out, q, held, plain, Ts, starts, pos0, 4, 64, BF16)
+    none = np.zeros(3, dtype=np.int32)
+    args.update(seg_len=i32(none), lengths=(none, args["lengths"][1]))
+    kernels.attention_kv4(q[:0].to(DEV), out[:0], **args)
+
+
+def test_captured_and_replayed():
+    """A captured call serves other positions, longer and shorter than those it was captured with; two graphs side by side in one stream."""
+    from xyntetik_runner_b200 import kernels
+    case = ([300, 40], 1, 8, 2, 128, 64, BF16, 0, 0, 0, 0, 0)
+    args, q, held, plain, Ts, starts, pos0 = attention_case(*case)
+    qd, graphs, outs = q.to(DEV), [], []
+    pos = args["seg_pos0"]
+    for ends in ([300, 40], [20, 10]):                               # captured as if the requests were this long
+        at = np.array([e - 1 for e in ends], dtype=np.int32)
+        pos.copy_(i32(at))
+        out = torch.zeros(2, 8 * 128, dtype=BF16, device=DEV)
+        call = lambda: kernels.attention_kv4(qd, out, **{**args, "lengths": (args["lengths"][0], at), "max_kv_len": 320})
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call()
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call()
+        graphs.append(g)
+        outs.append(out)
+    for ends in ([300, 40], [20, 10], [129, 1], [65, 33]):
+        at = np.array([e - 1 for e in ends])
+        pos.copy_(i32(at))
+        for g, out in zip(graphs, outs):
+            out.zero_()
+            g.replay()
+        for out in outs:
+            check(out, q, held, plain, Ts, starts, at, 8, 128, BF16)
+
+
+def test_store_read_and_attend_on_another_stream():
+    """The three together, as a step uses them, on a stream of their own and twice over."""
+    from xyntetik_runner_b200 import kernels
+    g = torch.Generator().manual_seed(9)
+    P, K, H, D, lens = 16, 2, 4, 64, [33, 70]
+    bt, n_pages = tables(lens, P, g)
+    rows = [torch.randn(sum(lens), K * D, generator=g).to(BF16) for _ in (0, 1)]
+    q = torch.randn(2, H * D, generator=g).to(BF16)
+    pos, seg = np.concatenate([np.arange(n) for n in lens]), np.repeat(np.arange(2), lens)
+    side = torch.cuda.Stream()
+    dev = [x.to(DEV) for x in (*rows, q)]
+    ints = [i32(x) for x in (pos, seg, bt, [0, 1], [1, 1], [n - 1 for n in lens], [0, 0], lens)]
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            cache = kernels.kv4_cache(n_pages, 1, K, D, P, DEV)
+            kernels.kv4_store(dev[0], dev[1], ints[0], ints[1], ints[2], cache, 0, P)
+            out, back = torch.empty_like(dev[2]), torch.empty(3 + 5, 2, K, P, D, dtype=BF16, device=DEV)
+            kernels.attention_kv4(dev[2], out, cache, 0, P, ints[3], ints[4], ints[5], ints[2], H, D, D ** -0.5,
+                                  (np.ones(2, dtype=np.int32), np.array(lens, dtype=np.int32) - 1))
+            kernels.kv4_read(cache, 0, P, ints[2], ints[6], ints[7], back)
+    torch.cuda.current_stream().wait_stream(side)
+    held = []
+    for r in range(2):
+        for x in rows:
+            held.append(plain_kv4.quantised(x[seg == r].reshape(-1, D))[2].reshape(-1, K, D))
+    check(out, q, held, dict(scale=D ** -0.5), [1, 1], [0, 1], [n - 1 for n in lens], H, D, BF16)
+    got = back.double().cpu()
+    assert torch.equal(got[:3].permute(1, 0, 3, 2, 4).reshape(2, -1, K, D)[:, :33], torch.stack(held[:2]))
+    assert torch.equal(got[3:].permute(1, 0, 3, 2, 4).reshape(2, -1, K, D)[:, :70], torch.stack(held[2:]))
+
+
+def check_nan(got, want, tol):
+    got = got.double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    fine = ~torch.isnan(want)
+    assert torch.all((got - want).abs()[fine] <= tol[fine])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("what,at", [("k", 20), ("v", 20), ("v", 37), ("k", 37), ("v", 38), ("v", 3), ("k", 3)])
+def test_rows_that_are_no_numbers(what, at, dtype):
+    """A NaN among a request's rows: in a portion of four tokens at 36 .. 39 with a window of 30, whoever does not see the row is as ever, a key's NaN
+    reaches whoever sees it, a value's its group of 32 elements."""
+    from xyntetik_runner_b200 import kernels
+    g = torch.Generator().manual_seed(at)
+    P, K, H, D, n, T = 8, 1, 2, 64, 40, 4
+    k, v = (torch.randn(n, D, generator=g).to(dtype) for _ in (0, 1))
+    (k if what == "k" else v)[at, 5] = math.nan
+    bt, n_pages = tables([n], P, g)
+    cache = kernels.kv4_cache(n_pages, 1, K, D, P, DEV)
+    kernels.kv4_store(k.to(DEV), v.to(DEV), i32(np.arange(n)), i32(np.zeros(n)), i32(bt), cache, 0, P)
+    q = torch.randn(T, H * D, generator=g).to(dtype)
+    out = torch.empty(T, H * D, dtype=dtype, device=DEV)
+    one = np.array([T], dtype=np.int32), np.array([n - T], dtype=np.int32)
+    kernels.attention_kv4(q.to(DEV), out, cache, 0, P, i32([0]), i32([T]), i32([n - T]), i32(bt), H, D, 0.125, one, window=30)
+    held = [plain_kv4.quantised(x)[2].reshape(n, 1, D) for x in (k, v)]
+    want, size, raw = plain_kv4.attention(q.double().reshape(T, H, D), held[0], held[1], n - T, 0.125, window=30)
+    tol = plain_kv4.tolerance(want, size, raw, D, dtype)
+    check_nan(out.reshape(T, H, D), want, tol)
+    assert torch.isnan(want).any() == (at > n - T - 30)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_values_of_many_sizes(dtype):
+    """Values that grow and shrink by powers of ten along a request, zeros first; queries of tiny and huge size, zeros, infinities and NaN among them."""
+    from xyntetik_runner_b200 import kernels
+    g = torch.Generator().manual_seed(4)
+    P, K, D, n = 16, 1, 128, 400
+    v = torch.randn(n, D, generator=g) * torch.pow(10.0, torch.linspace(-9, 9, n))[:, None]
+    v[:130] = 0.0
+    k = torch.randn(n, D, generator=g)
+    k, v = k.to(dtype), v.to(dtype)
+    q = torch.randn(8, D, generator=g)
+    q[1] *= 1e-30
+    q[2] = 0.0
+    q[3] *= 30.0
+    q[4, :100] *= 1e-6
+    q[5, 7] = math.nan
+    q[6, 9] = math.inf
+    q = q.to(dtype).reshape(1, 8 * D)
+    bt, n_pages = tables([n], P, g)
+    cache = kernels.kv4_cache(n_pages, 1, K, D, P, DEV)
+    kernels.kv4_store(k.to(DEV), v.to(DEV), i32(np.arange(n)), i32(np.zeros(n)), i32(bt), cache, 0, P)
+    out = torch.empty(1, 8 * D, dtype=dtype, device=DEV)
+    kernels.attention_kv4(q.to(DEV), out, cache, 0, P, i32([0]), i32([1]), i32([n - 1]), i32(bt), 8, D, 0.09, (np.array([1], dtype=np.int32), np.array([n - 1], dtype=np.int32)))
+    held = [plain_kv4.quantised(x)[2].reshape(n, 1, D) for x in (k, v)]
+    qq = q.double().reshape(1, 8, D)
+    want, size, raw = plain_kv4.attention(qq, held[0], held[1], n - 1, 0.09)
+    tol = plain_kv4.tolerance(want, size, raw, D, dtype)
+    got = out.double().cpu().reshape(1, 8, D)
+    assert torch.isnan(got[0, 5:7]).all()                           # (a score of an infinity, or of no number)
+    fine = [0, 1, 2, 3, 4, 7]
+    assert torch.all((got - want).abs()[0, fine] <= tol[0, fine]), ((got - want).abs() / tol)[0, fine].max()
+
+
+def test_pages_beyond_four_gigabytes():
+    """A cache whose pages lie further apart than 32 bits of bytes."""
+    from xyntetik_runner_b200 import kernels
+    K, D, P, n = 8, 128, 64, 150
+    per = K * kernels.kv4_block_bytes(D, P)
+    pages = (1 << 32) // per + 40
+    g = torch.Generator().manual_seed(2)
+    cache = torch.empty((pages, 1, K, kernels.kv4_block_bytes(D, P)), dtype=torch.uint8, device=DEV)
+    bt = i32([[pages - 1, 3, pages - 7, -1]])
+    k, v = (torch.randn(n, K * D, generator=g).to(BF16) for _ in (0, 1))
+    kernels.kv4_store(k.to(DEV), v.to(DEV), i32(np.arange(n)), i32(np.zeros(n)), bt, cache, 0, P)
+    q = torch.randn(1, K * D, generator=g).to(BF16)
+    out, back = torch.empty(1, K * D, dtype=BF16, device=DEV), torch.empty(3, 2, K, P, D, dtype=BF16, device=DEV)
+    kernels.attention_kv4(q.to(DEV), out, cache, 0, P, i32([0]), i32([1]), i32([n - 1]), bt, K, D, 0.09, (np.array([1], dtype=np.int32), np.array([n - 1], dtype=np.int32)))
+    kernels.kv4_read(cache, 0, P, bt, i32([0]), i32([n]), back)
+    held = [plain_kv4.quantised_rows(x.reshape(n, K, D)) for x in (k, v)]
+    check(out, q, held, dict(scale=0.09), [1], [0], [n - 1], K, D, BF16)
+    assert torch.equal(back.double().cpu().permute(1, 0, 3, 2, 4).reshape(2, -1, K, D)[:, :n], torch.stack(held))
+
+
+def test_refused_by_the_launchers():
+    """What the wrappers let through and the library does not take: a cache off its border, a scale that is not positive is the wrappers'."""
+    from xyntetik_runner_b200 import kernels
+    raw = torch.zeros(2 * 1 * 1 * kernels.kv4_block_bytes(64, 16) + 16, dtype=torch.uint8, device=DEV)
+    off = raw[4:4 + 2 * kernels.kv4_block_bytes(64, 16)].view(2, 1, 1, -1)
+    k = torch.zeros(1, 64, dtype=BF16, device=DEV)
+    with pytest.raises(kernels.KernelError, match="refuses these sizes"):
+        kernels.kv4_store(k, k, i32([0]), i32([0]), i32([[0]]), off, 0, 16)
+    with pytest.raises(kernels.KernelError, match="refuses these sizes"):
+        kernels.kv4_read(off, 0, 16, i32([[0]]), i32([0]), i32([1]), torch.zeros(1, 2, 1, 16, 64, device=DEV))
+    with pytest.raises(kernels.KernelError, match="refuses these sizes"):
+        kernels.attention_kv4(k, torch.zeros_like(k), off, 0, 16, i32([0]), i32([1]), i32([0]), i32([[0]]), 1, 64, 0.1,
+                              (np.array([1], dtype=np.int32), np.array([0], dtype=np.int32)))
+    with pytest.raises(kernels.KernelError, match="current CUDA device"):
+        kernels.kv4_store(k.cpu(), k.cpu(), i32([0]), i32([0]), i32([[0]]), off, 0, 16)

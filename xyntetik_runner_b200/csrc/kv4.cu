@@ -225,41 +225,48 @@ k_kv4_read(Kv4ReadArgs a) {
     for (int kvh = blockIdx.y; kvh < a.c.K; kvh += gridDim.y) {
         const uint8_t* run = a.c.run(max(page, 0), kvh);
         T* dst = (T*)a.out + ((size_t)j * 2 * a.c.K + kvh) * P * a.D;
+        if constexpr (WS > 0) {
+            // four words of the keys and four of the values a thread, their loads side by side
+            constexpr int N = 4;
+            for (int i0 = threadIdx.x; i0 < P << WS; i0 += N * 256) {
+                uint32_t word[2][N], s[2][N];
+#pragma unroll
+                for (int plane = 0; plane < 2; plane++)
+#pragma unroll
+                    for (int e = 0; e < N; e++) {
+                        const int i = i0 + e * 256, tok = i >> WS;
+                        word[plane][e] = s[plane][e] = 0;
+                        if (tok < a1 && (tok >= a0 || tok < kept)) {
+                            word[plane][e] = __ldcs(reinterpret_cast<const uint32_t*>(run + a.c.codes_at(plane)) + i);
+                            s[plane][e] = __ldg(reinterpret_cast<const unsigned short*>(run + a.c.scales_at(plane)) + (i >> 2));
+                        }
+                    }
+#pragma unroll
+                for (int plane = 0; plane < 2; plane++)
+#pragma unroll
+                    for (int e = 0; e < N; e++) {
+                        const int i = i0 + e * 256;
+                        if (i >= P << WS) break;
+                        kv4_eight<T>(word[plane][e], s[plane][e], dst + plane * plane_step + 8 * (size_t)i);
+                    }
+            }
+            continue;
+        }
 #pragma unroll
         for (int plane = 0; plane < 2; plane++) {
             const uint32_t* codes = reinterpret_cast<const uint32_t*>(run + a.c.codes_at(plane));
             const unsigned short* scales = reinterpret_cast<const unsigned short*>(run + a.c.scales_at(plane));
             T* to = dst + plane * plane_step;
-            if constexpr (WS > 0) {
-                // four words a thread, their loads side by side
-                constexpr int N = 4;
-                for (int i0 = threadIdx.x; i0 < P << WS; i0 += N * 256) {
-                    uint32_t word[N], s[N];
+            for (int i = threadIdx.x; i < P * used; i += 256) {
+                const int tok = i / used, w = i - tok * used;
+                uint32_t word = 0, s = 0;
+                if (tok < a1 && (tok >= a0 || tok < kept)) { word = __ldg(codes + tok * words + w); s = __ldg(scales + tok * (words >> 2) + (w >> 2)); }
+                if (a.wide && 8 * w + 8 <= a.D) { kv4_eight<T>(word, s, to + (size_t)tok * a.D + 8 * w); continue; }
+                uint32_t v[4];
+                kv4_values(word, s, v);
 #pragma unroll
-                    for (int e = 0; e < N; e++) {
-                        const int i = i0 + e * 256, tok = i >> WS;
-                        word[e] = s[e] = 0;
-                        if (tok < a1 && (tok >= a0 || tok < kept)) { word[e] = __ldg(codes + i); s[e] = __ldg(scales + (i >> 2)); }
-                    }
-#pragma unroll
-                    for (int e = 0; e < N; e++) {
-                        const int i = i0 + e * 256;
-                        if (i >= P << WS) break;
-                        kv4_eight<T>(word[e], s[e], to + 8 * (size_t)i);
-                    }
-                }
-            } else {
-                for (int i = threadIdx.x; i < P * used; i += 256) {
-                    const int tok = i / used, w = i - tok * used;
-                    uint32_t word = 0, s = 0;
-                    if (tok < a1 && (tok >= a0 || tok < kept)) { word = __ldg(codes + tok * words + w); s = __ldg(scales + tok * (words >> 2) + (w >> 2)); }
-                    if (a.wide && 8 * w + 8 <= a.D) { kv4_eight<T>(word, s, to + (size_t)tok * a.D + 8 * w); continue; }
-                    uint32_t v[4];
-                    kv4_values(word, s, v);
-#pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        if (8 * w + e < a.D) to[(size_t)tok * a.D + 8 * w + e] = xr_from_f32<T>(__uint_as_float(e & 1 ? v[e >> 1] & 0xffff0000u : v[e >> 1] << 16));
-                }
+                for (int e = 0; e < 8; e++)
+                    if (8 * w + e < a.D) to[(size_t)tok * a.D + 8 * w + e] = xr_from_f32<T>(__uint_as_float(e & 1 ? v[e >> 1] & 0xffff0000u : v[e >> 1] << 16));
             }
         }
     }
