@@ -87,12 +87,31 @@ def test_attention_refuses(change, message):
 def test_what_portions_ask_for():
     """Pages that are read back, row tiles and scratch, from lengths on the host (the library's part that needs no device)."""
     a = lambda *x: np.array(x, dtype=np.int32)
-    plan = lambda l, p, window=0, keep=0, most=0, n=100: kernels.kv4_plan((l, p), n, 2, 4, 64, 16, kernels.BF16, window, keep, most).tolist()[:8]
-    assert plan(a(1, 20), a(0, 15)) == [0, 2, 0, 1 + 3, 20, 2, 1 + 2, 35]
-    assert plan(a(0, 20), a(7, 15))[:4] == [0, 1, 0, 3]
-    assert plan(a(1), a(100), 10, 20)[3] == 2 + 2           # rows 91 .. 100 lie in pages 5 and 6, the kept in 0 and 1
-    assert plan(a(1), a(40), 20, 33)[3] == 1 + 2            # kept rows that the window's pages hold are not there twice
-    for l, p, n in ((a(-1), a(0), 9), (a(1), a(-1), 9), (a(5, 5), a(0, 0), 9)):
+    # (2,000 pairs: more row blocks than go by the codes, whatever the portions)
+    plan = lambda l, p, window=0, keep=0, most=0, n=100: kernels.kv4_plan((l, p), n, 2000, 4, 64, 16, kernels.BF16, window, keep, most).tolist()[:9]
+    assert plan(a(1, 60), a(0, 15)) == [0, 2, 0, 1 + 5, 60, 1 + 2, 1 + 4, 75, 0]
+    assert plan(a(0, 60), a(7, 15))[:4] == [0, 1, 0, 5]
+    assert plan(a(30), a(100), 10, 20)[3] == 2 + 4          # rows 91 .. 129 lie in pages 5 to 8, the kept in 0 and 1
+    assert plan(a(30), a(40), 20, 33)[3] == 1 + 4           # kept rows that the window's pages hold are not there twice
+    # anywhere up to `mx` rows: all pages of them, or the window's at its worst place and the kept
+    far = lambda l, p, window, keep, mx: kernels.kv4_plan((l, p), 100, 2000, 4, 64, 16, kernels.BF16, window, keep, 0, mx).tolist()
+    assert far(a(30), a(100), 0, 0, 500)[3] == 32 and far(a(30), a(100), 0, 0, 500)[7] == 500 and far(a(30), a(100), 0, 0, 90)[3] == 9
+    for window, keep in ((10, 20), (1, 0), (33, 5), (400, 3)):
+        held = far(a(30), a(0), window, keep, 300)[3]
+        need = [plan(a(30), a(p), window, keep)[3] for p in range(271)]
+        assert max(need) <= held <= max(need) + 1
+    assert plan(a(1, 60), a(0, 15), most=64)[:2] == [1, 1] and plan(a(1, 60), a(0, 15), most=64)[8] == 64
+    few = kernels.kv4_plan((a(1, 60), a(0, 15)), 100, 2, 4, 64, 16, kernels.BF16, 0, 0, 64).tolist()
+    assert few[:2] == [2, 0] and few[8] == 1 << 30          # 30 row blocks: by the codes
+    at = lambda kv, *l, d=128: kernels.kv4_plan((a(*l), a(*[900] * len(l))), 400, kv, 4, d, 16, kernels.BF16, 0, 0, 64).tolist()[:2]
+    assert at(16, 64) == [1, 0] and at(17, 64) == [0, 1]    # full row tiles: 256 row blocks, 272
+    assert at(20, 64, d=64) == [1, 0] and at(21, 64, d=64) == [0, 1]
+    assert at(16, 64, 1) == [2, 0] and at(17, 64, 1) == [1, 1]
+    assert at(64, 24) == [1, 0] and at(65, 24) == [0, 1]    # a part full one: 384, 390
+    assert at(96, 24, d=64) == [1, 0] and at(97, 24, d=48) == [0, 1]
+    assert at(8, 64, 64) == [2, 0] and at(12, 64, 64) == [0, 2]
+    assert at(16, 64, 24) == [2, 0] and at(18, 64, 24) == [0, 2]
+    for l, p, n in ((a(-1), a(0), 9), (a(1), a(-1), 9), (a(5, 5), a(0, 0), 9), (a(8), a(2 ** 31 - 8), 9)):
         with pytest.raises(kernels.KernelError, match="does not hold"):
             plan(l, p, n=n)
     for l, p in ((a(1), a(1, 2)), (a(1).astype(np.int64), a(1))):
@@ -115,6 +134,17 @@ def test_how_requests_are_cut(lens, K, G, D, cut):
             assert ("whole" if said["splits"] == 1 else "cluster" if said["clustered"] else "spans") == cut
         assert (said["floats"] > 0) == (said["splits"] > 1 and not said["clustered"]) and (not said["clustered"] or said["splits"] <= 8)
         assert said["splits"] * said["span_tiles"] * 64 >= max(lens)
+
+
+def test_a_plan_through_either_way_of_calling(monkeypatch):
+    """Buffers reach the library from the direct calls and through ctypes alike."""
+    l, p = np.array([1, 70, 0], dtype=np.int32), np.array([900, 30, 5], dtype=np.int32)
+    args = ((l, p), 80, 900, 4, 64, 16, kernels.BF16, 100, 3, 64)
+    direct = kernels.kv4_plan(*args)
+    monkeypatch.setattr(kernels, "_c", kernels._CtypesCalls(kernels.lib()))
+    assert kernels.kv4_plan(*args) == direct and direct[0] == 1 and direct[1] == 1
+    with pytest.raises((BufferError, ValueError), match="contiguous"):
+        kernels.kv4_plan((np.zeros(8, dtype=np.int32)[::2], np.zeros(8, dtype=np.int32)[::2]), *args[1:])
 
 
 def test_engine_refuses_before_it_looks_for_a_device():

@@ -86,6 +86,32 @@ def test_store_and_read(held, T, K, D, Vd, P, dtype, extra):
         assert torch.equal(out.double().cpu(), exp) and torch.equal(where.cpu(), torch.from_numpy(exp_where))
 
 
+def test_read_with_kept_rows():
+    """Kept first rows ahead of a window's, requests that have none, rows that both name, pages that were given back."""
+    from xyntetik_runner_b200 import kernels
+    g = torch.Generator().manual_seed(8)
+    P, K, D, lens, first, keep = 8, 2, 48, [100, 20, 9], [61, 15, 9], 11
+    bt, n_pages = tables(lens, P, g)
+    k, v = (torch.randn(sum(lens), K * D, generator=g).to(BF16) for _ in (0, 1))
+    pos, seg = np.concatenate([np.arange(n) for n in lens]), np.repeat(np.arange(3), lens)
+    cache = kernels.kv4_cache(n_pages, 1, K, D, P, DEV)
+    kernels.kv4_store(k.to(DEV), v.to(DEV), i32(pos), i32(seg), i32(bt), cache, 0, P)
+    bt[0, 2:7] = -1
+    held = torch.stack([plain_kv4.quantised(x.reshape(-1, D))[2].reshape(-1, K, D) for x in (k, v)])
+    want, pages = [], {0: [0, 1, 7, 8, 9, 10, 11, 12], 1: [0, 1, 2], 2: []}
+    for r in range(3):
+        for pi in pages[r]:
+            page = torch.zeros(2, K, P, D, dtype=torch.float64)
+            for t in range(P):
+                p = pi * P + t
+                if p < lens[r] and (p < keep or p >= first[r]) and bt[r, pi] >= 0:
+                    page[:, :, t] = held[:, int(np.flatnonzero((seg == r) & (pos == p))[0])]
+            want.append(page)
+    out = torch.full((len(want) + 1, 2, K, P, D), 3.0, dtype=BF16, device=DEV)
+    kernels.kv4_read(cache, 0, P, i32(bt), i32(first), i32(lens), out, keep_first=keep)
+    assert torch.equal(out[:-1].double().cpu(), torch.stack(want)) and torch.all(out[-1] == 3.0)
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, 2.0 ** 120, -2.0 ** 121, 2.0 ** 119, -2.0 ** -96, 2.0 ** -97, 0.0])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_borders_of_what_is_held(bad, dtype):
@@ -163,10 +189,12 @@ ATT = [  # contexts, tokens, H, K, D, page, dtype, window, keep, sink, cap, bias
     ([700], 1, 8, 1, 128, 16, BF16, 0, 0, 1, 0, 0), ([333, 40], 1, 4, 4, 256, 24, BF16, 0, 0, 0, 0, 0), ([100, 31], 1, 5, 1, 100, 40, BF16, 0, 0, 0, 0, 0),
     ([90], 3, 6, 2, 80, 32, BF16, 0, 0, 0, 0, 0), ([200, 17], 4, 16, 4, 128, 64, BF16, 0, 0, 1, 0, 0), ([150, 6], 6, 14, 2, 64, 8, BF16, 0, 0, 0, 20.0, 0),
     ([500, 260], 1, 8, 2, 128, 64, BF16, 100, 0, 0, 0, 0), ([500, 60], 1, 8, 2, 128, 16, BF16, 33, 5, 1, 0, 40), ([400], 5, 4, 1, 64, 16, BF16, 64, 70, 0, 0, 200),
-    ([300], 1, 71, 1, 64, 64, BF16, 0, 0, 0, 0, 0), ([120], 2, 20, 1, 192, 64, BF16, 50, 3, 1, 0, 0), ([77], 1, 3, 3, 16, 8, BF16, 0, 0, 0, 0, 0),
+    ([300], 1, 71, 1, 64, 64, BF16, 0, 0, 0, 0, 0), ([200], 3, 130, 2, 64, 64, BF16, 0, 0, 0, 0, 0), ([40], 40, 24, 1, 64, 16, F32, 0, 0, 0, 0, 0), ([120], 2, 20, 1, 192, 64, BF16, 50, 3, 1, 0, 0), ([77], 1, 3, 3, 16, 8, BF16, 0, 0, 0, 0, 0),
     ([1, 90], 1, 4, 2, 64, 64, F32, 0, 0, 0, 0, 0), ([333], 1, 8, 2, 128, 64, F32, 0, 0, 1, 30.0, 0), ([130, 20], 7, 6, 3, 100, 24, F32, 40, 9, 0, 0, 30),
     ([60], 60, 4, 2, 128, 16, F32, 0, 0, 0, 0, 0), ([80], 3, 2, 1, 256, 64, F32, 0, 0, 0, 0, 0),
-    # portions that are read back for the prompt kernels, beside short ones
+    # portions that are read back for the prompt kernels, beside short ones (enough row blocks for that; then fewer)
+    ([90, 30], [70, 5], 128, 16, 128, 64, BF16, 0, 0, 0, 0, 0), ([150], 33, 264, 66, 64, 16, BF16, 40, 5, 1, 0, 0), ([100], 80, 117, 39, 48, 24, BF16, 30, 10, 0, 0, 0),
+    ([200], 64, 82, 41, 64, 64, BF16, 0, 0, 0, 15.0, 0), ([90, 12, 110], [70, 1, 50], 64, 32, 128, 16, BF16, 60, 0, 1, 0, 70),
     ([90], 70, 8, 2, 128, 64, BF16, 0, 0, 0, 0, 0), ([150], 33, 4, 2, 64, 16, BF16, 40, 5, 1, 0, 0), ([100], 80, 3, 1, 48, 24, BF16, 30, 10, 0, 0, 0),
     ([70], 40, 3, 1, 100, 24, BF16, 0, 0, 0, 0, 0), ([120], 100, 2, 2, 256, 64, BF16, 0, 0, 0, 0, 0)]
 
@@ -220,6 +248,8 @@ def test_attention(contexts, T, H, K, D, P, dtype, window, keep, sink, cap, bias
     args, q, held, plain, Ts, starts, pos0 = attention_case(contexts, T, H, K, D, P, dtype, window, keep, sink, cap, bias)
     wide = torch.zeros(q.shape[0], H * D + 24, dtype=dtype, device=DEV)          # q's rows lie in wider ones
     wide[:, :H * D] = q.to(DEV)
+    if sum(T if isinstance(T, list) else [T]) * H > 5000 and dtype is BF16:      # (the cases that are there for the prompt kernels go through them)
+        assert kernels.kv4_plan(args["lengths"], q.shape[0], K, H // K, D, P, kernels.BF16, window, keep, 64)[1] > 0
     for rows in (q.to(DEV), wide, wide[:, :H * D]):
         out = torch.full((q.shape[0] + 3, H * D), 9.0, dtype=dtype, device=DEV)
         kernels.attention_kv4(rows, out[:q.shape[0]], **args)
@@ -290,6 +320,36 @@ def test_captured_and_replayed():
             g.replay()
         for out in outs:
             check(out, q, held, plain, Ts, starts, at, 8, 128, BF16)
+
+
+@pytest.mark.parametrize("window,keep", [(0, 0), (70, 20)])
+@pytest.mark.parametrize("said", [0, 450])
+def test_prompt_portions_captured_and_replayed(said, window, keep):
+    """Portions that are read back, captured near the start of their requests and replayed further on, where the rows they see take more pages."""
+    from xyntetik_runner_b200 import kernels
+    H, K, D, P = 64, 8, 64, 16
+    args, q, held, plain, Ts, starts, pos0 = attention_case([450, 300], [100, 50], H, K, D, P, BF16, 0, 0, 0, 0, 0)
+    args.update(window=window, keep_first=keep)
+    plain.update(window=window, keep=keep)
+    qd, pos, at = q.to(DEV), args["seg_pos0"], np.array([20, 0], dtype=np.int32)
+    assert kernels.kv4_plan((args["lengths"][0], at), 150, K, H // K, D, P, kernels.BF16, window, keep, 64)[1] == 2
+    out = torch.zeros(150, H * D, dtype=BF16, device=DEV)
+    call = lambda: kernels.attention_kv4(qd, out, **{**args, "lengths": (args["lengths"][0], at), "max_kv_len": said})
+    pos.copy_(i32(at))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call()
+    for where in ([20, 0], [350, 250], [0, 123], [337, 17]):
+        pos.copy_(i32(where))
+        out.zero_()
+        g.replay()
+        kernels.tc_check_status(torch.device(DEV))
+        check(out, q, held, plain, Ts, starts, where, H, D, BF16)
 
 
 def test_store_read_and_attend_on_another_stream():

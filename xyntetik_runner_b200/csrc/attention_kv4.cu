@@ -9,17 +9,30 @@
 // The keys are the M side of the matrix instruction (m16n8k16), the packed query rows (row i: token i / G, head i % G) the N side: eight
 // rows cost one instruction where rows on M would cost a half empty one.  S^T = K Q^T has a key's scores for two rows in a thread;
 // O^T = V^T P^T has two neighbouring elements of the value for the same two rows, so that the running maximum's factor is one number a
-// column in both.  P^T as the second product's operand is S^T turned by movmatrix.
+// column in both.  P^T as the second product's operand is S^T turned by movmatrix.  A block takes eight rows, or sixteen where some request has more
+// than eight; a request with more rows than a block takes several (and reads its keys as often).
 //
-// A fragment never leaves the thread that loads it: a thread's word of eight codes gives, pair by pair (a shift, a mask, and one fused
-// product and sum that takes off the bias and multiplies by the group's scale, exactly), the eight neighbouring elements of a key
-// that two k-steps want from it; and the words of two keys, their halves brought together by two byte permutations, give the pairs over KEYS
-// that the second product wants, for eight elements of the value.  The order of elements along k and of keys along k is free as long as both
-// operands share it: element order is the words', key order is `at_key` below, chosen so that neither load meets a bank twice too often.
+// Codes become operands without leaving the thread that loads them.  Two shifts and four masks bring a word's eight codes into the mantissas of float16
+// numbers, 256 + u and 16 + u by turns (u the code plus 8).  Keys are multiplied as that, exactly, into sums that start at what takes the bias off; a
+// group of 32 elements is two k-steps, and its scale a factor on their float32 result.  (bfloat16 operands, which hold one code at a time, want four
+// shifts and a fused product and sum a pair.)  The bias costs the sums log2(264 / 8) bits of 24; scores
+// are off by less than the weights' rounding.  q is scaled by a power of two a row, so that its eight bits are whole in float16.  Values are
+// scaled ahead of the product, where a thread's elements share a scale and its keys do not: (256 + u) s - 264 s in one rounding, which is none, because c s
+// has eight bits.  They are in units of a power of two that follows the largest scale; weights are rounded to float16 (2^-11) once.
+// The words of two keys, their halves brought together by two byte permutations, give the pairs over KEYS that the second product wants.  The
+// order of elements along k and of keys along k is free as long as both operands share it: a4_key.
 //
-// A warp walks tiles of its own (32 keys, 64 at head size 64) through a ring of bulk copies: four contiguous pieces a tile and page.
-// The warps of a block interleave the tiles of a span and meet once, at its end.  Spans of a request are combined by k_kv4_merge, in
-// ascending order.
+// A warp walks tiles of its own (64 keys, 32 at head size 256) through a ring of asynchronous copies, 16 bytes a lane; the next page's number is asked
+// for a tile ahead.  The warps of a block interleave the tiles of a span and meet once, at its end.  Spans of a request meet in a cluster of up to
+// eight blocks through its shared memory, or leave partial sums to k_kv4_merge; either way in ascending order.
+//
+// What bounds it: 55 requests of 8,192 keys, 32 heads on 8 of 128 elements, one block a pair and three an SM, take 3.0 us a tile of every warp: 0.83 of the copy
+// peak (6.54 TB/s), and as long where the cache fits in L2, with issue slots 44 to 62 % and the integer pipe 35 to 57 % busy and the tensor cores at 19 %: what
+// is left is warps waiting for one another's results.  Around that stand what a launch costs before its first tiles are there (about 9 us
+// with all SMs' first tiles on their way at once, 5.6 with a few) and what the last round of blocks leaves idle.
+// Measured and left: four blocks an SM (64 ragged requests of 40 heads 253 us against 214: registers spill), tiles of 32 keys at three (230), the next tile's scores
+// interleaved with this tile's values (55 requests of 8,192 keys 119.9 against 107.8), bulk copies instead of cp.async (equal), e4m3 operands (the
+// instruction runs at 0.16 a cycle and SM), equal shares of all tiles for resident blocks (268 and a second kernel against 214).
 //
 // float32: a float32 number is the exact sum of three bfloat16 numbers, the held values are bfloat16 numbers, so that three products on
 // the tensor cores (q in pieces, p in pieces) give float32's precision.
@@ -38,8 +51,8 @@ struct A4Args {
     const void* q; void* out;
     Kv4Cache c;
     const int* seg_start; const int* seg_len; const int* seg_pos0; const int* block_tables;
-    float* part_acc;                  // [n_seg][K * row_blocks][splits][rows][hs]
-    float* part_ml;                   // [n_seg][K * row_blocks][splits][rows][2]
+    float* part_acc;                  // [n_seg][K][row_blocks][splits][rows][hs]
+    float* part_ml;                   // [n_seg][K][row_blocks][splits][rows][2]
     long long q_stride;
     int H, G, D, max_pages, window, keep, splits, span_tiles, row_blocks, most_rows;
     float scale, softcap;
@@ -213,7 +226,7 @@ k_kv4_attention(A4Args a) {
     constexpr int VW = S::VW, MT = S::MT;
     extern __shared__ __align__(128) uint8_t smem[];
     uint2* q_sm = (uint2*)(smem + A4_WARPS * STAGES * STAGE);                        // [P][NT][KS][32]
-    const int seg = blockIdx.z, kvh = blockIdx.y % a.c.K, rb = blockIdx.y / a.c.K, span = blockIdx.x;
+    const int seg = blockIdx.z, kvh = blockIdx.y, rb = blockIdx.x / a.splits, span = blockIdx.x - rb * a.splits;
     // (a.early: portions, block tables and the rows of earlier steps are at rest, so that tiles of such rows set out before the kernel ahead is complete)
     if (!a.early) xr_pdl_wait();
     const int L = a.seg_len[seg];
@@ -700,7 +713,7 @@ k_kv4_attention(A4Args a) {
             if (g == 0) { ml_s[(warp * RB + r) * 2] = m[nt][e] - LIFT; ml_s[(warp * RB + r) * 2 + 1] = sum; }
         }
     __syncthreads();
-    const size_t item = ((size_t)seg * gridDim.y + blockIdx.y) * a.splits + span;
+    const size_t item = (((size_t)seg * a.c.K + kvh) * a.row_blocks + rb) * a.splits + span;
     for (int q = threadIdx.x; q < rows * (HS / 4); q += A4_THREADS) {
         const int r = q / (HS / 4), d = (q % (HS / 4)) * 4;
         float mm = -INFINITY;
@@ -776,7 +789,7 @@ k_kv4_merge(A4Args a) {
     __shared__ float wgt[RB][A4_MAX_SPLITS];
     __shared__ float row_max[RB], row_sum[RB];
     __shared__ float4 part[A4_MERGE_THREADS];
-    const int seg = blockIdx.y, kvh = blockIdx.x % a.c.K, rb = blockIdx.x / a.c.K;
+    const int seg = blockIdx.y, kvh = blockIdx.x / a.row_blocks, rb = blockIdx.x - kvh * a.row_blocks;
     xr_pdl_wait();
     const int L = a.seg_len[seg];
     const long long rows_all = (long long)L * a.G;
@@ -907,7 +920,7 @@ static int a4_launch(const A4Args& a, int n_seg, cudaStream_t stream) {
     static_assert((A4_WARPS * S::RB * (S::HS + 2) + 2 * S::RB) * 4 <= A4_WARPS * S::STAGES * S::STAGE, "the warps' sums lie in the ring");
     static bool ready[XR_DEVICES];
     if (!xr_once_per_device(ready, [] { return xr_allow_smem(k_kv4_attention<NG, NT, F32, EXTRA>, S::SMEM); })) return XR_ERR_LAUNCH;
-    const dim3 grid(a.splits, a.c.K * a.row_blocks, n_seg);
+    const dim3 grid(a.splits * a.row_blocks, a.c.K, n_seg);          // (a cluster is a row block's spans)
     if (a.clustered) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = grid; cfg.blockDim = dim3(A4_THREADS); cfg.dynamicSmemBytes = S::SMEM; cfg.stream = stream;
@@ -935,35 +948,57 @@ static int a4_launch(const A4Args& a, int n_seg, int f32, int wide, cudaStream_t
     return f32 ? a4_launch<NG, 1, true>(a, n_seg, stream) : wide ? a4_launch<NG, 2, false>(a, n_seg, stream) : a4_launch<NG, 1, false>(a, n_seg, stream);
 }
 
-// What a step's portions ask for, from their lengths and first positions on the HOST: said[0] portions of 1 to `most_rows` packed rows, [1] longer ones,
-// [2] float32 values of scratch that xr_kv4_attention needs for the short ones; of the longer ones [3] the pages that xr_kv4_read writes for
-// them, [4] the most tokens, [5], [6] the row tiles of 128 and 64 packed rows, [7] the furthest end; [8] .. [12] how the short ones are cut, as
-// xr_kv4_attention takes it.  n: tokens of the step.
+// Whether a step's longer portions go by the codes or through the prompt kernels.  By the codes every 16 rows of a kv head are a row block that walks
+// the keys for itself: time follows the number of blocks, 0.045 to 0.051 ns a key and block once the SMs are busy.  The prompt kernels read the rows back once and
+// walk the keys once for 128 rows: 11.4 ns a key while tiles are fewer than SMs, 22 where a tile is part full and the mask is asked for every
+// score.  So the border is a number of row blocks, one for full tiles and one for others.  32 heads on 8 of 128 elements, codes / prompt kernels in us:
+// full tiles, 256 blocks: 20.5 / 21.8 (2 requests, 1,000 keys), 100.7 / 101.0 (2, 8,192), 101.0 / 116.3 (4, 8,192); 320: 33.5 / 22.5, 144.4 / 94.3 (1 request);
+// part full, 384 blocks: 35.3 / 33.3 (4, 1,000), 160.2 / 207.9 (4, 8,192), 36.5 / 35.9 (8, 1,000); 400: 37.5 / 31.4 (2, 1,000), 37.9 / 29.7 (1, 1,000), but
+// 163.8 / 183.2 (1, 8,192).  Of 64 elements a block is cheaper: full tiles, 320: 84.4 / 90.6 (1, 8,192), 22.2 / 20.8 (1, 1,000), 384: 92.5 / 90.5, 23.6 / 20.8; part
+// full, 448: 62.5 / 97.8, 640: 91.1 / 98.3 (4, 4,096).  Near the borders the wrong side is at most a sixth slower.  The rule asks nothing of positions, so
+// that a replayed graph may have others.
+static bool a4_by_codes(long long row_blocks, bool full, int hs) { return row_blocks <= (hs == 64 ? (full ? 320 : 576) : (full ? 256 : 384)); }
+
+// What a step's portions ask for, from their lengths and first positions on the HOST: said[0] portions that attend to the codes, [1] ones that go through the
+// prompt kernels (of more than `most_rows` packed rows, all or none of them: a4_by_codes), [2] float32 values of scratch that xr_kv4_attention needs
+// for the first; of the others [3] the pages that xr_kv4_read writes for them, [4] the most tokens, [5], [6] the row tiles of 128 and 64 packed rows, [7] the
+// furthest end; [8] the most packed rows of a portion that attends to the codes; [9] .. [13] how those are cut, as xr_kv4_attention takes it.
+// n: tokens of the step; max_kv: how far requests may get by the time the launches run (0: as far as the portions go).
 XR_EXPORT int xr_kv4_plan(const int* len, const int* pos0, int n_seg, int n, int K, int G, int D, int page_size, int dtype, int window, int keep_first,
                           int most_rows, int max_kv, long long* said) {
-    if (n_seg < 1 || n < 0 || K < 1 || G < 1 || D < 1 || D > 256 || page_size < 1 || window < 0 || keep_first < 0 || most_rows < 0) return XR_ERR_ARG;
-    long long tokens = 0;
-    for (int i = 0; i < 13; i++) said[i] = 0;
+    if (n_seg < 1 || n < 0 || K < 1 || G < 1 || D < 1 || D > 256 || page_size < 1 || window < 0 || keep_first < 0 || most_rows < 0 || max_kv < 0) return XR_ERR_ARG;
+    long long tokens = 0, row_blocks = 0;
+    bool full = true;
+    for (int i = 0; i < 14; i++) said[i] = 0;
     for (int s = 0; s < n_seg; s++) {
         const long long l = len[s], p = pos0[s], rows = l * G;
-        if (l < 0 || p < 0) return XR_ERR_ARG;
+        if (l < 0 || p < 0 || p + l > 0x7fffffffLL) return XR_ERR_ARG;
         tokens += l;
+        if (rows > most_rows) { row_blocks += (rows + 15) / 16 * K; full = full && rows % 128 == 0; }
+    }
+    if (tokens > n) return XR_ERR_ARG;
+    if (row_blocks > 0 && a4_by_codes(row_blocks, full, kv4_held(D))) most_rows = 1 << 30;
+    said[8] = most_rows;
+    for (int s = 0; s < n_seg; s++) {
+        const long long l = len[s], p = pos0[s], rows = l * G;
         if (l == 0) continue;
         if (rows <= most_rows) { said[0]++; continue; }
         said[1]++;
-        const long long first = window > 0 && p - window + 1 > 0 ? p - window + 1 : 0, from = first / page_size;
-        const long long kept = ((long long)keep_first + page_size - 1) / page_size;
-        said[3] += (window > 0 ? (kept < from ? kept : from) : 0) + (p + l - 1) / page_size - from + 1;
+        const long long first = window > 0 && p - window + 1 > 0 ? p - window + 1 : 0, from = first / page_size, end = p + l > max_kv ? p + l : max_kv;
+        const long long kept = ((long long)keep_first + page_size - 1) / page_size, all = (end - 1) / page_size + 1;
+        // (with max_kv the portion may lie anywhere up to there: a window's rows touch one page more where they begin inside one)
+        const long long seen = window > 0 ? kept + ((long long)window + l - 2) / page_size + 2 : all;
+        if (max_kv > 0) said[3] += seen < all ? seen : all;
+        else said[3] += (window > 0 ? (kept < from ? kept : from) : 0) + (p + l - 1) / page_size - from + 1;
         if (l > said[4]) said[4] = l;
         said[5] += (rows + 127) / 128;
         said[6] += (rows + 63) / 64;
-        if (p + l > said[7]) said[7] = p + l;
+        if (end > said[7]) said[7] = end;
     }
-    if (tokens > n) return XR_ERR_ARG;
     if (said[0] > 0) {
         const int hs = kv4_held(D), f32 = dtype == XR_F32;
         const A4Plan p = a4_plan(len, pos0, n_seg, K, G, hs, f32, window, window > 0 ? keep_first : 0, most_rows, max_kv);
-        said[8] = p.row_blocks; said[9] = p.wide; said[10] = p.span_tiles; said[11] = p.splits; said[12] = p.clustered;
+        said[9] = p.row_blocks; said[10] = p.wide; said[11] = p.span_tiles; said[12] = p.splits; said[13] = p.clustered;
         if (p.splits > 1 && !p.clustered) said[2] = (long long)n_seg * K * p.row_blocks * p.splits * a4_rows(f32, p.wide) * (hs + 2);
     }
     return XR_OK;
@@ -981,7 +1016,7 @@ XR_EXPORT int xr_kv4_attention(const void* q, void* out, int dtype, const void* 
     if (n_seg < 1 || n_seg > 65535 || H < 1 || K < 1 || H % K != 0 || max_pages < 1 || window < 0 || keep_first < 0 || !(scale > 0.f) || !(softcap >= 0.f) ||
         (bias != nullptr && (bias_len < 1 || softcap > 0.f)) || most_rows < 1 || q_stride < (long long)H * D || (dtype != XR_F32 && dtype != XR_BF16) ||
         !kv4_cache_ok(cache, n_pages, layers, layer, K, block, page_size, D) || (long long)max_pages * page_size > 0x7fffffffLL - 64 || row_blocks < 1 ||
-        span_tiles < 1 || splits < 1 || splits > A4_MAX_SPLITS || (clustered && splits > A4_CLUSTER) || (long long)K * row_blocks > 65535)
+        span_tiles < 1 || splits < 1 || splits > A4_MAX_SPLITS || (clustered && splits > A4_CLUSTER) || (long long)splits * row_blocks > 0x7fffffffLL || (long long)K * row_blocks > 0x7fffffffLL)
         return XR_ERR_ARG;
     const int G = H / K, f32 = dtype == XR_F32, hs = kv4_held(D), keep = window > 0 ? keep_first : 0;
     const bool spans = splits > 1 && !clustered;

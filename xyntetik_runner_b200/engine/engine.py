@@ -293,7 +293,7 @@ class Engine:
         else:
             ids = table[0, :-(-n // P)].long()
             pages = self.kv[lay.group][ids.clamp(min=0), lay.layer_in_group] * (ids >= 0).view(-1, 1, 1, 1, 1)
-        rows = pages.permute(1, 0, 3, 2, 4).reshape(2, -1, g.kv_heads, g.head_dim)
+        rows = pages.permute(1, 0, 3, 2, 4).reshape(2, pages.shape[0] * P, g.kv_heads, g.head_dim)
         return rows[0, :n], rows[1, :n]
 
     def _open(self, request) -> int:

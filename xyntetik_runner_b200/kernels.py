@@ -878,19 +878,22 @@ def kv4_read(cache: torch.Tensor, layer: int, page_size: int, block_tables: torc
     _count()
 
 
-KV4_SHORT_ROWS = 64        # packed rows (tokens x query heads per kv head) up to which a portion attends to the codes themselves
+# Packed rows (tokens x query heads per kv head) up to which a portion always attends to the codes themselves; beyond, what the step's portions cost either
+# way decides (csrc/attention_kv4.cu: a4_by_codes).
+KV4_SHORT_ROWS = 64
 _KV4_ALL_ROWS = 1 << 30
 
 
 # what xr_kv4_plan says of a step's portions, in this order
-_PLAN = ("short", "long", "floats", "pages", "longest", "tiles_128", "tiles_64", "end", "row_blocks", "wide", "span_tiles", "splits", "clustered")
+_PLAN = ("short", "long", "floats", "pages", "longest", "tiles_128", "tiles_64", "end", "most", "row_blocks", "wide", "span_tiles", "splits", "clustered")
 
 
 def kv4_plan(lengths: tuple, n: int, kv_heads: int, group: int, head_dim: int, page_size: int, code: int, window: int, keep_first: int, most_rows: int,
              max_kv_len: int = 0):
-    """What the portions `lengths` = (tokens, first positions) ask for, on the host: how many are short (at most `most_rows` packed rows) and how many longer;
-    floats of scratch for the short ones; of the longer ones the pages that their rows are read back into, the tokens of the longest, their row
-    tiles of 128 and 64 rows, and the end of the furthest; then how the short ones are cut, as the launcher takes it.  Raises where they do not fit `n` tokens."""
+    """What the portions `lengths` = (tokens, first positions) ask for, on the host: how many attend to the codes and how many (of those of more than `most_rows`
+    packed rows) go through the prompt kernels; floats of scratch for the first; of the others the pages that their rows are read back into, the
+    tokens of the longest, their row tiles of 128 and 64 rows, and the end of the furthest; the most rows of one that attends to the codes; then how those are
+    cut, as the launcher takes it.  Raises where they do not fit `n` tokens."""
     h_len, h_pos = lengths
     if h_len.dtype.char != "i" or h_pos.dtype.char != "i" or h_len.ndim != 1 or h_len.shape != h_pos.shape:
         raise KernelError("lengths: two int32 numpy arrays, one value a portion")
@@ -907,9 +910,9 @@ def attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, layer
     """Causal attention of every token of the step over its request's rows of a cache in four bits, its own row included.  q [n, >= heads *
     head_dim] (bfloat16 or float32, strided by rows), out [n, heads * head_dim]; portion s is the seg_len[s] rows from seg_start[s] on, at positions
     seg_pos0[s] .., over row s of the block tables.  `lengths` = (seg_len, seg_pos0) on the host (numpy int32): they size the launches; a call
-    that is captured in a graph may be replayed with other positions (say in `max_kv_len` how long the requests may get, so that the cut suits
-    them) but the same seg_len.  Rows on a page that is not held count as zeros.  Options: see ``attention_simt``.
-    Single tokens, short portions and whatever the prompt kernels do not take attend to the codes; portions of more than KV4_SHORT_ROWS packed rows read the
+    that is captured in a graph may be replayed with other positions but the same seg_len (say in `max_kv_len` how long the requests may get: the
+    cut suits that, and scratch for rows read back holds that much; 0: as much as the block tables name).  Rows on a page that is not held count as zeros.  Options: see ``attention_simt``.
+    Single tokens, short portions and whatever the prompt kernels do not take attend to the codes; where longer portions are many rows, they read the
     rows they see back into `buf` (``buf(name, shape, dtype)`` gives scratch; None: allocated) and go through the prompt kernels.  `early`: the caller says that
     nothing still running writes the portions, the block tables or rows ahead of a portion's first (an engine's step); they may then be read before
     the kernel ahead in the stream is complete."""
@@ -939,14 +942,21 @@ def attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, layer
         raise KernelError("lengths: two int32 numpy arrays, one value a portion")
     # portions that the prompt kernels take: bfloat16 on 16-byte borders, head sizes that one of them has
     aligned = code == BF16 and q_row % 8 == 0 and q.data_ptr() % 16 == 0 and head_dim % 16 == 0 and head_dim <= 128 and out.data_ptr() % 16 == 0
-    most = KV4_SHORT_ROWS if aligned else _KV4_ALL_ROWS
-    short, long, floats, pages, longest, tiles_128, tiles_64, end, *cut = kv4_plan(lengths, n, K, G, head_dim, page_size, code, window, keep_first, most, max_kv_len)
+    if max_kv_len < 0:
+        raise KernelError("max_kv_len is not negative")
+    most = max(KV4_SHORT_ROWS, G) if aligned else _KV4_ALL_ROWS          # (single tokens never)
+    short, long, floats, pages, longest, tiles_128, tiles_64, end, most, *cut = kv4_plan(lengths, n, K, G, head_dim, page_size, code, window, keep_first, most, max_kv_len)
+    if long and max_kv_len == 0 and torch.cuda.is_current_stream_capturing():
+        reach = min(max_pages * page_size, 2 ** 31 - 1)
+        short, long, floats, pages, longest, tiles_128, tiles_64, end, most, *cut = kv4_plan(lengths, n, K, G, head_dim, page_size, code, window, keep_first, most, reach)
     if long:
         def scratch(name, shape, dt):
             return torch.empty(shape, dtype=dt, device=out.device) if buf is None else buf(name, shape, dt)
         ints = scratch("kv4_portions", (3 * n_seg + n_seg * max_pages,), _I32)
         first, last, long_len, tables = ints[:n_seg], ints[n_seg:2 * n_seg], ints[2 * n_seg:3 * n_seg], ints[3 * n_seg:].view(n_seg, max_pages)
-        values = scratch("kv4_values", (pages, 2, K, page_size, head_dim), torch.bfloat16)
+        # (rounded up, so that an engine's buffer is made anew a few times and not with every longer prompt)
+        room = pages if buf is None else 1 << (pages - 1).bit_length()
+        values = scratch("kv4_values", (room, 2, K, page_size, head_dim), torch.bfloat16)
         _check(_c.xr_kv4_long(at_len, at_pos, first.data_ptr(), last.data_ptr(), long_len.data_ptr(), tables.data_ptr(), n_seg, max_pages, G, window, most,
                               _stream()), "attention_kv4")
         _check(_c.xr_kv4_read(*args, block_tables.data_ptr(), first.data_ptr(), last.data_ptr(), values.data_ptr(), BF16, tables.data_ptr(), n_seg, max_pages,
@@ -963,7 +973,7 @@ def attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, layer
     if short:
         spans = None
         if floats:
-            spans = torch.empty(floats, dtype=torch.float32, device=out.device) if buf is None else buf("kv4_spans", (floats,), torch.float32)
+            spans = torch.empty(floats, dtype=torch.float32, device=out.device) if buf is None else buf("kv4_spans", (1 << (floats - 1).bit_length(),), torch.float32)
         _check(_c.xr_kv4_attention(q.data_ptr(), out.data_ptr(), code, *args, at_start, at_len, at_pos, block_tables.data_ptr(), _ptr(spans),
                                    floats, q_row, n_seg, heads, head_dim, max_pages, window, scale, _ptr(sink),
                                    softcap, keep_first, _ptr(bias), _bias_len(bias), most, int(early), *cut, _stream()), "attention_kv4")
