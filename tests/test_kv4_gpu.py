@@ -258,6 +258,28 @@ def test_attention(contexts, T, H, K, D, P, dtype, window, keep, sink, cap, bias
         assert torch.all(out[q.shape[0]:] == 9.0)
 
 
+@pytest.mark.parametrize("contexts,T,H,K,D,P", [([415, 300], 1, 8, 4, 256, 8), ([20000, 9000], 2, 8, 4, 16, 24), ([4000], 5, 6, 2, 128, 64)])
+def test_float32_is_as_exact_as_float32(contexts, T, H, K, D, P):
+    """Off by no more than twice what the formula in float32 with sums that are rounded to nearest is: both round every product's sum and every weight
+    once, the kernel's further roundings (of three pieces, of the spans' sums) are as many at most."""
+    from xyntetik_runner_b200 import kernels
+    args, q, held, plain, Ts, starts, pos0 = attention_case(contexts, T, H, K, D, P, F32, 0, 0, 0, 0, 0)
+    out = torch.empty(q.shape[0], H * D, device=DEV)
+    kernels.attention_kv4(q.to(DEV), out, **args)
+    mine = theirs = 0.0
+    for r, n in enumerate(Ts):
+        s, k, v = starts[r], held[2 * r], held[2 * r + 1]
+        x = q[s:s + n].reshape(n, H, D)
+        o = plain_kv4.attention(x.double(), k, v, int(pos0[r]), **plain)[0]
+        kk, vv = (y.float().repeat_interleave(H // K, 1) for y in (k, v))
+        score = torch.einsum("nhd,khd->hnk", x, kk) * D ** -0.5
+        score.masked_fill_(torch.arange(k.shape[0])[None, None, :] > int(pos0[r]) + torch.arange(n)[None, :, None], -math.inf)
+        f = torch.einsum("hnk,khd->nhd", torch.softmax(score, -1), vv)
+        mine += float((out[s:s + n].double().cpu().reshape(n, H, D) - o).square().sum())
+        theirs += float((f.double() - o).square().sum())
+    assert mine <= 4.0 * theirs, f"{math.sqrt(mine / theirs):.3g} times as far"
+
+
 def run_case(case, **change):
     from xyntetik_runner_b200 import kernels
     args, q, held, plain, Ts, starts, pos0 = attention_case(*case)
