@@ -114,7 +114,7 @@ def test_what_portions_ask_for():
     for l, p, n in ((a(-1), a(0), 9), (a(1), a(-1), 9), (a(5, 5), a(0, 0), 9), (a(8), a(2 ** 31 - 8), 9)):
         with pytest.raises(kernels.KernelError, match="does not hold"):
             plan(l, p, n=n)
-    for l, p in ((a(1), a(1, 2)), (a(1).astype(np.int64), a(1))):
+    for l, p in ((a(1), a(1, 2)), (a(1).astype(np.int64), a(1)), (a(1).astype(">i4"), a(1)), (a(1), a(1).astype(np.float32))):
         with pytest.raises(kernels.KernelError, match="one value a portion"):
             plan(l, p)
     with pytest.raises((BufferError, ValueError), match="contiguous"):

@@ -301,6 +301,53 @@ def test_requests_that_are_cut(case):
     check(out, q, held, plain, Ts, starts, pos0, case[2], case[4], case[6])
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("lowest", [-math.inf, torch.finfo(torch.float32).min])
+@pytest.mark.parametrize("near", [0, 7])
+def test_a_bias_that_hides_keys(dtype, lowest, near):
+    """Distances of `near` and more have the lowest bias there is: such keys have no weight beside others; where all keys have it (near 0) and it is a number,
+    scores are lost beside it and the row is the keys' average; the softmax of nothing but minus infinity is no number."""
+    from xyntetik_runner_b200 import kernels
+    H, K, D, P, n, T = 4, 2, 64, 16, 100, 3
+    args, q, held, plain, Ts, starts, pos0 = attention_case([n], T, H, K, D, P, dtype, 0, 0, 0, 0, 20)
+    table = plain["bias"].float()
+    table[:, near:] = lowest
+    args["bias"] = table.to(DEV)
+    out = torch.full((T, H * D), 9.0, dtype=dtype, device=DEV)
+    kernels.attention_kv4(q.to(DEV), out, **args)
+    if near == 0:
+        # equal weights; sums of 100 values in float32, the output's rounding
+        tol = (2.0 ** -7 if dtype is BF16 else 2.0 ** -18) * float(held[1].abs().max())
+        for i in range(T):
+            want = held[1][:n - T + 1 + i].mean(0).repeat_interleave(H // K, 0)
+            got = out[i].double().cpu().reshape(H, D)
+            assert torch.isnan(got).all() if lowest == -math.inf else torch.all((got - want).abs() <= tol)
+        return
+    # (what is seen is a window of seven)
+    check(out, q, held, {**plain, "window": near, "bias": table.clamp(min=-100.0).double()}, Ts, starts, pos0, H, D, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("cap,bias", [(0, 0), (20.0, 0), (0, 30)])
+def test_queries_that_are_no_numbers(dtype, bad, cap, bias):
+    """One element of one head's query: that head of that token is no number (some key is zero there), all others are as ever."""
+    from xyntetik_runner_b200 import kernels
+    H, K, D, P, T = 6, 2, 64, 16, 3
+    args, q, held, plain, Ts, starts, pos0 = attention_case([90], T, H, K, D, P, dtype, 0, 0, 0, cap, bias)
+    assert (held[0][:88, 1, 9] == 0).any()
+    q[1, 4 * D + 9] = bad
+    out = torch.full((T, H * D), 9.0, dtype=dtype, device=DEV)
+    kernels.attention_kv4(q.to(DEV), out, **args)
+    got = out.double().cpu().reshape(T, H, D)
+    assert torch.isnan(got[1, 4]).all()
+    q[1, 4 * D + 9] = 0.0
+    o, size, raw = plain_kv4.attention(q.double().reshape(T, H, D), held[0], held[1], int(pos0[0]), **plain)
+    near = (got - o).abs() <= plain_kv4.tolerance(o, size, raw, D, dtype)
+    near[1, 4] = True
+    assert near.all()
+
+
 def test_empty_portions():
     """Portions of no tokens beside others, and a call without any token."""
     from xyntetik_runner_b200 import kernels

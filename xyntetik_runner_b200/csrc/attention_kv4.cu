@@ -227,7 +227,10 @@ k_kv4_attention(A4Args a) {
     extern __shared__ __align__(128) uint8_t smem[];
     uint2* q_sm = (uint2*)(smem + A4_WARPS * STAGES * STAGE);                        // [P][NT][KS][32]
     const int seg = blockIdx.z, kvh = blockIdx.y, rb = blockIdx.x / a.splits, span = blockIdx.x - rb * a.splits;
-    // (a.early: portions, block tables and the rows of earlier steps are at rest, so that tiles of such rows set out before the kernel ahead is complete)
+    // (a.early: portions, block tables and the rows of earlier steps are at rest, so that tiles of such rows set out before the kernel ahead is complete.  It
+    // takes more than that kernel's wait to say so, for kernels here let the next one start before they wait themselves: an engine's step begins with
+    // the copy of its description, which waits for all of the last step, and stores no rows but its own.  Blocks without work leave without a wait;
+    // a launch has one that waits, or it is not made.)
     if (!a.early) xr_pdl_wait();
     const int L = a.seg_len[seg];
     const long long rows_all = (long long)L * a.G;
@@ -402,7 +405,7 @@ k_kv4_attention(A4Args a) {
     constexpr float LIFT = F32 ? 0.f : 5.f;
     float unit[NT][2];                                               // what turns a column's scores into exponents of two
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) { unit[nt][0] = EXTRA ? sl : sl * q_unit[nt][0]; unit[nt][1] = EXTRA ? sl : sl * q_unit[nt][1]; }
+    for (int nt = 0; nt < NT; nt++) { unit[nt][0] = EXTRA ? 1.f : sl * q_unit[nt][0]; unit[nt][1] = EXTRA ? 1.f : sl * q_unit[nt][1]; }
     float o[NT][MT][4], m[NT][2], l[NT][2];
     float v_unit = 1.f, v_inv = 1.f, v_most = F32 ? INFINITY : 0.f;  // the sums' unit, its inverse, the largest scale in it
 #pragma unroll
@@ -511,14 +514,14 @@ k_kv4_attention(A4Args a) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         float& x = s[sub][nt][e];
-                        if (!F32) x *= q_unit[nt][e & 1];
+                        // (exponents of two, so that `unit` is one: scores that are equal and huge, a bias of the lowest number for one, differ by exactly zero)
                         if (a.softcap > 0.f) {
-                            // c tanh(x scale / c) / scale, through one exponential: tanh(y) = 1 - 2 / (exp(2 y) + 1)
-                            const float cap = a.softcap / a.scale, ex = __expf(2.0f * x * (a.scale / a.softcap));
-                            x = F32 ? cap * tanhf(x * (a.scale / a.softcap)) : cap * (1.0f - __fdividef(2.0f, ex + 1.0f));
+                            // c tanh(x scale / c), through one exponential: tanh(y) = 1 - 2 / (exp(2 y) + 1)
+                            const float cap = a.softcap * A4_LOG2E, y = x * q_unit[nt][e & 1] * (a.scale / a.softcap);
+                            x = F32 ? cap * tanhf(y) : cap * (1.0f - __fdividef(2.0f, __expf(2.0f * y) + 1.0f));
                         } else {
                             const int row = row0 + min(nt * 8 + 2 * t + (e & 1), rows - 1);
-                            x += xr_bias_at(a.bias.table + (size_t)(kvh * a.G + row % a.G) * a.bias.len, a.bias.len, pos_r[nt][e & 1] - (k0 + sub * 16 + key_a + 4 * (e & 2)));
+                            x = (x * q_unit[nt][e & 1] + xr_bias_at(a.bias.table + (size_t)(kvh * a.G + row % a.G) * a.bias.len, a.bias.len, pos_r[nt][e & 1] - (k0 + sub * 16 + key_a + 4 * (e & 2)))) * sl;
                         }
                     }
         }

@@ -882,6 +882,7 @@ def kv4_read(cache: torch.Tensor, layer: int, page_size: int, block_tables: torc
 # way decides (csrc/attention_kv4.cu: a4_by_codes).
 KV4_SHORT_ROWS = 64
 _KV4_ALL_ROWS = 1 << 30
+_NP_I32 = np.dtype(np.int32)
 
 
 # what xr_kv4_plan says of a step's portions, in this order
@@ -895,7 +896,7 @@ def kv4_plan(lengths: tuple, n: int, kv_heads: int, group: int, head_dim: int, p
     tokens of the longest, their row tiles of 128 and 64 rows, and the end of the furthest; the most rows of one that attends to the codes; then how those are
     cut, as the launcher takes it.  Raises where they do not fit `n` tokens."""
     h_len, h_pos = lengths
-    if h_len.dtype.char != "i" or h_pos.dtype.char != "i" or h_len.ndim != 1 or h_len.shape != h_pos.shape:
+    if h_len.dtype != _NP_I32 or h_pos.dtype != _NP_I32 or h_len.ndim != 1 or h_len.shape != h_pos.shape:
         raise KernelError("lengths: two int32 numpy arrays, one value a portion")
     said = array("q", (0,) * len(_PLAN))
     if _c.xr_kv4_plan(h_len, h_pos, h_len.size, n, kv_heads, group, head_dim, page_size, code, window, keep_first, most_rows, max_kv_len, said) != 0:
