@@ -968,7 +968,7 @@ static int a4_launch(const A4Args& a, int n_seg, int f32, int wide, cudaStream_t
 // full tiles, 256 blocks: 20.5 / 21.8 (2 requests, 1,000 keys), 100.7 / 101.0 (2, 8,192), 101.0 / 116.3 (4, 8,192); 320: 33.5 / 22.5, 144.4 / 94.3 (1 request);
 // part full, 384 blocks: 35.3 / 33.3 (4, 1,000), 160.2 / 207.9 (4, 8,192), 36.5 / 35.9 (8, 1,000); 400: 37.5 / 31.4 (2, 1,000), 37.9 / 29.7 (1, 1,000), but
 // 163.8 / 183.2 (1, 8,192).  Of 64 elements a block is cheaper: full tiles, 320: 84.4 / 90.6 (1, 8,192), 22.2 / 20.8 (1, 1,000), 384: 92.5 / 90.5, 23.6 / 20.8; part
-// full, 448: 62.5 / 97.8, 640: 91.1 / 98.3 (4, 4,096).  Near the borders the wrong side is at most a sixth slower.  The rule asks nothing of positions, so
+// full, 448: 62.5 / 97.8, 640: 91.1 / 98.3 (4, 4,096).  Near the borders the wrong side is at most 1.18 times slower.  The rule asks nothing of positions, so
 // that a replayed graph may have others.
 static bool a4_by_codes(long long row_blocks, bool full, int hs) { return row_blocks <= (hs == 64 ? (full ? 320 : 576) : (full ? 256 : 384)); }
 
