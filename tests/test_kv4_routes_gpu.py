@@ -1,0 +1,54 @@
+"""The cache in four bits where calls follow one another, share scratch, or leave the common sizes; against the plain form in 64 bits (plain_kv4.py)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import plain_kv4
+from test_kv4_gpu import BF16, DEV, F32, attention_case, check, i32
+
+pytestmark = pytest.mark.gpu
+
+
+def shared():
+    """Scratch as an engine keeps it: one buffer a name and type, made anew when it is too small."""
+    held = {}
+
+    def buf(name, shape, dtype):
+        n = math.prod(shape)
+        if (name, dtype) not in held or held[name, dtype].numel() < n:
+            held[name, dtype] = torch.empty(n, dtype=dtype, device=DEV)
+        return held[name, dtype][:n].view(*shape)
+    return buf
+
+
+@pytest.mark.parametrize("H,K,D,P,kernel", [(64, 8, 128, 64, "attention_tc"), (66, 33, 48, 24, "attention_mma")])
+def test_prompt_portions_one_call_after_the_other(H, K, D, P, kernel, monkeypatch):
+    """Calls with other lengths every time through one scratch, all queued behind a long call: each finds the lengths of its own portions, not those that the
+    call ahead of it left in the scratch."""
+    from xyntetik_runner_b200 import kernels
+    used = []
+    real = getattr(kernels, kernel)
+    monkeypatch.setattr(kernels, kernel, lambda *a, **k: (used.append(1), real(*a, **k)))
+    contexts = [400, 300, 500]
+    first = attention_case(contexts, [100, 1, 150], H, K, D, P, BF16, 0, 0, 0, 0, 0)
+    buf, calls = shared(), []
+    for Ts in ([100, 1, 150], [1, 130, 60], [150, 90, 0], [40, 110, 100], [1, 1, 248], [248, 1, 1]):
+        # the same requests and rows, other portions of them
+        pos0 = np.array(contexts) - np.array(Ts)
+        starts = np.concatenate([[0], np.cumsum(Ts)[:-1]])
+        args = {**first[0], "seg_start": i32(starts), "seg_len": i32(Ts), "seg_pos0": i32(pos0), "lengths": (np.array(Ts, dtype=np.int32), pos0.astype(np.int32))}
+        q = torch.randn(sum(Ts), H * D, generator=torch.Generator().manual_seed(Ts[0])).to(BF16)
+        calls.append((args, q, q.to(DEV), torch.full((sum(Ts) + 9, H * D), 9.0, dtype=BF16, device=DEV), Ts, starts, pos0))
+    long = attention_case([6000] * 4, 4, 32, 8, 128, 64, BF16, 0, 0, 0, 0, 0, seed=2)
+    far, long_q = torch.empty(16, 32 * 128, dtype=BF16, device=DEV), long[1].to(DEV)
+    torch.cuda.synchronize()
+    for args, q, qd, out, *_ in calls:
+        kernels.attention_kv4(long_q, far, **long[0])
+        kernels.attention_kv4(qd, out[:-9], **args, buf=buf)
+    kernels.tc_check_status(torch.device(DEV))
+    assert len(used) == len(calls)
+    for args, q, qd, out, Ts, starts, pos0 in calls:
+        check(out[:-9], q, first[2], first[3], Ts, starts, pos0, H, D, BF16)
+        assert torch.all(out[-9:] == 9.0)

@@ -354,7 +354,9 @@ k_attention_rows(AttnMmaArgs a, int n_seg) {
     __nv_bfloat16* kbuf = qs + ATT_ROWS * LD;                      // [2][64][LD]
     __nv_bfloat16* vbuf = kbuf + 2 * ATT_TILE * LD;                // [2][64][LD]
     // The row tiles of the portions with more than 16 packed rows, laid end to end, are the grid's x (short portions
-    // belong to the keys kernel and have no blocks here); a block finds its (portion, tile) by walking the lengths.
+    // belong to the keys kernel and have no blocks here); a block finds its (portion, tile) by walking the lengths, ahead of the
+    // wait: whatever wrote them is complete before the kernel ahead of this one lets this one start (the copy of a step's description,
+    // or k_kv4_long, which k_kv4_read waits for first).
     const int kvh = blockIdx.y;
     int seg = -1, tile = 0;
     {

@@ -226,6 +226,8 @@ k_attention_tc(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
     const int kvh = blockIdx.y;
     int seg = -1, tile = 0;
     int flat_row0 = 0;                                              // FLAT: the row of the portion's key 0 (it may lie before the array)
+    // (The lengths are read ahead of the wait: whatever wrote them is complete before the kernel ahead of this one lets this one start -- the copy of a
+    // step's description, or k_kv4_long, which k_kv4_read waits for first.)
     {
         const int want = (int)gridDim.x - 1 - (int)blockIdx.x;
         int before = 0;

@@ -189,9 +189,11 @@ __device__ __forceinline__ void kv4_eight(uint32_t word, uint32_t s, T* to) {
 template <typename T, int WS>
 __global__ void __launch_bounds__(256)
 k_kv4_read(Kv4ReadArgs a) {
-    xr_pdl_launch();
     __shared__ int found[2];
     xr_pdl_wait();
+    // Behind the wait, not ahead of it: the prompt kernels walk the portions' lengths before they wait themselves, and on the route of attention_kv4
+    // those lengths are k_kv4_long's.  Nothing behind this kernel starts before that one is complete.
+    xr_pdl_launch();
     const int j = blockIdx.x;
     if (threadIdx.x < 32) {
         int before = 0;
