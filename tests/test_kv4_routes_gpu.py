@@ -52,3 +52,22 @@ def test_prompt_portions_one_call_after_the_other(H, K, D, P, kernel, monkeypatc
     for args, q, qd, out, Ts, starts, pos0 in calls:
         check(out[:-9], q, first[2], first[3], Ts, starts, pos0, H, D, BF16)
         assert torch.all(out[-9:] == 9.0)
+
+
+@pytest.mark.parametrize("case,cut", [
+    (([640], 1, 1, 1, 64, 64, BF16, 0, 0, 0, 0, 0), "cluster"), (([640, 500, 77], 1, 3, 3, 64, 16, F32, 0, 0, 1, 0, 0), "cluster"),
+    (([1000] * 5, 1, 24, 8, 128, 64, BF16, 300, 9, 1, 0, 60), "cluster"), (([1200, 900], 3, 8, 2, 256, 64, BF16, 0, 0, 0, 20.0, 0), "cluster"),
+    (([700, 90], 2, 6, 2, 100, 24, F32, 0, 0, 0, 30.0, 0), "cluster"), (([9000, 300], 1, 2, 1, 64, 64, BF16, 0, 0, 0, 0, 0), "spans")])
+def test_spans_that_meet(case, cut):
+    """Rows of half a warp's quadruples, and counts that part a warp, ahead of the cluster's barriers: right, and the same bits every time."""
+    from xyntetik_runner_b200 import kernels
+    args, q, held, plain, Ts, starts, pos0 = attention_case(*case)
+    H, K, D, P, dtype = case[2:7]
+    said = dict(zip(kernels._PLAN, kernels.kv4_plan(args["lengths"], q.shape[0], K, H // K, D, P, kernels.dtype_code(dtype), case[7], case[8], 1 << 30)))
+    assert said["splits"] > 1 and bool(said["clustered"]) == (cut == "cluster")
+    qd = q.to(DEV)
+    outs = [torch.full((q.shape[0], H * D), 9.0, dtype=dtype, device=DEV) for _ in range(40)]
+    for out in outs:
+        kernels.attention_kv4(qd, out, **args)
+    check(outs[0], q, held, plain, Ts, starts, pos0, H, D, dtype)
+    assert all(torch.equal(out, outs[0]) for out in outs)

@@ -109,7 +109,9 @@ __device__ __forceinline__ float2 a4_far2(uint32_t at) {
     asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
     return v;
 }
+// (The barrier is defined for warps whose lanes run it together, and loops of other lengths a lane lie ahead of it.)
 __device__ __forceinline__ void a4_cluster_sync() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -610,6 +612,7 @@ k_kv4_attention(A4Args a) {
                         }
                 }
             }
+            __syncwarp();                                             // (lanes parted in there, and the matrix instructions want them together)
         }
         // bfloat16 queries: values are multiplied in float16, in units of v_unit, a power of two: scales within 2^-20 .. 248 units make values that are exact.  The
         // unit is chosen by the first tile with values that are not zero (2^6 times its largest scale), and again where a scale outgrows it.
