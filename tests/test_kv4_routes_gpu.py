@@ -56,7 +56,7 @@ def test_prompt_portions_one_call_after_the_other(H, K, D, P, kernel, monkeypatc
 
 @pytest.mark.parametrize("case,cut", [
     (([640], 1, 1, 1, 64, 64, BF16, 0, 0, 0, 0, 0), "cluster"), (([640, 500, 77], 1, 3, 3, 64, 16, F32, 0, 0, 1, 0, 0), "cluster"),
-    (([1000] * 5, 1, 24, 8, 128, 64, BF16, 300, 9, 1, 0, 60), "cluster"), (([1200, 900], 3, 8, 2, 256, 64, BF16, 0, 0, 0, 20.0, 0), "cluster"),
+    (([1000] * 5, 1, 24, 8, 128, 64, BF16, 300, 9, 1, 0, 60), "cluster"), (([1200, 900], 3, 8, 2, 256, 64, BF16, 0, 0, 0, 20.0, 0), "spans"),
     (([700, 90], 2, 6, 2, 100, 24, F32, 0, 0, 0, 30.0, 0), "cluster"), (([9000, 300], 1, 2, 1, 64, 64, BF16, 0, 0, 0, 0, 0), "spans")])
 def test_spans_that_meet(case, cut):
     """Rows of half a warp's quadruples, and counts that part a warp, ahead of the cluster's barriers: right, and the same bits every time."""
@@ -71,3 +71,25 @@ def test_spans_that_meet(case, cut):
         kernels.attention_kv4(qd, out, **args)
     check(outs[0], q, held, plain, Ts, starts, pos0, H, D, dtype)
     assert all(torch.equal(out, outs[0]) for out in outs)
+
+
+@pytest.mark.parametrize("case,kernel", [(([100], 80, 117, 39, 48, 24, BF16, 0, 0, 0, 0, 0), "attention_mma"), (([120, 90], 40, 117, 39, 80, 24, BF16, 50, 9, 0, 0, 0), "attention_mma"),
+                                         (([200], 64, 82, 41, 64, 64, BF16, 0, 0, 0, 0, 0), "attention_tc"), (([100, 80], 3, 4, 2, 64, 24, F32, 0, 0, 0, 0, 0), None)])
+def test_positions_beyond_the_tables(case, kernel, monkeypatch):
+    """Block tables that name fewer rows than a request has: the others count as zeros, whichever way the portion goes."""
+    from xyntetik_runner_b200 import kernels
+    used = []
+    if kernel:
+        real = getattr(kernels, kernel)
+        monkeypatch.setattr(kernels, kernel, lambda *a, **k: (used.append(1), real(*a, **k)))
+    args, q, held, plain, Ts, starts, pos0 = attention_case(*case)
+    H, D, P, dtype = case[2], case[4], case[5], case[6]
+    pages = min(case[0]) // P - 1                                     # (the last request's neighbour in the array would be the next row's first pages)
+    args["block_tables"] = args["block_tables"][:, :pages].contiguous()
+    for x in held:
+        x[pages * P:] = 0.0
+    out = torch.full((q.shape[0], H * D), 9.0, dtype=dtype, device=DEV)
+    kernels.attention_kv4(q.to(DEV), out, **args)
+    kernels.tc_check_status(torch.device(DEV))
+    assert bool(used) == bool(kernel)
+    check(out, q, held, plain, Ts, starts, pos0, H, D, dtype)

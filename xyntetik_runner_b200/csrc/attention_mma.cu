@@ -155,7 +155,7 @@ __device__ __forceinline__ void load_kv_tile(__nv_bfloat16* kdst, __nv_bfloat16*
             int pi;
             if (a.page_shift >= 0) { pi = kp >> a.page_shift; off = kp & (a.page_size - 1); }
             else { pi = kp / a.page_size; off = kp - pi * a.page_size; }
-            page = bt[pi];
+            page = pi < a.max_pages ? bt[pi] : -1;
         }
         __nv_bfloat16* kd = kdst + r * LD;
         __nv_bfloat16* vd = vdst + r * LD;
