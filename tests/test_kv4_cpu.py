@@ -165,3 +165,25 @@ def test_bytes_of_a_token():
 def test_option():
     from xyntetik_runner_b200 import cli
     assert cli.build_parser().parse_args(["-m", "x"]).kv == "same" and cli.build_parser().parse_args(["-m", "x", "--kv", "int4"]).kv == "int4"
+
+
+def test_plans_of_the_longest_windows_and_kept_rows():
+    """Up to the largest 32-bit number: as if there were no window."""
+    l, p = np.array([1, 3, 70], dtype=np.int32), np.array([5000, 40, 900], dtype=np.int32)
+    for most in (64, 1 << 30):
+        plain = kernels.kv4_plan((l, p), 100, 900, 4, 64, 16, kernels.BF16, 0, 0, most)
+        for window, keep in ((40, 2 ** 31 - 1), (2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1)):
+            assert kernels.kv4_plan((l, p), 100, 900, 4, 64, 16, kernels.BF16, window, keep, most) == plain
+            kernels.kv4_plan((l, p), 100, 900, 4, 64, 16, kernels.BF16, window, keep, most, 2 ** 31 - 1)
+
+
+@pytest.mark.parametrize("name", ["window", "keep_first", "max_kv_len"])
+def test_numbers_that_have_more_than_31_bits(name):
+    p, i = _parts(), torch.zeros(2, dtype=torch.int32)
+    two = np.array([2, 2], dtype=np.int32)
+    for much in (2 ** 31, 2 ** 32 + 5):
+        with pytest.raises(kernels.KernelError, match="31 bits"):
+            kernels.attention_kv4(torch.zeros(4, 256), torch.zeros(4, 256), p["cache"], 0, 16, i, i, i, p["block_tables"], 4, 64, 0.1, (two, two), **{name: much})
+    if name == "keep_first":
+        with pytest.raises(kernels.KernelError, match="keep_first"):
+            kernels.kv4_read(p["cache"], 0, 16, p["block_tables"], i, i, torch.zeros(2, 2, 2, 16, 64), keep_first=2 ** 31)

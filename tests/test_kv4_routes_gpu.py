@@ -93,3 +93,31 @@ def test_positions_beyond_the_tables(case, kernel, monkeypatch):
     kernels.tc_check_status(torch.device(DEV))
     assert bool(used) == bool(kernel)
     check(out, q, held, plain, Ts, starts, pos0, H, D, dtype)
+
+
+@pytest.mark.parametrize("case", [([200, 90], 1, 4, 2, 64, 16, BF16, 40, 0, 0, 0, 0), ([200], 3, 4, 2, 64, 16, F32, 40, 0, 0, 0, 0),
+                                  ([150], 70, 64, 16, 64, 16, BF16, 40, 0, 0, 0, 0), ([150], 70, 66, 33, 48, 24, BF16, 40, 0, 0, 0, 0)])
+@pytest.mark.parametrize("window,keep", [(40, 2 ** 31 - 1), (2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1)])
+def test_the_longest_windows_and_kept_rows(case, window, keep):
+    """Every row is seen."""
+    from xyntetik_runner_b200 import kernels
+    args, q, held, plain, Ts, starts, pos0 = attention_case(*case[:7], 0, 0, 0, 0, 0)
+    out = torch.full((q.shape[0], case[2] * case[4]), 9.0, dtype=case[6], device=DEV)
+    kernels.attention_kv4(q.to(DEV), out, **{**args, "window": window, "keep_first": keep})
+    check(out, q, held, plain, Ts, starts, pos0, case[2], case[4], case[6])
+
+
+def test_reading_from_before_the_first_row():
+    """A first row below zero reads from row 0 on; as many kept rows as there are numbers are all rows."""
+    from xyntetik_runner_b200 import kernels
+    g = torch.Generator().manual_seed(7)
+    P, K, D, n = 16, 2, 64, 60
+    k, v = (torch.randn(n, K * D, generator=g).to(BF16) for _ in (0, 1))
+    cache, bt = kernels.kv4_cache(4, 1, K, D, P, DEV), i32([[2, 0, 3, 1]])
+    kernels.kv4_store(k.to(DEV), v.to(DEV), i32(np.arange(n)), i32(np.zeros(n)), bt, cache, 0, P)
+    want = torch.stack([plain_kv4.quantised_rows(x.reshape(n, K, D)) for x in (k, v)])
+    for first, keep in ((0, 0), (-1, 0), (-2 ** 31, 0), (59, 2 ** 31 - 1), (-2 ** 31, 2 ** 31 - 1)):
+        out = torch.full((4, 2, K, P, D), 3.0, dtype=BF16, device=DEV)
+        kernels.kv4_read(cache, 0, P, bt, i32([first]), i32([n]), out, keep_first=keep)
+        got = out.double().cpu().permute(1, 0, 3, 2, 4).reshape(2, 4 * P, K, D)
+        assert torch.equal(got[:, :n], want) and not got[:, n:].any(), (first, keep)

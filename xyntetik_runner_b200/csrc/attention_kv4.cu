@@ -921,8 +921,8 @@ static A4Plan a4_plan(const int* len, const int* pos0, int n_seg, int K, int G, 
     p.span_tiles = best * A4_WARPS;
     if (max_kv > 0) {
         // (a captured launch may meet requests up to this length; beyond the grid's spans the last one takes the rest)
-        const long long range = window > 0 && window + 16 < max_kv ? window + 16 : max_kv;
-        const long long t = (range + tile - 1) / tile + 1 + (window > 0 ? (keep + tile - 1) / tile : 0);
+        const long long range = window > 0 && window + 16LL < max_kv ? window + 16LL : max_kv;
+        const long long t = (range + tile - 1) / tile + 1 + (window > 0 ? (keep + tile - 1LL) / tile : 0);
         const long long more = best * (long long)A4_WARPS * (p.clustered ? A4_CLUSTER : A4_MAX_SPLITS);
         longest = (int)(t > longest ? (t < more ? t : (more > longest ? more : longest)) : longest);
     }

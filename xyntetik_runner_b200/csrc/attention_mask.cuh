@@ -17,7 +17,7 @@ struct XrBias {
 };
 
 __host__ __device__ __forceinline__ int xr_kept_tiles(int keep_first, int lo, int tile) {
-    const int kept = (keep_first + tile - 1) / tile, first = lo / tile;
+    const int kept = (int)(((unsigned)keep_first + tile - 1) / tile), first = lo / tile;      // (any keep_first that is not negative)
     return kept < first ? kept : first;
 }
 // the tile at place i of a walk whose window begins with tile t_lo

@@ -164,7 +164,7 @@ struct Kv4ReadArgs {
 __device__ __forceinline__ void kv4_pages_of(const Kv4ReadArgs& a, int seg, int& kept, int& from, int& count) {
     const int P = a.c.page_size, f = max(0, a.first[seg]), e = (int)min((long long)a.end[seg], (long long)a.max_pages * P);
     from = f / P;
-    kept = f < e ? min((a.keep + P - 1) / P, from) : 0;
+    kept = f < e ? min((int)(((unsigned)a.keep + P - 1) / P), from) : 0;
     count = f < e ? (e - 1) / P - from + 1 : 0;
 }
 
@@ -220,7 +220,7 @@ k_kv4_read(Kv4ReadArgs a) {
     __syncthreads();
     const int seg = found[0];
     if (seg < 0) return;                                                 // (more pages of output than the requests take: left as they were)
-    const int pi = found[1], P = a.c.page_size, first = a.first[seg], end = a.end[seg];
+    const int pi = found[1], P = a.c.page_size, first = max(0, a.first[seg]), end = a.end[seg];
     int page = a.block_tables[(size_t)seg * a.max_pages + pi];
     if (page >= a.c.n_pages) page = -1;
     const int words = a.c.hs >> 3, used = (a.D + 7) >> 3, p0 = pi * P;

@@ -866,7 +866,7 @@ def kv4_read(cache: torch.Tensor, layer: int, page_size: int, block_tables: torc
     at_first, at_end = _ints(first, n_seg, "first"), _ints(end, n_seg, "end")
     if tables is not None and (tables.shape != block_tables.shape or tables.dtype != torch.int32 or not tables.is_contiguous()):
         raise KernelError("tables has the block tables' shape and type")
-    if keep_first < 0:
+    if not 0 <= keep_first < 2 ** 31:
         raise KernelError(f"keep_first {keep_first}")
     _on_current(cache, block_tables, first, end, out, tables)
     args = _kv4_args(cache, layer, page_size, D)
@@ -929,8 +929,10 @@ def attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, layer
         raise KernelError("q and out are rows of the same tokens in one type, out [tokens, heads * elements]")
     if n < 2:
         q_row = cols                       # (one row has no stride: torch may say anything)
-    if window < 0 or keep_first < 0 or not scale > 0 or not softcap >= 0 or (bias is not None and softcap > 0):
-        raise KernelError("window and keep_first are not negative, the scale is positive, a bias goes without a cap")
+    if not 0 <= window < 2 ** 31 or not 0 <= keep_first < 2 ** 31 or not scale > 0 or not softcap >= 0 or (bias is not None and softcap > 0):
+        raise KernelError("window and keep_first are not negative and have 31 bits, the scale is positive, a bias goes without a cap")
+    if not 0 <= max_kv_len < 2 ** 31:
+        raise KernelError("max_kv_len is not negative and has 31 bits")
     if sink is not None and (sink.dtype is not torch.float32 or sink.numel() != heads or not sink.is_contiguous()):
         raise KernelError("sink: one float32 logit a query head")
     if bias is not None:
@@ -943,8 +945,6 @@ def attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, layer
         raise KernelError("lengths: two int32 numpy arrays, one value a portion")
     # portions that the prompt kernels take: bfloat16 on 16-byte borders, head sizes that one of them has
     aligned = code == BF16 and q_row % 8 == 0 and q.data_ptr() % 16 == 0 and head_dim % 16 == 0 and head_dim <= 128 and out.data_ptr() % 16 == 0
-    if max_kv_len < 0:
-        raise KernelError("max_kv_len is not negative")
     most = max(KV4_SHORT_ROWS, G) if aligned else _KV4_ALL_ROWS          # (single tokens never)
     short, long, floats, pages, longest, tiles_128, tiles_64, end, most, *cut = kv4_plan(lengths, n, K, G, head_dim, page_size, code, window, keep_first, most, max_kv_len)
     if long and max_kv_len == 0 and torch.cuda.is_current_stream_capturing():
