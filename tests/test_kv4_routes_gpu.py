@@ -121,3 +121,21 @@ def test_reading_from_before_the_first_row():
         kernels.kv4_read(cache, 0, P, bt, i32([first]), i32([n]), out, keep_first=keep)
         got = out.double().cpu().permute(1, 0, 3, 2, 4).reshape(2, 4 * P, K, D)
         assert torch.equal(got[:, :n], want) and not got[:, n:].any(), (first, keep)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("scale", [0.1, 0.7, 1.0, 3.0])
+@pytest.mark.parametrize("value", [-1.0, 1.0])
+def test_a_bias_of_the_largest_size_on_every_key(dtype, scale, value):
+    """The lowest and the highest number as the bias of all keys: scores are lost beside it, whatever the scale, and the row is the keys' average."""
+    from xyntetik_runner_b200 import kernels
+    H, K, D, P, n, T = 4, 2, 64, 16, 700, 3
+    args, q, held, plain, Ts, starts, pos0 = attention_case([n], T, H, K, D, P, dtype, 0, 0, 0, 0, 20)
+    args.update(bias=torch.full((H, 20), value * torch.finfo(torch.float32).max, device=DEV), scale=scale)
+    out = torch.full((T, H * D), 9.0, dtype=dtype, device=DEV)
+    kernels.attention_kv4(q.to(DEV), out, **args)
+    # weights that are equal and exact; sums of 700 values in float32 and the output's rounding
+    tol = (2.0 ** -8 if dtype is BF16 else 2.0 ** -24 * 700) * float(held[1].abs().max())
+    for i in range(T):
+        want = held[1][:n - T + 1 + i].mean(0).repeat_interleave(H // K, 0)
+        assert torch.all((out[i].double().cpu().reshape(H, D) - want).abs() <= tol)

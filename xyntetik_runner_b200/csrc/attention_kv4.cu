@@ -523,7 +523,10 @@ k_kv4_attention(A4Args a) {
                             x = F32 ? cap * tanhf(y) : cap * (1.0f - __fdividef(2.0f, __expf(2.0f * y) + 1.0f));
                         } else {
                             const int row = row0 + min(nt * 8 + 2 * t + (e & 1), rows - 1);
-                            x = (x * q_unit[nt][e & 1] + xr_bias_at(a.bias.table + (size_t)(kvh * a.G + row % a.G) * a.bias.len, a.bias.len, pos_r[nt][e & 1] - (k0 + sub * 16 + key_a + 4 * (e & 2)))) * sl;
+                            const float y = x * q_unit[nt][e & 1] + xr_bias_at(a.bias.table + (size_t)(kvh * a.G + row % a.G) * a.bias.len, a.bias.len, pos_r[nt][e & 1] - (k0 + sub * 16 + key_a + 4 * (e & 2)));
+                            x = y * sl;
+                            // (a score that is a number stays one: a scale above ln 2 takes the largest ones out of float32)
+                            if (sl > 1.f && fabsf(x) == INFINITY && fabsf(y) < INFINITY) x = copysignf(3.402823466e38f, y);
                         }
                     }
         }
