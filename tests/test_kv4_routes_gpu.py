@@ -139,3 +139,75 @@ def test_a_bias_of_the_largest_size_on_every_key(dtype, scale, value):
     for i in range(T):
         want = held[1][:n - T + 1 + i].mean(0).repeat_interleave(H // K, 0)
         assert torch.all((out[i].double().cpu().reshape(H, D) - want).abs() <= tol)
+
+
+def sized_case(v, dtype, heads=1, T=1, requests=1):
+    """Requests with the same rows, values v [n, D], keys and queries normal: (outputs, queries, held rows of one)."""
+    from xyntetik_runner_b200 import kernels
+    g = torch.Generator().manual_seed(3)
+    n, D = v.shape
+    P = 16
+    pages = -(-n // P)
+    cache = kernels.kv4_cache(pages, 1, 1, D, P, DEV)
+    k, v = torch.randn(n, D, generator=g).to(dtype), v.to(dtype)
+    bt = i32([np.arange(pages)] * requests)
+    kernels.kv4_store(k.to(DEV), v.to(DEV), i32(np.arange(n)), i32(np.zeros(n)), bt, cache, 0, P)
+    q = torch.randn(T * requests, heads * D, generator=g).to(dtype)
+    out = torch.full((T * requests, heads * D), 9.0, dtype=dtype, device=DEV)
+    at = np.full(requests, T, dtype=np.int32), np.full(requests, n - T, dtype=np.int32)
+    said = kernels.kv4_plan(at, T * requests, 1, heads, D, P, kernels.dtype_code(dtype), 0, 0, 1 << 30)
+    assert requests == 1 or dict(zip(kernels._PLAN, said))["splits"] == 1        # (many requests: one block walks all keys of one)
+    kernels.attention_kv4(q.to(DEV), out, cache, 0, P, i32(T * np.arange(requests)), i32(at[0]), i32(at[1]), bt, heads, D, D ** -0.5, at)
+    return out, q, [plain_kv4.quantised(x)[2].reshape(n, 1, D) for x in (k, v)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("D", [64, 100, 128, 256])
+@pytest.mark.parametrize("T", [1, 9])
+def test_groups_of_other_sizes_within_a_head(dtype, D, T):
+    """A head's groups of 32 elements lie powers of two apart, 2^-40 to 2^30: every element is as exact as it would be alone."""
+    g = torch.Generator().manual_seed(D)
+    sizes = torch.tensor([0.0, -21.0, 30.0, -40.0, 8.0, -13.0, -30.0, 14.0])
+    v = torch.randn(300, D, generator=g) * torch.exp2(sizes.repeat_interleave(32)[:D])
+    out, q, held = sized_case(v, dtype, heads=2, T=T)
+    check(out, q, held, dict(scale=D ** -0.5), [T], [0], [300 - T], 2, D, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("first,then", [(-90.0, 100.0), (100.0, -90.0), (-95.0, 30.0), (0.0, -20.0), (3.0, -14.0)])
+def test_values_that_begin_small_or_large(dtype, first, then):
+    """The first 320 tokens' values are of one size, the others' of another: within what is held, however far apart."""
+    g = torch.Generator().manual_seed(1)
+    v = torch.randn(640, 64, generator=g)
+    v[:320] *= 2.0 ** first
+    v[320:] *= 2.0 ** then
+    for requests in (1, 1000):
+        out, q, held = sized_case(v, dtype, heads=3, requests=requests)
+        for r in (0, requests - 1):
+            check(out[r:r + 1], q[r:r + 1], held, dict(scale=0.125), [1], [0], [639], 3, 64, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_loud_token_that_nobody_looks_at(dtype):
+    """One token's values are 2^20 times the others', and a bias hides it: the row is what the others make, as exact as ever."""
+    from xyntetik_runner_b200 import kernels
+    H, K, D, P, n = 2, 1, 64, 16, 300
+    g = torch.Generator().manual_seed(2)
+    k, v = torch.randn(n, D, generator=g).to(dtype), torch.randn(n, D, generator=g)
+    v[n - 4] *= 2.0 ** 20
+    v = v.to(dtype)
+    cache = kernels.kv4_cache(19, 1, 1, D, P, DEV)
+    bt = i32([np.arange(19)])
+    kernels.kv4_store(k.to(DEV), v.to(DEV), i32(np.arange(n)), i32(np.zeros(n)), bt, cache, 0, P)
+    q = torch.randn(1, H * D, generator=g).to(dtype)
+    table = torch.zeros(H, 6)
+    table[:, 3] = torch.finfo(torch.float32).min
+    out = torch.empty(1, H * D, dtype=dtype, device=DEV)
+    at = np.array([1], dtype=np.int32), np.array([n - 1], dtype=np.int32)
+    kernels.attention_kv4(q.to(DEV), out, cache, 0, P, i32([0]), i32([1]), i32([n - 1]), bt, H, D, 0.125, at, bias=table.to(DEV))
+    held = [plain_kv4.quantised(x)[2].reshape(n, 1, D) for x in (k, v)]
+    held[1][n - 4] = 0.0
+    table[:, 3] = -1e4                                               # (no weight either way)
+    o, size, _ = plain_kv4.attention(q.double().reshape(1, H, D), *held, n - 1, 0.125, bias=table.double())
+    raw = plain_kv4.attention(q.double().reshape(1, H, D), *held, n - 1, 0.125)[2]
+    assert torch.all((out.double().cpu().reshape(1, H, D) - o).abs() <= plain_kv4.tolerance(o, size, raw, D, dtype))

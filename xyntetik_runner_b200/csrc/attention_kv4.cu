@@ -18,7 +18,8 @@
 // shifts and a fused product and sum a pair.)  The bias costs the sums log2(264 / 8) bits of 24; scores
 // are off by less than the weights' rounding.  q is scaled by a power of two a row, so that its eight bits are whole in float16.  Values are
 // scaled ahead of the product, where a thread's elements share a scale and its keys do not: (256 + u) s - 264 s in one rounding, which is none, because c s
-// has eight bits.  They are in units of a power of two that follows the largest scale; weights are rounded to float16 (2^-11) once.
+// has eight bits.  They are in units of a power of two, one a group of elements, that follows the largest scale (2^-23 of it is what keeps all its bits); weights are rounded
+// to float16 (2^-11) once.
 // The words of two keys, their halves brought together by two byte permutations, give the pairs over KEYS that the second product wants.  The
 // order of elements along k and of keys along k is free as long as both operands share it: a4_key.
 //
@@ -409,7 +410,7 @@ k_kv4_attention(A4Args a) {
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) { unit[nt][0] = EXTRA ? 1.f : sl * q_unit[nt][0]; unit[nt][1] = EXTRA ? 1.f : sl * q_unit[nt][1]; }
     float o[NT][MT][4], m[NT][2], l[NT][2];
-    float v_unit = 1.f, v_inv = 1.f, v_most = F32 ? INFINITY : 0.f;  // the sums' unit, its inverse, the largest scale in it
+    float v_unit = 1.f, v_inv = 1.f, v_most = F32 ? INFINITY : 0.f;  // the sums' unit, its inverse, the largest scale that it takes
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -617,28 +618,37 @@ k_kv4_attention(A4Args a) {
             }
             __syncwarp();                                             // (lanes parted in there, and the matrix instructions want them together)
         }
-        // bfloat16 queries: values are multiplied in float16, in units of v_unit, a power of two: scales within 2^-20 .. 248 units make values that are exact.  The
-        // unit is chosen by the first tile with values that are not zero (2^6 times its largest scale), and again where a scale outgrows it.
+        // bfloat16 queries: values are multiplied in float16, in units of a power of two: scales within 2^-20 .. 248 units make values that are exact.  A unit belongs
+        // to the elements that four lanes share (of one group: a head's groups may differ in size as they like).  It is chosen by the first tile with values
+        // that are not zero, so that the largest scale is 8 to 16 of it, and again where a scale outgrows it.  So a value keeps all its bits down to 2^-23 of the
+        // largest one of its elements, and is zero from 2^-29 on: beside weights of the same size nothing, and what a hidden or hardly seen row takes from the others.
+        // Units are compared and changed by the scales' own bits: the range of what is held is wider than that of a float32 quotient.
         uint32_t v_scale[F32 ? 1 : SUB][2];                            // pairs of scales in float16
         if constexpr (!F32) {
             float vs[SUB][4], top = 0.f;
 #pragma unroll
             for (int sub = 0; sub < SUB; sub++)
 #pragma unroll
-                for (int c = 0; c < 4; c++) { vs[sub][c] = __uint_as_float(sv[sub][c] << 16) * v_inv; top = fmaxf(top, fabsf(vs[sub][c])); }
+                for (int c = 0; c < 4; c++) { vs[sub][c] = __uint_as_float(sv[sub][c] << 16); top = fmaxf(top, fabsf(vs[sub][c])); }
             if (__any_sync(0xffffffffu, top > v_most)) {
-                top = xr_warp_max(top);
-                const float grow = __int_as_float(((int)(__float_as_uint(top) >> 23) + 6) << 23), less = __int_as_float((254 - (int)(__float_as_uint(top) >> 23) - 6) << 23);
-                v_unit *= grow; v_inv *= less; v_most = 248.f;
-#pragma unroll
-                for (int sub = 0; sub < SUB; sub++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++) vs[sub][c] *= less;
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                float less = 1.f;
+                if (top > v_most) {
+                    const int e = min(max((int)(__float_as_uint(top) >> 23) - 3, 1), 253);
+                    const float inv = __int_as_float((254 - e) << 23);
+                    less = v_unit * inv;                               // (the first time there is nothing but zeros to change)
+                    v_unit = __int_as_float(e << 23); v_inv = inv; v_most = 248.f * v_unit;
+                }
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int d = 0; d < MT; d++) { o[nt][d][0] *= less; o[nt][d][1] *= less; o[nt][d][2] *= less; o[nt][d][3] *= less; }
             }
+#pragma unroll
+            for (int sub = 0; sub < SUB; sub++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) vs[sub][c] *= v_inv;
 #pragma unroll
             for (int sub = 0; sub < SUB; sub++) { v_scale[sub][0] = a4_pack_half(vs[sub][0], vs[sub][1]); v_scale[sub][1] = a4_pack_half(vs[sub][2], vs[sub][3]); }
         }

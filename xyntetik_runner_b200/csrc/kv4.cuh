@@ -7,8 +7,9 @@
 // values 0.0074 of their square; a scale of e / 7 and codes -7 .. 7 have 0.0094, e / 7.5 0.0089).
 //
 // c has at most three significant bits (or is -8, a power of two) and s five, so that c s has eight: a bfloat16, EXACTLY.  What the
-// attention multiplies, what is read back for the prompt kernels and what a float32 model reads are the same numbers, and no kernel
-// rounds a held value.  s has its sign and its exponent: bfloat16 holds it.
+// attention multiplies, what is read back for the prompt kernels and what a float32 model reads are the same numbers.  No kernel rounds a
+// held value but one: the attention of bfloat16 queries has values in float16 units of the largest ones, token by token, and those below 2^-23 of them lose
+// bits (attention_kv4.cu).  s has its sign and its exponent: bfloat16 holds it.
 //
 // Groups whose largest magnitude is below 2^-96 are held as zeros (s = 0), groups with an element of 2^120 or more, or one that is no number,
 // as NaN (s = NaN: every value of the group is NaN): between those borders s, c s and 24 s are normal bfloat16 numbers.
