@@ -211,3 +211,17 @@ def test_a_loud_token_that_nobody_looks_at(dtype):
     o, size, _ = plain_kv4.attention(q.double().reshape(1, H, D), *held, n - 1, 0.125, bias=table.double())
     raw = plain_kv4.attention(q.double().reshape(1, H, D), *held, n - 1, 0.125)[2]
     assert torch.all((out.double().cpu().reshape(1, H, D) - o).abs() <= plain_kv4.tolerance(o, size, raw, D, dtype))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_query_of_zeros_and_the_smallest_scales(dtype):
+    """Scores of zero: equal weights, for every position and every positive scale."""
+    from xyntetik_runner_b200 import kernels
+    for scale in (1.0, 1e-3, 1e-12, 1e-30, 1e-38):
+        args, q, held, plain, Ts, starts, pos0 = attention_case([200, 70], 3, 4, 2, 64, 16, dtype, 0, 0, 0, 0, 0)
+        q[:, :] = 0.0
+        q[1] = 1e-20
+        args["scale"] = plain["scale"] = scale
+        out = torch.full((q.shape[0], 4 * 64), 9.0, dtype=dtype, device=DEV)
+        kernels.attention_kv4(q.to(DEV), out, **args)
+        check(out, q, held, plain, Ts, starts, pos0, 4, 64, dtype)

@@ -408,7 +408,12 @@ k_kv4_attention(A4Args a) {
     constexpr float LIFT = F32 ? 0.f : 5.f;
     float unit[NT][2];                                               // what turns a column's scores into exponents of two
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) { unit[nt][0] = EXTRA ? 1.f : sl * q_unit[nt][0]; unit[nt][1] = EXTRA ? 1.f : sl * q_unit[nt][1]; }
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            unit[nt][e] = EXTRA ? 1.f : sl * q_unit[nt][e];
+            if (unit[nt][e] == 0.f) unit[nt][e] = __int_as_float(1);       // (below float32: a hidden key's minus infinity times it is to stay that)
+        }
     float o[NT][MT][4], m[NT][2], l[NT][2];
     float v_unit = 1.f, v_inv = 1.f, v_most = F32 ? INFINITY : 0.f;  // the sums' unit, its inverse, the largest scale that it takes
 #pragma unroll
