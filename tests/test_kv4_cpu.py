@@ -187,3 +187,24 @@ def test_numbers_that_have_more_than_31_bits(name):
     if name == "keep_first":
         with pytest.raises(kernels.KernelError, match="keep_first"):
             kernels.kv4_read(p["cache"], 0, 16, p["block_tables"], i, i, torch.zeros(2, 2, 2, 16, 64), keep_first=2 ** 31)
+
+
+def test_portions_that_are_read_back_together():
+    """Neighbours up to so many pages, one at least, none without a page; the sums are those of one plan over each."""
+    l, p = np.array([60, 1, 90, 0, 60, 200, 60], dtype=np.int32), np.array([100, 900, 10, 4, 0, 800, 4], dtype=np.int32)
+    plan = lambda a, b: kernels.kv4_plan((l[a:b], p[a:b]), 1000, 900, 4, 64, 16, kernels.BF16, 0, 0, 64, 0, rule=False)
+    each = [plan(i, i + 1)[3] for i in range(7)]
+    assert each == [10, 0, 7, 0, 4, 63, 4]
+    for at_once in (1, 10, 11, 17, 21, 84, 88, 1000):
+        groups = kernels._kv4_groups(plan, 7, at_once)
+        assert sum(g[2] for g in groups) == sum(each) and [g[0] for g in groups] == sorted(g[0] for g in groups)
+        for a, b, pages, longest, t128, t64, end in groups:
+            long = [i for i in range(a, b) if each[i]]
+            assert pages == sum(each[a:b]) and (pages <= at_once or len(long) == 1)
+            assert longest == max(l[i] for i in long) and end == max(l[i] + p[i] for i in long)
+            assert t128 == sum(-(-4 * l[i] // 128) for i in long) and t64 == sum(-(-4 * l[i] // 64) for i in long)
+    assert len(kernels._kv4_groups(plan, 7, 1000)) == 1 and len(kernels._kv4_groups(plan, 7, 1)) == 5
+    # a rule that is asked may send portions to the codes; one that stands does not
+    few = (np.array([60], dtype=np.int32), np.array([15], dtype=np.int32))
+    asked, stands = (kernels.kv4_plan(few, 100, 2, 4, 64, 16, kernels.BF16, 0, 0, 64, 0, rule=r) for r in (True, False))
+    assert asked[:2].tolist() == [1, 0] and stands[:2].tolist() == [0, 1] and stands[8] == 64

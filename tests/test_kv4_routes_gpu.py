@@ -240,3 +240,32 @@ def test_a_query_of_zeros_and_the_smallest_scales(dtype):
         out = torch.full((q.shape[0], 4 * 64), 9.0, dtype=dtype, device=DEV)
         kernels.attention_kv4(q.to(DEV), out, **args)
         check(out, q, held, plain, Ts, starts, pos0, 4, 64, dtype)
+
+
+@pytest.mark.parametrize("H,K,D,P", [(64, 8, 128, 64), (66, 33, 48, 24)])
+@pytest.mark.parametrize("captured", [False, True])
+def test_rows_read_back_a_few_requests_at_a_time(H, K, D, P, captured, monkeypatch):
+    """A step whose rows are more than are read back at once: the same bits as in one go, within the bytes that are said or one request's."""
+    from xyntetik_runner_b200 import kernels
+    contexts, Ts = [400, 90, 300, 5, 700, 200, 120], [100, 1, 60, 5, 90, 0, 120]
+    args, q, held, plain, Ts, starts, pos0 = attention_case(contexts, Ts, H, K, D, P, BF16, 0, 0, 0, 0, 0)
+    qd, outs, asked = q.to(DEV), [], []
+    for pages in (10 ** 6, 9, 1):
+        monkeypatch.setattr(kernels, "KV4_VALUES_BYTES", pages * 4 * K * P * D)
+        out, buf, sizes = torch.full((q.shape[0] + 5, H * D), 9.0, dtype=BF16, device=DEV), shared(), {}
+        call = lambda: kernels.attention_kv4(qd, out[:-5], **args, buf=lambda name, shape, dtype: (sizes.__setitem__(name, shape), buf(name, shape, dtype))[1])
+        call()
+        if captured:
+            g = torch.cuda.CUDAGraph()
+            torch.cuda.synchronize()
+            with torch.cuda.graph(g):
+                call()
+            out[:-5] = 9.0
+            g.replay()
+        kernels.tc_check_status(torch.device(DEV))
+        outs.append(out)
+        asked.append(sizes["kv4_values"][0])
+    check_many(outs[0][:-5], q, held, Ts, starts, pos0, H, D, BF16)
+    assert all(torch.equal(out, outs[0]) for out in outs) and torch.all(outs[0][-5:] == 9.0)
+    longest = args["block_tables"].shape[1]
+    assert asked[0] >= sum(-(-c // P) for c, T in zip(contexts, Ts) if T * H // K > 64) and asked[1] <= max(9, longest) and asked[2] <= longest

@@ -997,9 +997,10 @@ static bool a4_by_codes(long long row_blocks, bool full, int hs) { return row_bl
 // prompt kernels (of more than `most_rows` packed rows, all or none of them: a4_by_codes), [2] float32 values of scratch that xr_kv4_attention needs
 // for the first; of the others [3] the pages that xr_kv4_read writes for them, [4] the most tokens, [5], [6] the row tiles of 128 and 64 packed rows, [7] the
 // furthest end; [8] the most packed rows of a portion that attends to the codes; [9] .. [13] how those are cut, as xr_kv4_attention takes it.
-// n: tokens of the step; max_kv: how far requests may get by the time the launches run (0: as far as the portions go).
+// n: tokens of the step; max_kv: how far requests may get by the time the launches run (0: as far as the portions go); rule: whether a4_by_codes is asked, or
+// most_rows stands as it is (some portions of a step whose rule has been asked).
 XR_EXPORT int xr_kv4_plan(const int* len, const int* pos0, int n_seg, int n, int K, int G, int D, int page_size, int dtype, int window, int keep_first,
-                          int most_rows, int max_kv, long long* said) {
+                          int most_rows, int max_kv, int rule, long long* said) {
     if (n_seg < 1 || n < 0 || K < 1 || G < 1 || D < 1 || D > 256 || page_size < 1 || window < 0 || keep_first < 0 || most_rows < 0 || max_kv < 0) return XR_ERR_ARG;
     long long tokens = 0, row_blocks = 0;
     bool full = true;
@@ -1011,7 +1012,7 @@ XR_EXPORT int xr_kv4_plan(const int* len, const int* pos0, int n_seg, int n, int
         if (rows > most_rows) { row_blocks += (rows + 15) / 16 * K; full = full && rows % 128 == 0; }
     }
     if (tokens > n) return XR_ERR_ARG;
-    if (row_blocks > 0 && a4_by_codes(row_blocks, full, kv4_held(D))) most_rows = 1 << 30;
+    if (rule && row_blocks > 0 && a4_by_codes(row_blocks, full, kv4_held(D))) most_rows = 1 << 30;
     said[8] = most_rows;
     for (int s = 0; s < n_seg; s++) {
         const long long l = len[s], p = pos0[s], rows = l * G;

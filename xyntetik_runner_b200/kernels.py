@@ -882,6 +882,9 @@ def kv4_read(cache: torch.Tensor, layer: int, page_size: int, block_tables: torc
 # way decides (csrc/attention_kv4.cu: a4_by_codes).
 KV4_SHORT_ROWS = 64
 _KV4_ALL_ROWS = 1 << 30
+# Bytes of rows that are read back at once (what the latent attention takes for its expanded rows, too): the portions of a step that see more go a few
+# requests at a time, one request at least.  65,536 rows of 8 kv heads of 128 elements.
+KV4_VALUES_BYTES = 1 << 29
 _NP_I32 = np.dtype(np.int32)
 
 
@@ -890,18 +893,34 @@ _PLAN = ("short", "long", "floats", "pages", "longest", "tiles_128", "tiles_64",
 
 
 def kv4_plan(lengths: tuple, n: int, kv_heads: int, group: int, head_dim: int, page_size: int, code: int, window: int, keep_first: int, most_rows: int,
-             max_kv_len: int = 0):
+             max_kv_len: int = 0, rule: bool = True):
     """What the portions `lengths` = (tokens, first positions) ask for, on the host: how many attend to the codes and how many (of those of more than `most_rows`
     packed rows) go through the prompt kernels; floats of scratch for the first; of the others the pages that their rows are read back into, the
     tokens of the longest, their row tiles of 128 and 64 rows, and the end of the furthest; the most rows of one that attends to the codes; then how those are
-    cut, as the launcher takes it.  Raises where they do not fit `n` tokens."""
+    cut, as the launcher takes it.  `rule` False: `most_rows` stands, whatever the portions would cost either way.  Raises where they do not fit `n` tokens."""
     h_len, h_pos = lengths
     if h_len.dtype != _NP_I32 or h_pos.dtype != _NP_I32 or h_len.ndim != 1 or h_len.shape != h_pos.shape:
         raise KernelError("lengths: two int32 numpy arrays, one value a portion")
     said = array("q", (0,) * len(_PLAN))
-    if _c.xr_kv4_plan(h_len, h_pos, h_len.size, n, kv_heads, group, head_dim, page_size, code, window, keep_first, most_rows, max_kv_len, said) != 0:
+    if _c.xr_kv4_plan(h_len, h_pos, h_len.size, n, kv_heads, group, head_dim, page_size, code, window, keep_first, most_rows, max_kv_len, int(rule), said) != 0:
         raise KernelError("lengths: portions that q does not hold, or positions below zero")
     return said
+
+
+def _kv4_groups(plan, n_seg: int, at_once: int):
+    """Neighbouring portions whose rows are read back together, at most `at_once` pages of them or a single one: (first portion, end, pages, tokens of the longest,
+    row tiles of 128 and 64 rows, furthest end).  plan(a, b): ``kv4_plan`` of portions a .. b - 1."""
+    each = [plan(i, i + 1) for i in range(n_seg)]
+    groups, a = [], 0
+    while a < n_seg:
+        b, pages = a + 1, each[a][3]
+        while b < n_seg and pages + each[b][3] <= at_once:
+            pages += each[b][3]
+            b += 1
+        if pages:
+            groups.append((a, b, *plan(a, b)[3:8]))
+        a = b
+    return groups
 
 
 def attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, layer: int, page_size: int, seg_start: torch.Tensor, seg_len: torch.Tensor,
@@ -914,7 +933,7 @@ def attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, layer
     that is captured in a graph may be replayed with other positions but the same seg_len (say in `max_kv_len` how long the requests may get: the
     cut suits that, and scratch for rows read back holds that much; 0: as much as the block tables name).  Rows on a page that is not held count as zeros.  Options: see ``attention_simt``.
     Single tokens, short portions and whatever the prompt kernels do not take attend to the codes; where longer portions are many rows, they read the
-    rows they see back into `buf` (``buf(name, shape, dtype)`` gives scratch; None: allocated) and go through the prompt kernels.  `early`: the caller says that
+    rows they see back, a few requests at a time (KV4_VALUES_BYTES), into `buf` (``buf(name, shape, dtype)`` gives scratch; None: allocated) and go through the prompt kernels.  `early`: the caller says that
     nothing still running writes the portions, the block tables or rows ahead of a portion's first (an engine's step); they may then be read before
     the kernel ahead in the stream is complete."""
     K = cache.shape[2] if cache.ndim == 4 else 0
@@ -947,30 +966,41 @@ def attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, layer
     aligned = code == BF16 and q_row % 8 == 0 and q.data_ptr() % 16 == 0 and head_dim % 16 == 0 and head_dim <= 128 and out.data_ptr() % 16 == 0
     most = max(KV4_SHORT_ROWS, G) if aligned else _KV4_ALL_ROWS          # (single tokens never)
     short, long, floats, pages, longest, tiles_128, tiles_64, end, most, *cut = kv4_plan(lengths, n, K, G, head_dim, page_size, code, window, keep_first, most, max_kv_len)
+    reach = max_kv_len
     if long and max_kv_len == 0 and torch.cuda.is_current_stream_capturing():
         reach = min(max_pages * page_size, 2 ** 31 - 1)
         short, long, floats, pages, longest, tiles_128, tiles_64, end, most, *cut = kv4_plan(lengths, n, K, G, head_dim, page_size, code, window, keep_first, most, reach)
     if long:
         def scratch(name, shape, dt):
             return torch.empty(shape, dtype=dt, device=out.device) if buf is None else buf(name, shape, dt)
+        plan = lambda a, b: kv4_plan((lengths[0][a:b], lengths[1][a:b]), n, K, G, head_dim, page_size, code, window, keep_first, most, reach, rule=False)
+        at_once = max(1, KV4_VALUES_BYTES // (4 * K * page_size * head_dim))
+        groups, room = ((0, n_seg, pages, longest, tiles_128, tiles_64, end),), pages
+        if pages > at_once:
+            groups = _kv4_groups(plan, n_seg, at_once)
+            room = max(g[2] for g in groups)
+        if buf is not None:
+            # (rounded up, so that an engine's buffer is made anew a few times and not with every longer prompt; to what one request may take)
+            room = max(room, min(1 << (room - 1).bit_length(), max(at_once, max_pages)))
         ints = scratch("kv4_portions", (3 * n_seg + n_seg * max_pages,), _I32)
-        first, last, long_len, tables = ints[:n_seg], ints[n_seg:2 * n_seg], ints[2 * n_seg:3 * n_seg], ints[3 * n_seg:].view(n_seg, max_pages)
-        # (rounded up, so that an engine's buffer is made anew a few times and not with every longer prompt)
-        room = pages if buf is None else 1 << (pages - 1).bit_length()
         values = scratch("kv4_values", (room, 2, K, page_size, head_dim), torch.bfloat16)
-        _check(_c.xr_kv4_long(at_len, at_pos, first.data_ptr(), last.data_ptr(), long_len.data_ptr(), tables.data_ptr(), n_seg, max_pages, G, window, most,
-                              _stream()), "attention_kv4")
-        _check(_c.xr_kv4_read(*args, block_tables.data_ptr(), first.data_ptr(), last.data_ptr(), values.data_ptr(), BF16, tables.data_ptr(), n_seg, max_pages,
-                              head_dim, keep_first, pages, _stream()), "attention_kv4")
-        _count(2)
         half = K * page_size * head_dim
-        if attention_tc_supported(dtype, heads, K, head_dim, page_size):
-            attention_tc(q, out, seg_start, long_len, seg_pos0, tables, (values.data_ptr(), pages, 1, 0), heads, K, head_dim, max_pages, page_size, window,
-                         scale, n_seg, longest, row_tiles=tiles_128, sink=sink, softcap=softcap, keep_first=keep_first, bias=bias)
-        else:
-            attention_mma(q, q_row, out, values.data_ptr(), seg_start, long_len, seg_pos0, tables, None, None, 2 * half, half, heads, K, head_dim, max_pages,
-                          page_size, window, scale, n_seg, longest, end, 0, False, True, row_tiles=tiles_64, sink=sink, softcap=softcap,
-                          keep_first=keep_first, bias=bias)
+        for a, b, pages, longest, tiles_128, tiles_64, end in groups:
+            s = b - a
+            starts, lens, pos0, bt = (seg_start, seg_len, seg_pos0, block_tables) if s == n_seg else (t[a:b] for t in (seg_start, seg_len, seg_pos0, block_tables))
+            first, last, long_len, tables = ints[:s], ints[s:2 * s], ints[2 * s:3 * s], ints[3 * s:3 * s + s * max_pages].view(s, max_pages)
+            _check(_c.xr_kv4_long(lens.data_ptr(), pos0.data_ptr(), first.data_ptr(), last.data_ptr(), long_len.data_ptr(), tables.data_ptr(), s, max_pages, G,
+                                  window, most, _stream()), "attention_kv4")
+            _check(_c.xr_kv4_read(*args, bt.data_ptr(), first.data_ptr(), last.data_ptr(), values.data_ptr(), BF16, tables.data_ptr(), s, max_pages, head_dim,
+                                  keep_first, pages, _stream()), "attention_kv4")
+            _count(2)
+            if attention_tc_supported(dtype, heads, K, head_dim, page_size):
+                attention_tc(q, out, starts, long_len, pos0, tables, (values.data_ptr(), pages, 1, 0), heads, K, head_dim, max_pages, page_size, window,
+                             scale, s, longest, row_tiles=tiles_128, sink=sink, softcap=softcap, keep_first=keep_first, bias=bias)
+            else:
+                attention_mma(q, q_row, out, values.data_ptr(), starts, long_len, pos0, tables, None, None, 2 * half, half, heads, K, head_dim, max_pages,
+                              page_size, window, scale, s, longest, end, 0, False, True, row_tiles=tiles_64, sink=sink, softcap=softcap,
+                              keep_first=keep_first, bias=bias)
     if short:
         spans = None
         if floats:
