@@ -208,3 +208,63 @@ def test_portions_that_are_read_back_together():
     few = (np.array([60], dtype=np.int32), np.array([15], dtype=np.int32))
     asked, stands = (kernels.kv4_plan(few, 100, 2, 4, 64, 16, kernels.BF16, 0, 0, 64, 0, rule=r) for r in (True, False))
     assert asked[:2].tolist() == [1, 0] and stands[:2].tolist() == [0, 1] and stands[8] == 64
+
+
+def test_the_context_that_fits(monkeypatch):
+    """-c 0 with four bits: the pool and the buffer of rows read back, as the attention asks for it, fit; one more page of every request does not."""
+    from xyntetik_runner_b200 import architectures  # noqa: F401
+    from xyntetik_runner_b200.config import registry
+    from xyntetik_runner_b200.engine.runner import Runner
+    d = {"architectures": ["LlamaForCausalLM"], "hidden_size": 256, "num_hidden_layers": 3, "num_attention_heads": 8, "num_key_value_heads": 2, "head_dim": 64,
+         "intermediate_size": 320, "vocab_size": 300, "rms_norm_eps": 1e-5, "rope_theta": 10000.0, "max_position_embeddings": 1 << 30,
+         "tie_word_embeddings": False, "torch_dtype": "bfloat16"}
+    arch = registry.resolve(registry.architecture_name(d))
+    for dtype, heads_dim in (("bfloat16", 64), ("bfloat16", 100), ("float32", 64)):
+        cfg = arch.config_from_dict({**d, "head_dim": heads_dim})
+        weights = 2 * sum(math.prod(s.shape) for s in arch.build_plan(cfg).tensor_specs().values())
+        reads = dtype == "bfloat16" and heads_dim % 16 == 0
+        for free in (1 << 26, 1 << 30, 7 << 30, 150 << 30):
+            monkeypatch.setattr(torch.cuda, "mem_get_info", lambda *a, f=free: (f, 1 << 38))
+            for parallel in (1, 3, 64):
+                for P in (16, 64):
+                    room = int(0.9 * free) - 2 * weights
+                    token = 3 * 2 * kernels.kv4_block_bytes(heads_dim, 8) // 8
+                    values = 2 * 2 * heads_dim * 2 if reads else 0
+
+                    def held(n):
+                        rows = max(kernels.KV4_VALUES_BYTES, values * n)              # one request's rows, or so many bytes of several
+                        return n * token * parallel + min(rows, 2 * values * n * parallel)
+                    n = Runner._fit_context(arch, cfg, 1 << 30, parallel, P, dtype, "cuda:0", "int4")
+                    assert n % P == 0 and held(n) <= room and (held(n + P) > room or n == 1 << 30)
+                    elem = 2 if dtype == "bfloat16" else 4
+                    same = Runner._fit_context(arch, cfg, 1 << 30, parallel, P, dtype, "cuda:0")
+                    assert same == room // (3 * 2 * 2 * heads_dim * elem * parallel) // P * P
+        monkeypatch.setattr(torch.cuda, "mem_get_info", lambda *a: (2 * weights, 1 << 38))
+        with pytest.raises(ValueError, match="no context fits"):
+            Runner._fit_context(arch, cfg, 1 << 30, 4, 16, dtype, "cuda:0", "int4")
+
+
+def test_a_larger_buffer_does_not_wait_beside_the_old_one(monkeypatch):
+    """An engine's buffer that grows: the old one and everything that holds it are gone when the new one is made; a failure leaves none behind."""
+    import weakref
+    from types import SimpleNamespace
+    from xyntetik_runner_b200.engine.engine import Engine, StepContext
+    eng = Engine.__new__(Engine)
+    eng.params, eng.device = SimpleNamespace(max_step_tokens=0), torch.device("cpu")
+    eng._bufs, eng._views, eng._graphs, eng._uneven_of_shape, eng._buf_generation = {}, {}, {}, {}, 0
+    ctx = StepContext.__new__(StepContext)
+    ctx._eng, ctx._views = eng, eng._views
+    ctx.buf("a", (10,), torch.int32)
+    old = weakref.ref(eng._bufs[("a", torch.int32)])
+    eng._graphs["one"] = object()
+    real, seen = torch.empty, []
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: (seen.append(old() is None and not eng._graphs), real(*a, **k))[1])
+    assert ctx.buf("a", (11,), torch.int32).shape == (11,) and seen == [True] and eng._buf_generation == 2
+
+    def fails(*a, **k):
+        raise torch.cuda.OutOfMemoryError("no room")
+    monkeypatch.setattr(torch, "empty", fails)
+    with pytest.raises(torch.cuda.OutOfMemoryError):
+        ctx.buf("a", (12,), torch.int32)
+    monkeypatch.setattr(torch, "empty", real)
+    assert ctx.buf("a", (12,), torch.int32).shape == (12,) and eng._buf_generation == 4

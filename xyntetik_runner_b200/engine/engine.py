@@ -249,12 +249,14 @@ class Engine:
             cap = n
             if t is None and len(shape) == 2 and shape[0] < self.params.max_step_tokens and name != "logits":
                 cap = self.params.max_step_tokens * int(shape[1])
-            t = torch.empty(max(cap, 1), dtype=dtype, device=self.device)
-            self._bufs[key] = t
+            # the old buffer goes first, with all that holds it: the two need not fit side by side
+            self._bufs.pop(key, None)
+            t = None
             self._buf_generation += 1
             self._views.clear()
             self._graphs.clear()
             self._uneven_of_shape.clear()
+            t = self._bufs[key] = torch.empty(max(cap, 1), dtype=dtype, device=self.device)
         return t[:n].view(*shape)
 
     # ---- requests ----------------------------------------------------------------

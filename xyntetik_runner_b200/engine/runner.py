@@ -174,14 +174,22 @@ class Runner:
             if need is not None and e.cache_from is None:
                 in_four = kv == "int4" and need.four_bits
                 per_token += need.kv_heads * kv_head_bytes(need, elem, True) if in_four else 2 * need.kv_heads * need.head_dim * elem
-                if in_four and elem == 2:
+                if in_four and kernels.kv4_reads_back(torch.bfloat16 if elem == 2 else torch.float32, need.head_dim):
                     values = max(values, 2 * need.kv_heads * need.head_dim * elem)
-        per_token += values
         free, _ = torch.cuda.mem_get_info(torch.device(device))
         room = int(0.9 * free) - 2 * wbytes                      # (packing a matrix needs a second copy for a moment)
         if per_token == 0:
             return model_limit
-        fit = room // (per_token * parallel) // page_size * page_size
+        fit = room // (per_token * parallel) // page_size
+        if values:
+            # (the rows read back grow with the context, but not always: the most pages whose rows fit beside the buffer, by halves)
+            held = lambda pages: pages * page_size * per_token * parallel + kernels.kv4_read_back_bytes(values, pages * page_size, parallel)
+            least, fit = 0, max(fit, 0) + 1
+            while fit - least > 1:
+                half = (least + fit) // 2
+                least, fit = (half, fit) if held(half) <= room else (least, half)
+            fit = least
+        fit *= page_size
         if fit < page_size:
             raise ValueError(f"-c 0: no context fits beside the weights ({free >> 20} MiB free, weights {wbytes >> 20} MiB)")
         return int(min(model_limit, fit))

@@ -907,6 +907,17 @@ def kv4_plan(lengths: tuple, n: int, kv_heads: int, group: int, head_dim: int, p
     return said
 
 
+def kv4_reads_back(dtype: torch.dtype, head_dim: int) -> bool:
+    """Whether longer portions may go through a prompt kernel, by their type and head size."""
+    return dtype is torch.bfloat16 and head_dim % 16 == 0 and head_dim <= 128
+
+
+def kv4_read_back_bytes(bytes_per_token: int, tokens: int, requests: int) -> int:
+    """The most that an engine's buffer of rows read back takes, for `requests` of up to `tokens` rows of so many bytes: one request's, or KV4_VALUES_BYTES of
+    several; the rows that there are, rounded up, where those are fewer."""
+    return min(2 * bytes_per_token * tokens * requests, max(KV4_VALUES_BYTES, bytes_per_token * tokens))
+
+
 def _kv4_groups(plan, n_seg: int, at_once: int):
     """Neighbouring portions whose rows are read back together, at most `at_once` pages of them or a single one: (first portion, end, pages, tokens of the longest,
     row tiles of 128 and 64 rows, furthest end).  plan(a, b): ``kv4_plan`` of portions a .. b - 1."""
@@ -963,7 +974,7 @@ def attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, layer
     if lengths[0].size != n_seg:
         raise KernelError("lengths: two int32 numpy arrays, one value a portion")
     # portions that the prompt kernels take: bfloat16 on 16-byte borders, head sizes that one of them has
-    aligned = code == BF16 and q_row % 8 == 0 and q.data_ptr() % 16 == 0 and head_dim % 16 == 0 and head_dim <= 128 and out.data_ptr() % 16 == 0
+    aligned = kv4_reads_back(dtype, head_dim) and q_row % 8 == 0 and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0
     most = max(KV4_SHORT_ROWS, G) if aligned else _KV4_ALL_ROWS          # (single tokens never)
     short, long, floats, pages, longest, tiles_128, tiles_64, end, most, *cut = kv4_plan(lengths, n, K, G, head_dim, page_size, code, window, keep_first, most, max_kv_len)
     reach = max_kv_len
@@ -980,9 +991,10 @@ def attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, layer
             groups = _kv4_groups(plan, n_seg, at_once)
             room = max(g[2] for g in groups)
         if buf is not None:
-            # (rounded up, so that an engine's buffer is made anew a few times and not with every longer prompt; to what one request may take)
+            # (rounded up, so that an engine's buffers are made anew a few times and not with every longer prompt or batch; the rows to what one request may take)
             room = max(room, min(1 << (room - 1).bit_length(), max(at_once, max_pages)))
-        ints = scratch("kv4_portions", (3 * n_seg + n_seg * max_pages,), _I32)
+        need = n_seg * (3 + max_pages)
+        ints = scratch("kv4_portions", (need if buf is None else 1 << (need - 1).bit_length(),), _I32)
         values = scratch("kv4_values", (room, 2, K, page_size, head_dim), torch.bfloat16)
         half = K * page_size * head_dim
         for a, b, pages, longest, tiles_128, tiles_64, end in groups:
