@@ -268,3 +268,15 @@ def test_a_larger_buffer_does_not_wait_beside_the_old_one(monkeypatch):
         ctx.buf("a", (12,), torch.int32)
     monkeypatch.setattr(torch, "empty", real)
     assert ctx.buf("a", (12,), torch.int32).shape == (12,) and eng._buf_generation == 4
+
+
+@pytest.mark.parametrize("lens,ends,K,G,D,code", [([1985] + [1] * 63, [1985] + [8001] * 63, 8, 4, 128, 0), ([40] + [1] * 63, [40] + [8001] * 62 + [131001], 8, 4, 128, 1),
+                                                  ([1900, 1], [1900, 100001], 8, 4, 192, 1), ([1900] + [1] * 31, [1900] + [8001] * 31, 2, 4, 256, 1)])
+def test_scratch_of_steps_that_mix_portions_and_single_tokens(lens, ends, K, G, D, code):
+    """Scratch goes by the row blocks that there are, within 256 MB; every tile still belongs to a span."""
+    l, e = np.array(lens, dtype=np.int32), np.array(ends, dtype=np.int32)
+    said = dict(zip(kernels._PLAN, kernels.kv4_plan((l, e - l), int(l.sum()), K, G, D, 64, code, 0, 0, 1 << 30)))
+    rows = 8 if code == 0 or not said["wide"] else 16
+    assert said["splits"] > 1 and not said["clustered"] and said["blocks"] == sum(-(-n * G // rows) for n in lens)
+    assert said["floats"] == said["blocks"] * K * said["splits"] * rows * (plain_kv4.held(D) + 2) <= 1 << 26
+    assert said["splits"] * said["span_tiles"] * (64 if D <= 128 else 32) >= max(ends)

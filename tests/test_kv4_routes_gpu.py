@@ -269,3 +269,29 @@ def test_rows_read_back_a_few_requests_at_a_time(H, K, D, P, captured, monkeypat
     assert all(torch.equal(out, outs[0]) for out in outs) and torch.all(outs[0][-5:] == 9.0)
     longest = args["block_tables"].shape[1]
     assert asked[0] >= sum(-(-c // P) for c, T in zip(contexts, Ts) if T * H // K > 64) and asked[1] <= max(9, longest) and asked[2] <= longest
+
+
+@pytest.mark.parametrize("contexts,Ts,H,K,D,P,dtype", [
+    ([9000, 300, 5000, 60], [1, 40, 5, 0], 8, 2, 64, 64, BF16), ([9000, 300, 5000, 60], [1, 40, 5, 0], 8, 2, 64, 64, F32),
+    ([6000, 300, 300, 700], [1, 210, 8, 7], 32, 4, 128, 64, BF16), ([4000, 9000, 300, 2000], [3, 1, 30, 7], 6, 3, 100, 24, BF16)])
+def test_partial_sums_of_portions_of_many_lengths(contexts, Ts, H, K, D, P, dtype):
+    """Spans of portions with one row block and with many, empty ones and ones that go another way among them, in the scratch that the plan says and no further."""
+    from xyntetik_runner_b200 import kernels
+    args, q, held, plain, Ts, starts, pos0 = attention_case(contexts, Ts, H, K, D, P, dtype, 0, 0, 0, 0, 0)
+    aligned = dtype is BF16 and D % 16 == 0
+    said = dict(zip(kernels._PLAN, kernels.kv4_plan(args["lengths"], q.shape[0], K, H // K, D, P, kernels.dtype_code(dtype), 0, 0, 64 if aligned else 1 << 30)))
+    assert said["floats"] > 0 and said["row_blocks"] > 1 and (said["long"] > 0) == (H == 32)
+    whole = {}
+
+    def buf(name, shape, dt):
+        t = torch.empty(math.prod(shape) + 64, dtype=dt, device=DEV)
+        if name == "kv4_spans":
+            t.fill_(math.nan)
+            whole[name] = t
+        return t[:math.prod(shape)].view(*shape)
+    for b in (None, buf):
+        out = torch.full((q.shape[0], H * D), 9.0, dtype=dtype, device=DEV)
+        kernels.attention_kv4(q.to(DEV), out, **args, buf=b)
+        kernels.tc_check_status(torch.device(DEV))
+        check_many(out, q, held, Ts, starts, pos0, H, D, dtype)
+    assert torch.isnan(whole["kv4_spans"][said["floats"]:]).all()

@@ -52,8 +52,9 @@ struct A4Args {
     const void* q; void* out;
     Kv4Cache c;
     const int* seg_start; const int* seg_len; const int* seg_pos0; const int* block_tables;
-    float* part_acc;                  // [n_seg][K][row_blocks][splits][rows][hs]
-    float* part_ml;                   // [n_seg][K][row_blocks][splits][rows][2]
+    float* part_acc;                  // [blocks][K][splits][rows][hs]
+    float* part_ml;                   // [blocks][K][splits][rows][2]
+    int blocks;                       // row blocks of all portions, one after another (a4_place)
     long long q_stride;
     int H, G, D, max_pages, window, keep, splits, span_tiles, row_blocks, most_rows;
     float scale, softcap;
@@ -207,6 +208,17 @@ __device__ __forceinline__ A4Walk a4_walk(int first_pos, int last_pos, int windo
 // Spans of a request: a.span_tiles tiles each, the last of the grid's takes what is left (a captured launch may meet longer requests
 // than the one it was planned for).
 __device__ __forceinline__ int a4_spans(const A4Args& a, const A4Walk& w) { return min((w.n + a.span_tiles - 1) / a.span_tiles, a.splits); }
+
+// The place of a row block in the scratch for partial sums: row blocks of all portions that are taken lie one after another.  All lanes of a warp.
+__device__ __forceinline__ int a4_place(const A4Args& a, int seg, int rb, int rows) {
+    if (a.row_blocks == 1) return seg;                               // (one a portion; none for an empty one, whose place stays free)
+    int ahead = 0;
+    for (int s = threadIdx.x & 31; s < seg; s += 32) {
+        const long long r = (long long)a.seg_len[s] * a.G;
+        if (r > 0 && r <= a.most_rows) ahead += (int)((r + rows - 1) / rows);
+    }
+    return __reduce_add_sync(0xffffffffu, ahead) + rb;
+}
 
 // NG: groups of 32 elements a held head (2, 4, 8); NT: eight-row tiles a block; F32: float32 queries and outputs, in pieces (NT 1);
 // EXTRA: a cap or a bias on the scores
@@ -747,7 +759,12 @@ k_kv4_attention(A4Args a) {
             if (g == 0) { ml_s[(warp * RB + r) * 2] = m[nt][e] - LIFT; ml_s[(warp * RB + r) * 2 + 1] = sum; }
         }
     __syncthreads();
-    const size_t item = (((size_t)seg * a.c.K + kvh) * a.row_blocks + rb) * a.splits + span;
+    size_t item = 0;
+    if (n_spans > 1 && !a.clustered) {
+        const int place = a4_place(a, seg, rb, RB);
+        if ((unsigned)place >= (unsigned)a.blocks) return;           // (lengths that the launch was not made for: nothing is written beyond the scratch)
+        item = ((size_t)place * a.c.K + kvh) * a.splits + span;
+    }
     for (int q = threadIdx.x; q < rows * (HS / 4); q += A4_THREADS) {
         const int r = q / (HS / 4), d = (q % (HS / 4)) * 4;
         float mm = -INFINITY;
@@ -812,6 +829,7 @@ k_kv4_attention(A4Args a) {
 // ---------------------------------------------------------------------------------------------
 #define A4_MERGE_THREADS 512
 #define A4_MAX_SPLITS 256
+#define A4_MAX_FLOATS (1LL << 26)      // of scratch for partial sums (256 MB): spans are made longer until they fit
 #define A4_START 1.5
 #define A4_MEET 0.5
 #define A4_MERGE 1.3
@@ -831,7 +849,9 @@ k_kv4_merge(A4Args a) {
     const int row0 = rb * RB, rows = (int)min((long long)RB, rows_all - row0), pos0 = a.seg_pos0[seg];
     const int n_spans = a4_spans(a, a4_walk(pos0 + row0 / a.G, pos0 + (row0 + rows - 1) / a.G, a.window, a.keep, TK));
     if (n_spans == 1) return;                                        // (written already)
-    const size_t item = ((size_t)seg * gridDim.x + blockIdx.x) * a.splits;
+    const int place = a4_place(a, seg, rb, RB);
+    if ((unsigned)place >= (unsigned)a.blocks) return;
+    const size_t item = ((size_t)place * a.c.K + kvh) * a.splits;
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + item * RB;
     const float4* acc = reinterpret_cast<const float4*>(a.part_acc) + item * RB * QUADS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -884,7 +904,7 @@ static int a4_tile(int hs) { return hs <= 128 ? 64 : 32; }
 
 // How a step is cut: row blocks of the longest portion that is taken (at most `most_rows` packed rows), tiles a span, spans of the longest
 // request.  len, pos0: the portions on the HOST; max_kv: the longest key range to be prepared for (0: what the portions say).
-struct A4Plan { int row_blocks, wide, span_tiles, splits, clustered; };
+struct A4Plan { int row_blocks, wide, span_tiles, splits, clustered, blocks; };
 static A4Plan a4_plan(const int* len, const int* pos0, int n_seg, int K, int G, int hs, int f32, int window, int keep, int most_rows, int max_kv) {
     const int tile = a4_tile(hs);
     long long rows = 0;
@@ -892,7 +912,7 @@ static A4Plan a4_plan(const int* len, const int* pos0, int n_seg, int K, int G, 
         const long long r = (long long)len[s] * G;
         if (r <= most_rows && r > rows) rows = r;
     }
-    A4Plan p{0, rows > 8, A4_WARPS, 1, 0};
+    A4Plan p{0, rows > 8, A4_WARPS, 1, 0, n_seg};
     if (rows < 1) return p;
     const int rb = a4_rows(f32, p.wide);
     p.row_blocks = (int)((rows + rb - 1) / rb);
@@ -945,6 +965,18 @@ static A4Plan a4_plan(const int* len, const int* pos0, int n_seg, int K, int G, 
         longest = (int)(t > longest ? (t < more ? t : (more > longest ? more : longest)) : longest);
     }
     p.splits = (longest + p.span_tiles - 1) / p.span_tiles;
+    if (p.row_blocks > 1) {
+        p.blocks = 0;
+        for (int s = 0; s < n_seg; s++)
+            if (taken(s)) p.blocks += (int)(((long long)len[s] * G + rb - 1) / rb);
+    }
+    const long long span_floats = (long long)p.blocks * K * rb * (hs + 2);
+    if (p.splits > 1 && !p.clustered && p.splits * span_floats > A4_MAX_FLOATS) {
+        // (many row blocks beside a long request: nearly all of them are one span, but each has room for as many as the longest)
+        const long long most_spans = A4_MAX_FLOATS / span_floats > 1 ? A4_MAX_FLOATS / span_floats : 1;
+        p.span_tiles = (int)((longest + most_spans * A4_WARPS - 1) / (most_spans * A4_WARPS)) * A4_WARPS;
+        p.splits = (longest + p.span_tiles - 1) / p.span_tiles;
+    }
     return p;
 }
 
@@ -996,7 +1028,7 @@ static bool a4_by_codes(long long row_blocks, bool full, int hs) { return row_bl
 // What a step's portions ask for, from their lengths and first positions on the HOST: said[0] portions that attend to the codes, [1] ones that go through the
 // prompt kernels (of more than `most_rows` packed rows, all or none of them: a4_by_codes), [2] float32 values of scratch that xr_kv4_attention needs
 // for the first; of the others [3] the pages that xr_kv4_read writes for them, [4] the most tokens, [5], [6] the row tiles of 128 and 64 packed rows, [7] the
-// furthest end; [8] the most packed rows of a portion that attends to the codes; [9] .. [13] how those are cut, as xr_kv4_attention takes it.
+// furthest end; [8] the most packed rows of a portion that attends to the codes; [9] .. [14] how those are cut, as xr_kv4_attention takes it.
 // n: tokens of the step; max_kv: how far requests may get by the time the launches run (0: as far as the portions go); rule: whether a4_by_codes is asked, or
 // most_rows stands as it is (some portions of a step whose rule has been asked).
 XR_EXPORT int xr_kv4_plan(const int* len, const int* pos0, int n_seg, int n, int K, int G, int D, int page_size, int dtype, int window, int keep_first,
@@ -1004,7 +1036,7 @@ XR_EXPORT int xr_kv4_plan(const int* len, const int* pos0, int n_seg, int n, int
     if (n_seg < 1 || n < 0 || K < 1 || G < 1 || D < 1 || D > 256 || page_size < 1 || window < 0 || keep_first < 0 || most_rows < 0 || max_kv < 0) return XR_ERR_ARG;
     long long tokens = 0, row_blocks = 0;
     bool full = true;
-    for (int i = 0; i < 14; i++) said[i] = 0;
+    for (int i = 0; i < 15; i++) said[i] = 0;
     for (int s = 0; s < n_seg; s++) {
         const long long l = len[s], p = pos0[s], rows = l * G;
         if (l < 0 || p < 0 || p + l > 0x7fffffffLL) return XR_ERR_ARG;
@@ -1033,32 +1065,32 @@ XR_EXPORT int xr_kv4_plan(const int* len, const int* pos0, int n_seg, int n, int
     if (said[0] > 0) {
         const int hs = kv4_held(D), f32 = dtype == XR_F32;
         const A4Plan p = a4_plan(len, pos0, n_seg, K, G, hs, f32, window, window > 0 ? keep_first : 0, most_rows, max_kv);
-        said[9] = p.row_blocks; said[10] = p.wide; said[11] = p.span_tiles; said[12] = p.splits; said[13] = p.clustered;
-        if (p.splits > 1 && !p.clustered) said[2] = (long long)n_seg * K * p.row_blocks * p.splits * a4_rows(f32, p.wide) * (hs + 2);
+        said[9] = p.row_blocks; said[10] = p.wide; said[11] = p.span_tiles; said[12] = p.splits; said[13] = p.clustered; said[14] = p.blocks;
+        if (p.splits > 1 && !p.clustered) said[2] = (long long)p.blocks * K * p.splits * a4_rows(f32, p.wide) * (hs + 2);
     }
     return XR_OK;
 }
 
 // q: token t, head h at q + t * q_stride + h * D; out [n][H * D], both of `dtype`.  Portions of at most `most_rows` packed rows (tokens x heads per
-// kv head) are computed, longer ones passed over.  row_blocks, wide, span_tiles, splits, clustered: xr_kv4_plan's answer for the portions' lengths on the
+// kv head) are computed, longer ones passed over.  row_blocks, wide, span_tiles, splits, clustered, blocks: xr_kv4_plan's answer for the portions' lengths on the
 // host (they cut the work; what is computed goes by seg_len and seg_pos0 on the device, of at most row_blocks row blocks).  early: nothing that is still
 // running writes the portions, the block tables or rows before a portion's first.
 XR_EXPORT int xr_kv4_attention(const void* q, void* out, int dtype, const void* cache, long long n_pages, int layers, int layer, int K, int block, int page_size,
                                const int* seg_start, const int* seg_len, const int* seg_pos0, const int* block_tables, float* scratch, long long floats,
                                long long q_stride, int n_seg, int H, int D, int max_pages, int window, float scale, const float* sink, float softcap,
                                int keep_first, const float* bias, int bias_len, int most_rows, int early, int row_blocks, int wide, int span_tiles,
-                               int splits, int clustered, cudaStream_t stream) {
+                               int splits, int clustered, int blocks, cudaStream_t stream) {
     if (n_seg < 1 || n_seg > 65535 || H < 1 || K < 1 || H % K != 0 || max_pages < 1 || window < 0 || keep_first < 0 || !(scale > 0.f) || !(softcap >= 0.f) ||
         (bias != nullptr && (bias_len < 1 || softcap > 0.f)) || most_rows < 1 || q_stride < (long long)H * D || (dtype != XR_F32 && dtype != XR_BF16) ||
         !kv4_cache_ok(cache, n_pages, layers, layer, K, block, page_size, D) || (long long)max_pages * page_size > 0x7fffffffLL - 64 || row_blocks < 1 ||
-        span_tiles < 1 || splits < 1 || splits > A4_MAX_SPLITS || (clustered && splits > A4_CLUSTER) || (long long)splits * row_blocks > 0x7fffffffLL || (long long)K * row_blocks > 0x7fffffffLL)
+        span_tiles < 1 || blocks < 1 || splits < 1 || splits > A4_MAX_SPLITS || (clustered && splits > A4_CLUSTER) || (long long)splits * row_blocks > 0x7fffffffLL || (long long)K * row_blocks > 0x7fffffffLL)
         return XR_ERR_ARG;
     const int G = H / K, f32 = dtype == XR_F32, hs = kv4_held(D), keep = window > 0 ? keep_first : 0;
     const bool spans = splits > 1 && !clustered;
-    const long long items = spans ? (long long)n_seg * K * row_blocks * splits : 0, rb = a4_rows(f32, wide);
+    const long long items = spans ? (long long)blocks * K * splits : 0, rb = a4_rows(f32, wide);
     if (spans && (scratch == nullptr || ((uintptr_t)scratch & 15) || floats < items * rb * (hs + 2))) return XR_ERR_ARG;
     A4Args a{q, out, kv4_cache(cache, n_pages, layers, layer, K, page_size, D), seg_start, seg_len, seg_pos0, block_tables, scratch,
-             spans ? scratch + items * rb * hs : nullptr, q_stride, H, G, D, max_pages, window, keep, splits, span_tiles, row_blocks, most_rows,
+             spans ? scratch + items * rb * hs : nullptr, blocks, q_stride, H, G, D, max_pages, window, keep, splits, span_tiles, row_blocks, most_rows,
              scale, softcap, sink, {bias, bias_len}, 0, 0, early, clustered && splits > 1, -1};
     const int lot = f32 ? 4 : 8;                                     // elements of 16 bytes
     a.wide = D % 8 == 0 && q_stride % lot == 0 && !((uintptr_t)q & 15);

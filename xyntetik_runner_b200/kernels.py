@@ -889,7 +889,7 @@ _NP_I32 = np.dtype(np.int32)
 
 
 # what xr_kv4_plan says of a step's portions, in this order
-_PLAN = ("short", "long", "floats", "pages", "longest", "tiles_128", "tiles_64", "end", "most", "row_blocks", "wide", "span_tiles", "splits", "clustered")
+_PLAN = ("short", "long", "floats", "pages", "longest", "tiles_128", "tiles_64", "end", "most", "row_blocks", "wide", "span_tiles", "splits", "clustered", "blocks")
 
 
 def kv4_plan(lengths: tuple, n: int, kv_heads: int, group: int, head_dim: int, page_size: int, code: int, window: int, keep_first: int, most_rows: int,
