@@ -280,3 +280,11 @@ def test_scratch_of_steps_that_mix_portions_and_single_tokens(lens, ends, K, G, 
     assert said["splits"] > 1 and not said["clustered"] and said["blocks"] == sum(-(-n * G // rows) for n in lens)
     assert said["floats"] == said["blocks"] * K * said["splits"] * rows * (plain_kv4.held(D) + 2) <= 1 << 26
     assert said["splits"] * said["span_tiles"] * (64 if D <= 128 else 32) >= max(ends)
+
+
+@pytest.mark.parametrize("T,H,code,blocks", [(1, 8, 0, 148), (1, 16, 0, 148), (4, 32, 1, 148), (1, 32, 1, 296)])
+def test_spans_of_heads_of_256_elements_run_at_once(T, H, code, blocks):
+    """Equal requests that fit in one round are cut into one: an SM holds one block of sixteen rows or of float32, two of eight bfloat16 rows (148 SMs)."""
+    l, p = np.full(8, T, dtype=np.int32), np.full(8, 8192 - T, dtype=np.int32)
+    said = dict(zip(kernels._PLAN, kernels.kv4_plan((l, p), 8 * T, 8, H // 8, 256, 64, code, 0, 0, 1 << 30)))
+    assert said["splits"] > 1 and 8 * 8 * said["splits"] <= blocks

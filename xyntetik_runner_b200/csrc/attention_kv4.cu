@@ -228,8 +228,10 @@ template <int NG, int NT, bool F32, bool EXTRA> struct A4Shape {
     static constexpr int STAGE = TK * 2 * (CODES + SCALES);
     static constexpr int VW = NG / 2, MT = 4 * VW;                   // words of a value's row a thread takes; m-tiles of O^T
     static constexpr bool Q_REGS = KS * 2 * NT * P <= 48;            // q's fragments in registers, else in shared memory
-    static constexpr int BLOCKS = NG <= 4 && NT == 1 && !F32 ? 3 : 2;            // blocks an SM (registers, shared memory)
     static constexpr int SMEM = A4_WARPS * STAGES * STAGE + (Q_REGS ? 0 : P * NT * KS * 32 * 8) + 16;
+    // Blocks an SM: by registers, and by its 228 KB of shared memory, of which a block takes one more.  (Heads of 256 elements: two of eight bfloat16 rows, one of
+    // sixteen or of float32.)
+    static constexpr int BY_REGS = NG <= 4 && NT == 1 && !F32 ? 3 : 2, BY_SMEM = 228 * 1024 / (SMEM + 1024), BLOCKS = BY_REGS < BY_SMEM ? BY_REGS : BY_SMEM;
 };
 
 template <int NG, int NT, bool F32, bool EXTRA>
@@ -899,7 +901,12 @@ k_kv4_merge(A4Args a) {
 // ---------------------------------------------------------------------------------------------
 // Blocks that are resident at once, and a row block's size, for a head size and type.  wide_rows: some request has more than eight packed rows.
 static int a4_rows(int f32, int wide_rows) { return f32 || !wide_rows ? 8 : 16; }
-static int a4_resident(int hs, int f32, int wide_rows) { return (hs <= 128 && !f32 && !wide_rows ? 3 : 2) * xr_sm_count(); }
+template <int NG> static int a4_blocks(int f32, int wide_rows) {
+    return f32 ? A4Shape<NG, 1, true, false>::BLOCKS : wide_rows ? A4Shape<NG, 2, false, false>::BLOCKS : A4Shape<NG, 1, false, false>::BLOCKS;
+}
+static int a4_resident(int hs, int f32, int wide_rows) {
+    return (hs == 64 ? a4_blocks<2>(f32, wide_rows) : hs == 128 ? a4_blocks<4>(f32, wide_rows) : a4_blocks<8>(f32, wide_rows)) * xr_sm_count();
+}
 static int a4_tile(int hs) { return hs <= 128 ? 64 : 32; }
 
 // How a step is cut: row blocks of the longest portion that is taken (at most `most_rows` packed rows), tiles a span, spans of the longest
