@@ -288,3 +288,18 @@ def test_spans_of_heads_of_256_elements_run_at_once(T, H, code, blocks):
     l, p = np.full(8, T, dtype=np.int32), np.full(8, 8192 - T, dtype=np.int32)
     said = dict(zip(kernels._PLAN, kernels.kv4_plan((l, p), 8 * T, 8, H // 8, 256, 64, code, 0, 0, 1 << 30)))
     assert said["splits"] > 1 and 8 * 8 * said["splits"] <= blocks
+
+
+@pytest.mark.parametrize("requests,keys,reach,window,splits,cut", [
+    (64, 1000, 1024, 0, 1, "whole"), (64, 200, 1024, 0, 1, "whole"), (64, 8192, 8192, 0, 4, "spans"), (1, 8192, 8192, 0, 32, "spans"), (1, 100, 1024, 0, 4, "cluster"),
+    (1, 300, 1024, 0, 4, "cluster"), (8, 7300, 8192, 0, 6, "cluster"), (32, 5000, 5120, 1024, 1, "whole"), (1, 5000, 5120, 1024, 5, "cluster")])
+def test_captured_steps_are_cut_for_the_lengths_that_they_may_meet(requests, keys, reach, window, splits, cut):
+    """8 kv heads of 128 elements, single tokens: what is planned does not hang on the lengths at capture, and is what the longest lengths ask for."""
+    one = np.ones(requests, dtype=np.int32)
+    plan = lambda n, reach: dict(zip(kernels._PLAN, kernels.kv4_plan((one, np.full(requests, n - 1, dtype=np.int32)), requests, 8, 4, 128, 64, kernels.BF16, window, 0, 64, reach)))
+    said = plan(keys, reach)
+    assert said["splits"] == splits and ("whole" if splits == 1 else "cluster" if said["clustered"] else "spans") == cut
+    assert (said["floats"] > 0) == (cut == "spans")
+    assert all(plan(n, reach) == said for n in (max(1, reach - 1000), reach - 500, reach))
+    if not window:
+        assert plan(reach, 0) == said

@@ -910,7 +910,9 @@ static int a4_resident(int hs, int f32, int wide_rows) {
 static int a4_tile(int hs) { return hs <= 128 ? 64 : 32; }
 
 // How a step is cut: row blocks of the longest portion that is taken (at most `most_rows` packed rows), tiles a span, spans of the longest
-// request.  len, pos0: the portions on the HOST; max_kv: the longest key range to be prepared for (0: what the portions say).
+// request.  len, pos0: the portions on the HOST; max_kv: how far requests may get by the time the launch runs (0: as far as they say).  A captured launch is cut for
+// the lengths that it may meet: all portions as far on as brings the furthest to max_kv.  (Cut for the lengths at capture, 64 requests of 200 keys ran
+// up to 1,024 keys in four spans and a second kernel, where one span is planned for 1,024.)  Beyond the grid's spans the last one takes the rest.
 struct A4Plan { int row_blocks, wide, span_tiles, splits, clustered, blocks; };
 static A4Plan a4_plan(const int* len, const int* pos0, int n_seg, int K, int G, int hs, int f32, int window, int keep, int most_rows, int max_kv) {
     const int tile = a4_tile(hs);
@@ -924,11 +926,20 @@ static A4Plan a4_plan(const int* len, const int* pos0, int n_seg, int K, int G, 
     const int rb = a4_rows(f32, p.wide);
     p.row_blocks = (int)((rows + rb - 1) / rb);
     const long long resident = a4_resident(hs, f32, p.wide);
-    auto tiles_of = [&](int s) {                                     // (of the last row block, whose window is the furthest)
-        const int end = pos0[s] + len[s], lo = window > 0 ? (end - len[s] - window + 1 > 0 ? end - len[s] - window + 1 : 0) : 0;
-        return (end - 1) / tile - lo / tile + 1 + xr_kept_tiles(keep, lo, tile);
-    };
     auto taken = [&](int s) { return len[s] >= 1 && (long long)len[s] * G <= most_rows; };
+    int ahead = 0;
+    if (max_kv > 0) {
+        int furthest = 0;
+        for (int s = 0; s < n_seg; s++)
+            if (taken(s) && pos0[s] + len[s] > furthest) furthest = pos0[s] + len[s];
+        ahead = max_kv > furthest ? max_kv - furthest : 0;
+    }
+    auto tiles_of = [&](int s) {                                     // (of the last row block, whose window is the furthest)
+        const int end = pos0[s] + len[s] + ahead, lo = window > 0 ? (end - len[s] - window + 1 > 0 ? end - len[s] - window + 1 : 0) : 0;
+        // (a window that moves begins inside a tile nearly always)
+        const int seen = max_kv > 0 && lo > 0 ? (int)((end - (long long)lo + tile - 2) / tile) + 1 : (end - 1) / tile - lo / tile + 1;
+        return seen + xr_kept_tiles(keep, lo, tile);
+    };
     int longest = 1;
     for (int s = 0; s < n_seg; s++)
         if (taken(s)) { const int t = tiles_of(s); longest = t > longest ? t : longest; }
@@ -964,13 +975,6 @@ static A4Plan a4_plan(const int* len, const int* pos0, int n_seg, int K, int G, 
         if (work / resident > 1.5 * best_cost) break;
     }
     p.span_tiles = best * A4_WARPS;
-    if (max_kv > 0) {
-        // (a captured launch may meet requests up to this length; beyond the grid's spans the last one takes the rest)
-        const long long range = window > 0 && window + 16LL < max_kv ? window + 16LL : max_kv;
-        const long long t = (range + tile - 1) / tile + 1 + (window > 0 ? (keep + tile - 1LL) / tile : 0);
-        const long long more = best * (long long)A4_WARPS * (p.clustered ? A4_CLUSTER : A4_MAX_SPLITS);
-        longest = (int)(t > longest ? (t < more ? t : (more > longest ? more : longest)) : longest);
-    }
     p.splits = (longest + p.span_tiles - 1) / p.span_tiles;
     if (p.row_blocks > 1) {
         p.blocks = 0;
