@@ -303,3 +303,23 @@ def test_captured_steps_are_cut_for_the_lengths_that_they_may_meet(requests, key
     assert all(plan(n, reach) == said for n in (max(1, reach - 1000), reach - 500, reach))
     if not window:
         assert plan(reach, 0) == said
+
+
+def test_rows_on_pages_that_were_let_go_are_zeros():
+    """An engine without four bits: nothing of the page that stands in for a missing one, numbers or not; the cache stays as it is."""
+    from types import SimpleNamespace
+    from xyntetik_runner_b200.engine.engine import Engine
+    eng = Engine.__new__(Engine)
+    P, K, D = 4, 2, 3
+    eng.device, eng.act_dtype, eng.params = torch.device("cpu"), torch.float32, SimpleNamespace(page_size=P)
+    eng.model = SimpleNamespace(layers=[SimpleNamespace(group=0, layer_in_group=1)], groups=[SimpleNamespace(planes=2, kv_heads=K, head_dim=D)])
+    kv = torch.arange(3 * 2 * 2 * K * P * D, dtype=torch.float32).view(3, 2, 2, K, P, D)
+    kv[0, 1, 0], kv[0, 1, 1] = math.nan, math.inf
+    eng.kv, eng.four_bits = [kv], [False]
+    eng.cache = SimpleNamespace(length=lambda r: 10, block_table=lambda g, r: np.array([-1, 2, 1, -1], dtype=np.int32))
+    before = kv.clone()
+    k, v = eng.cached_rows("a", 0)
+    for rows, plane in ((k, 0), (v, 1)):
+        assert rows.shape == (10, K, D) and not rows[:4].any()
+        assert torch.equal(rows[4:8], kv[2, 1, plane].permute(1, 0, 2)) and torch.equal(rows[8:], kv[1, 1, plane, :, :2].permute(1, 0, 2))
+    assert torch.equal(torch.nan_to_num(kv), torch.nan_to_num(before))

@@ -294,7 +294,7 @@ class Engine:
             kernels.kv4_read(self.kv[lay.group], lay.layer_in_group, P, table, span[:1], span[1:], pages)
         else:
             ids = table[0, :-(-n // P)].long()
-            pages = self.kv[lay.group][ids.clamp(min=0), lay.layer_in_group] * (ids >= 0).view(-1, 1, 1, 1, 1)
+            pages = self.kv[lay.group][ids.clamp(min=0), lay.layer_in_group].masked_fill_((ids < 0).view(-1, 1, 1, 1, 1), 0.0)
         rows = pages.permute(1, 0, 3, 2, 4).reshape(2, pages.shape[0] * P, g.kv_heads, g.head_dim)
         return rows[0, :n], rows[1, :n]
 
