@@ -323,3 +323,29 @@ def test_rows_on_pages_that_were_let_go_are_zeros():
         assert rows.shape == (10, K, D) and not rows[:4].any()
         assert torch.equal(rows[4:8], kv[2, 1, plane].permute(1, 0, 2)) and torch.equal(rows[8:], kv[1, 1, plane, :, :2].permute(1, 0, 2))
     assert torch.equal(torch.nan_to_num(kv), torch.nan_to_num(before))
+
+
+def test_entries_that_can_and_that_cannot(monkeypatch):
+    """Mixers that cannot have their rows in four bits beside others that can: without four bits they share groups and caches as ever; with them a
+    cache is in four bits where everyone who writes or reads it can."""
+    from types import SimpleNamespace
+    from xyntetik_runner_b200.engine import model
+    from xyntetik_runner_b200.parts.base import KVNeed
+    mixer = lambda four, **k: SimpleNamespace(mixer=SimpleNamespace(kv_need=lambda: KVNeed(2, 64, four_bits=four, **k), state_need=lambda: None))
+    state = SimpleNamespace(mixer=SimpleNamespace(kv_need=lambda: None, state_need=lambda: None))
+    blocks = [mixer(True), mixer(False), mixer(True, window=9), mixer(True), state]
+    entry = model.ScheduleEntry
+    schedule = [entry(0), entry(1), entry(0), entry(1, cache_from=2), entry(2), entry(3), entry(4), entry(0, cache_from=1), entry(3, cache_from=5)]
+    plan = model.ModelPlan(None, blocks, schedule, None, None, 64, 10, 100)
+    plan.validate()
+    assert plan.four_bits() == [True, False, False, False, True, True, False, True, True]
+    monkeypatch.setattr(model.ModelPlan, "parts", lambda self: [])
+    monkeypatch.setattr(model, "load_tensors", lambda *a: {})
+    rt = SimpleNamespace(device="cpu")
+    same, four = model.LoadedModel(plan, None, rt), model.LoadedModel(plan, None, rt, four_bits=True)
+    # entries 0, 1, 2, 5 need the same; entry 4 has a window
+    assert [(g.n_layers, g.spec.window) for g in same.groups] == [(4, None), (1, 9)]
+    assert [(lay.group, lay.layer_in_group) for lay in same.layers] == [(0, 0), (0, 1), (0, 2), (0, 2), (1, 0), (0, 3), (-1, -1), (0, 1), (0, 3)]
+    assert [(g.n_layers, g.spec.window, g.four_bits) for g in four.groups] == [(2, None, True), (2, None, False), (1, 9, True)]
+    assert [lay.group for lay in four.layers] == [0, 1, 1, 1, 2, 0, -1, 1, 0]
+    assert same.kv_bytes_per_token(2) == 5 * 2 * 256 and four.kv_bytes_per_token(2, True) == 3 * 2 * 72 + 2 * 2 * 256

@@ -176,7 +176,7 @@ class Engine:
             self.config = config
         plan: ModelPlan = arch.build_plan(self.config)
         rt = Runtime(self.device, self.act_dtype, p.page_size, p.max_step_tokens, p.max_requests)
-        self.model = LoadedModel(plan, source, rt)
+        self.model = LoadedModel(plan, source, rt, four_bits=p.kv == "int4")
         self.plan = plan
         n_pages = max(1, -(-p.max_tokens // p.page_size))
         max_req = p.max_request_tokens or min(plan.max_positions, n_pages * p.page_size)

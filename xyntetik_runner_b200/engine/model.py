@@ -75,8 +75,17 @@ class ModelPlan:
                     raise ValueError(f"schedule entry {i}: cache_from must name an earlier entry that owns a cache")
                 a = self.blocks[e.layer].mixer.kv_need()
                 b = self.blocks[self.schedule[e.cache_from].layer].mixer.kv_need()
-                if a is None or b is None or (a.kv_heads, a.head_dim, a.planes, a.four_bits) != (b.kv_heads, b.head_dim, b.planes, b.four_bits):
+                if a is None or b is None or (a.kv_heads, a.head_dim, a.planes) != (b.kv_heads, b.head_dim, b.planes):
                     raise ValueError(f"schedule entry {i}: cannot read the cache of entry {e.cache_from} (geometry differs)")
+
+    def four_bits(self) -> List[bool]:
+        """By schedule entry: its mixer, and every one that reads the cache it owns, can have that in four bits."""
+        needs = [self.blocks[e.layer].mixer.kv_need() for e in self.schedule]
+        can = [need is not None and need.four_bits for need in needs]
+        for i, e in enumerate(self.schedule):
+            if e.cache_from is not None:
+                can[e.cache_from] = can[e.cache_from] and can[i]
+        return can
 
 
 @dataclass
@@ -96,7 +105,7 @@ class CacheGroupLayout:
     head_dim: int
     n_layers: int = 0
     planes: int = 2
-    four_bits: bool = False       # every mixer of the group can keep its rows in four bits
+    four_bits: bool = False       # every mixer that writes or reads the group's rows can have them in four bits
 
 
 def kv_head_bytes(need, elem_size: int, four_bits: bool) -> int:
@@ -110,7 +119,8 @@ def kv_head_bytes(need, elem_size: int, four_bits: bool) -> int:
 class LoadedModel:
     """Plan + tensors on the device + the cache layout the schedule implies."""
 
-    def __init__(self, plan: ModelPlan, source: TensorSource, rt: Runtime):
+    def __init__(self, plan: ModelPlan, source: TensorSource, rt: Runtime, four_bits: bool = False):
+        """`four_bits`: entries that can have their cache in four bits and others that need the same do not share a group."""
         plan.validate()
         self.plan, self.rt = plan, rt
         tensors = load_tensors(plan.tensor_specs(), source, rt.device)
@@ -121,6 +131,7 @@ class LoadedModel:
         self.layers: List[LayerRuntime] = []
         self.state_needs: List[Tuple[int, StateNeed]] = []
         keys: Dict[Tuple[int, int, Optional[int], int, int, bool], int] = {}
+        can = plan.four_bits()
         for i, e in enumerate(plan.schedule):
             mixer = plan.blocks[e.layer].mixer
             lay = LayerRuntime(entry=i)
@@ -130,13 +141,14 @@ class LoadedModel:
                     src = self.layers[e.cache_from]
                     lay.group, lay.layer_in_group, lay.writes_cache = src.group, src.layer_in_group, False
                 else:
-                    key = (need.kv_heads, need.head_dim, need.window, need.planes, need.keep_first, need.four_bits)
+                    key = (need.kv_heads, need.head_dim, need.window, need.planes, need.keep_first, four_bits and can[i])
                     if key not in keys:
                         keys[key] = len(self.groups)
                         name = "full" if need.window is None else f"window{need.window}" + (f"+{need.keep_first}" if need.keep_first else "")
                         self.groups.append(CacheGroupLayout(GroupSpec(f"{name}:{need.planes}x{need.kv_heads}x{need.head_dim}", need.window, need.keep_first),
-                                                            need.kv_heads, need.head_dim, planes=need.planes, four_bits=need.four_bits))
+                                                            need.kv_heads, need.head_dim, planes=need.planes, four_bits=True))
                     g = keys[key]
+                    self.groups[g].four_bits = self.groups[g].four_bits and can[i]
                     lay.group, lay.layer_in_group, lay.writes_cache = g, self.groups[g].n_layers, True
                     self.groups[g].n_layers += 1
             sn = mixer.state_need()

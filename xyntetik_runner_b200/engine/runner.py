@@ -169,10 +169,10 @@ class Runner:
             wbytes += n * wdt
         per_token = 0
         values = 0                                               # what a portion's rows are read back into, a layer at a time
-        for e in plan.schedule:
+        for e, can in zip(plan.schedule, plan.four_bits()):
             need = plan.blocks[e.layer].mixer.kv_need()
             if need is not None and e.cache_from is None:
-                in_four = kv == "int4" and need.four_bits
+                in_four = kv == "int4" and can
                 per_token += need.kv_heads * kv_head_bytes(need, elem, True) if in_four else 2 * need.kv_heads * need.head_dim * elem
                 if in_four and kernels.kv4_reads_back(torch.bfloat16 if elem == 2 else torch.float32, need.head_dim):
                     values = max(values, 2 * need.kv_heads * need.head_dim * elem)
