@@ -295,3 +295,27 @@ def test_partial_sums_of_portions_of_many_lengths(contexts, Ts, H, K, D, P, dtyp
         kernels.tc_check_status(torch.device(DEV))
         check_many(out, q, held, Ts, starts, pos0, H, D, dtype)
     assert torch.isnan(whole["kv4_spans"][said["floats"]:]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_pages_of_no_tokens_are_refused(dtype):
+    """A page size of 0 is a mistake, not another way to store: the rotation writes rows only where it is told to, and then the same keys and values."""
+    from xyntetik_runner_b200 import kernels
+    g = torch.Generator().manual_seed(3)
+    n, H, K, D, P = 5, 4, 2, 64, 8
+    qkv = torch.randn(n, (H + 2 * K) * D, generator=g).to(dtype).to(DEV)
+    pos, seg, bt = i32(np.arange(n)), i32(np.zeros(n)), i32([[0]])
+    freq = (10000.0 ** (-torch.arange(32) / 32.0))
+    pages, rows = torch.zeros(1, 2, K, P, D, dtype=dtype, device=DEV), torch.zeros(n, 2 * K * D, dtype=dtype, device=DEV)
+    turn = lambda cache, stride, v_at, page, **k: kernels.rope_store(qkv.clone(), pos, seg, bt, freq.to(DEV), cache.data_ptr(), stride, v_at, H, K, D, D, 1, page, **k)
+    norm = lambda cache, stride, v_at, page, **k: kernels.qk_norm_rope_store(
+        qkv, torch.zeros(n, H * D, dtype=dtype, device=DEV), pos, seg, bt, freq.double().to(DEV), None, None, cache.data_ptr(), stride, v_at, H, K, D, D, D, D, 1, page, False, 1e-5, **k)
+    for fn in (turn, norm):
+        for page in (0, -1):
+            with pytest.raises(kernels.KernelError, match="refuses these sizes"):
+                fn(pages, 2 * K * P * D, K * P * D, page)
+        assert not pages.any()
+        fn(pages, 2 * K * P * D, K * P * D, P)
+        fn(rows, 2 * K * D, K * D, P, to_rows=True)
+        assert torch.equal(pages[0, :, :, :n].permute(2, 0, 1, 3).reshape(n, -1), rows) and rows.any()
+        pages.zero_(), rows.zero_()

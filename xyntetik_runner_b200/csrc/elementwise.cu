@@ -179,8 +179,8 @@ XR_EXPORT int xr_rmsnorm(const float* x, const int* rows, const float* w, void* 
 // The cache of a layer group is [page][layer][K|V][kv head][token in page][hd];
 // `cache_k` points at this layer's K block of page 0.
 // ---------------------------------------------------------------------------
-// Where token t's K heads go, and how far they lie apart: into its page, or with page_size 0 into rows, one a token, page_stride apart with
-// the heads side by side (another kernel takes them from there).
+// Where token t's K heads go, and how far they lie apart: into its page, or (to_rows, which the launchers hand on as a page_size of 0) into rows, one a
+// token, page_stride apart with the heads side by side (another kernel takes them from there).
 template <typename T>
 __device__ __forceinline__ T* xr_store_row(void* cache_k, const int* block_tables, const int* tok_seg, int t, int pos, int max_pages, int page_size,
                                            long long page_stride, int hd) {
@@ -322,12 +322,12 @@ k_rope_store_vec(RopeStoreArgs a) {
 XR_EXPORT int xr_rope_store(void* qkv, int dtype, const int* positions, const int* tok_seg, const int* block_tables,
                             const float* inv_freq, void* cache_k, long long page_stride, long long v_offset,
                             int n, int H, int K, int hd, int rotary_dim, int max_pages, int page_size,
-                            int adjacent_pairs, float mscale, cudaStream_t stream) {
+                            int adjacent_pairs, float mscale, int to_rows, cudaStream_t stream) {
     if (n < 1 || H < 1 || K < 1 || hd < 1 || rotary_dim < 0 || rotary_dim > hd || (rotary_dim & 1) ||
-        page_size < 0 || H + 2 * K > 65535)
+        (page_size < 1 && !to_rows) || H + 2 * K > 65535)
         return XR_ERR_ARG;
     RopeStoreArgs a{qkv, positions, tok_seg, block_tables, inv_freq, cache_k, page_stride, v_offset,
-                    n, H, K, hd, rotary_dim, max_pages, page_size, adjacent_pairs ? 1 : 0, mscale};
+                    n, H, K, hd, rotary_dim, max_pages, to_rows ? 0 : page_size, adjacent_pairs ? 1 : 0, mscale};
     int threads = 256;
     if (dtype == XR_BF16 && (hd & 7) == 0 && (rotary_dim & 15) == 0 && ((uintptr_t)qkv & 15) == 0 &&
         (cache_k == nullptr || ((((uintptr_t)cache_k) & 15) == 0 && (page_stride & 7) == 0 && (v_offset & 7) == 0))) {
@@ -697,16 +697,16 @@ XR_EXPORT int xr_qk_norm_rope_store(const void* in, int dtype, long long ld_in, 
                                     void* cache_k, long long page_stride, long long v_offset, int n, int H, int K, int D, int Vd, int hd,
                                     int rotary_dim, int max_pages, int page_size, int adjacent_pairs, float eps, int unit_norm,
                                     float q_coef, int q_every, const float* partial, int splits, const float* bias, int cols,
-                                    float mscale, int norm_after, void* v_first, int v_mix, float v_lambda, cudaStream_t stream) {
+                                    float mscale, int norm_after, void* v_first, int v_mix, float v_lambda, int to_rows, cudaStream_t stream) {
     if (v_mix < 0 || v_mix > 2 || (v_mix != 0 && (v_first == nullptr || cache_k == nullptr || ((uintptr_t)v_first & 15)))) return XR_ERR_ARG;
     if (partial != nullptr && (splits < 1 || D > 256 || cols < (H + K) * D + K * Vd || cols > ld_in)) return XR_ERR_ARG;
     if (n < 1 || H < 1 || K < 1 || D < 1 || Vd < 1 || hd < D || hd < Vd || rotary_dim < 0 || rotary_dim > D || (rotary_dim & 1) ||
-        page_size < 0 || (rotary_dim > 0 && freq == nullptr) || (q_w == nullptr) != (k_w == nullptr) || q_every < 0 ||
+        (page_size < 1 && !to_rows) || (rotary_dim > 0 && freq == nullptr) || (q_w == nullptr) != (k_w == nullptr) || q_every < 0 ||
         (unit_norm && q_w != nullptr) || (norm_after && !unit_norm))
         return XR_ERR_ARG;
     const int pairs = !((D | hd | ld_in | q_ld | page_stride) & 1) && !(((uintptr_t)in | (uintptr_t)q_out | (uintptr_t)cache_k) & 3);
     QkNormStoreArgs a{in, ld_in, q_out, q_ld, positions, tok_seg, block_tables, freq, q_w, k_w, cache_k, page_stride, v_offset,
-                      H, K, D, Vd, hd, rotary_dim, max_pages, page_size, adjacent_pairs ? 1 : 0, eps, pairs, unit_norm ? 1 : 0,
+                      H, K, D, Vd, hd, rotary_dim, max_pages, to_rows ? 0 : page_size, adjacent_pairs ? 1 : 0, eps, pairs, unit_norm ? 1 : 0,
                       q_coef, q_every, partial, bias, splits, cols, n, mscale, norm_after ? 1 : 0, v_first, v_mix, v_lambda};
     const size_t smem = ((size_t)rotary_dim + 8 * (size_t)D) * sizeof(float);
     if (smem > 48 * 1024) return XR_ERR_ARG;

@@ -182,8 +182,8 @@ def rmsnorm(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, eps: float, row
 
 def rope_store(qkv: torch.Tensor, positions, tok_seg, block_tables, inv_freq: Optional[torch.Tensor],
                cache_k_ptr: Optional[int], page_stride: int, v_offset: int, H: int, K: int, hd: int,
-               rotary_dim: int, max_pages: int, page_size: int, adjacent: bool = False, mscale: float = 1.0) -> None:
-    """Rotate Q in place, rotate K and store K, V into their pages (cache_k_ptr None: store nothing; page_size 0: into rows, token t's K heads
+               rotary_dim: int, max_pages: int, page_size: int, adjacent: bool = False, mscale: float = 1.0, to_rows: bool = False) -> None:
+    """Rotate Q in place, rotate K and store K, V into their pages (cache_k_ptr None: store nothing; `to_rows`: not into pages, but token t's K heads
     at cache_k_ptr + t * page_stride elements, side by side, and its V heads `v_offset` elements further).  Pair j of
     a head is elements (j, j + rotary_dim/2), or (2j, 2j + 1) with `adjacent`; cosines and sines are multiplied
     by `mscale` (src/model.c:3514-3532)."""
@@ -193,7 +193,7 @@ def rope_store(qkv: torch.Tensor, positions, tok_seg, block_tables, inv_freq: Op
     assert rotary_dim == 0 or (inv_freq is not None and inv_freq.dtype == torch.float32 and inv_freq.numel() >= rotary_dim // 2)
     _check(_c.xr_rope_store(qkv.data_ptr(), dtype_code(qkv.dtype), positions.data_ptr(), tok_seg.data_ptr(),
                                block_tables.data_ptr(), _ptr(inv_freq), cache_k_ptr, page_stride, v_offset,
-                               n, H, K, hd, rotary_dim, max_pages, page_size, int(adjacent), float(mscale), _stream()),
+                               n, H, K, hd, rotary_dim, max_pages, page_size, int(adjacent), float(mscale), int(to_rows), _stream()),
            "rope_store")
     _count()
 
@@ -220,11 +220,11 @@ def qk_norm_rope_store(inp: torch.Tensor, q_out: torch.Tensor, positions, tok_se
                        H: int, K: int, D: int, Vd: int, hd: int, rotary_dim: int, max_pages: int, page_size: int, adjacent: bool,
                        eps: float, unit_norm: bool = False, q_coef: float = 0.0, q_every: int = 0, partial: Optional[torch.Tensor] = None,
                        splits: int = 0, bias: Optional[torch.Tensor] = None, mscale: float = 1.0, norm_after: bool = False,
-                       v_first: Optional[torch.Tensor] = None, v_lambda: Optional[float] = None) -> None:
+                       v_first: Optional[torch.Tensor] = None, v_lambda: Optional[float] = None, to_rows: bool = False) -> None:
     """inp [n, >= (H + K) D + K Vd] (rows may be strided): Q heads, K heads (D each), V heads (Vd each).  Every Q and K head is
     RMS-normed with the weight q_w / k_w (float32 [D], shared by the heads; None: no norm), its first `rotary_dim` elements rotated
     (freq: float64 [rotary_dim / 2]); Q goes to q_out [n, *] (head h at column h * hd), K and V into the token's cache rows, every
-    head filled up to `hd` elements with zeros (cache_k_ptr None: nothing is stored; page_size 0: into rows, see ``rope_store``).  `unit_norm` (with no weights): every Q
+    head filled up to `hd` elements with zeros (cache_k_ptr None: nothing is stored; `to_rows`: see ``rope_store``).  `unit_norm` (with no weights): every Q
     and K head is divided by its root mean square all the same.  `q_every` > 0: the Q heads of the token at position p are
     multiplied by 1 + q_coef ln(floor((p + 1) / q_every) + 1).  `partial` (float32 [splits][n][inp.shape[1]], with `bias`): the rows are
     still the partial sums of a product cut along K; the kernel sums them (+ bias) into `inp`, every column, before it reads them.
@@ -246,7 +246,7 @@ def qk_norm_rope_store(inp: torch.Tensor, q_out: torch.Tensor, positions, tok_se
                                        int(adjacent), float(eps), int(unit_norm), float(q_coef), int(q_every), _ptr(partial), int(splits),
                                        _ptr(bias) if partial is not None else None, inp.shape[1], float(mscale), int(norm_after),
                                        _ptr(v_first), 0 if v_first is None else (1 if v_lambda is None else 2), float(v_lambda or 0.0),
-                                       _stream()),
+                                       int(to_rows), _stream()),
            "qk_norm_rope_store")
     _count()
 

@@ -241,18 +241,17 @@ class GQAAttention(Mixer):
         qkv = ctx.buf("attn_qkv", (n, qkv_dim), ctx.act_dtype)
         bt = ctx.block_tables[lay.group]
         four = ctx.cache_four_bits(lay)
-        page_size = ctx.page_size
         if four is None:
             k_ptr, page_stride, v_offset = ctx.cache_layer(lay)
         elif self.general:
             # rows of keys and values, which kernels.kv4_store then takes: beside the queries, in their own array
             rows = ctx.buf("attn_kv_rows", (n, 2 * self.K * self.hd), ctx.act_dtype)
             k_rows, v_rows = rows[:, :self.K * self.hd], rows[:, self.K * self.hd:]
-            k_ptr, page_stride, v_offset, page_size = rows.data_ptr(), rows.shape[1], self.K * self.hd, 0
+            k_ptr, page_stride, v_offset = rows.data_ptr(), rows.shape[1], self.K * self.hd
         else:
             # ... or where the projection left them
             k_rows, v_rows = qkv[:, self.H * self.hd:(self.H + self.K) * self.hd], qkv[:, (self.H + self.K) * self.hd:]
-            k_ptr, page_stride, v_offset, page_size = k_rows.data_ptr(), qkv_dim, self.K * self.hd, 0
+            k_ptr, page_stride, v_offset = k_rows.data_ptr(), qkv_dim, self.K * self.hd
         store_ptr = k_ptr if lay.writes_cache else None
         rot_dim, rot_freq, adjacent, mscale = self.rot
         if self.general:
@@ -270,10 +269,10 @@ class GQAAttention(Mixer):
             coef, every = self.q_temp if self.q_temp is not None else (0.0, 0)
             kernels.qk_norm_rope_store(proj, qkv, ctx.positions, ctx.tok_seg, bt, self.freq64, self.q_norm_w, self.k_norm_w, store_ptr,
                                        page_stride, v_offset, self.H, self.K, self.D, self.Vd, self.hd, rot_dim, ctx.max_pages,
-                                       page_size, adjacent, self.norm_eps, self.unit_norm, coef, every,
+                                       ctx.page_size, adjacent, self.norm_eps, self.unit_norm, coef, every,
                                        partial=None if pend is None else pend.partial, splits=0 if pend is None else pend.splits,
                                        bias=None if pend is None else pend.bias, mscale=mscale, norm_after=self.norm_after,
-                                       v_first=v_first, v_lambda=self.v_lambda)
+                                       v_first=v_first, v_lambda=self.v_lambda, to_rows=four is not None)
             if pend is not None:
                 pend.release()
         else:
@@ -288,7 +287,7 @@ class GQAAttention(Mixer):
                 if pend is not None:
                     pend.finish()
                 kernels.rope_store(qkv, ctx.positions, ctx.tok_seg, bt, rot_freq, store_ptr, page_stride,
-                                   v_offset, self.H, self.K, self.hd, rot_dim, ctx.max_pages, page_size, adjacent, mscale)
+                                   v_offset, self.H, self.K, self.hd, rot_dim, ctx.max_pages, ctx.page_size, adjacent, mscale, to_rows=four is not None)
         if four is not None and lay.writes_cache:
             kernels.kv4_store(k_rows, v_rows, ctx.positions, ctx.tok_seg, bt, four, lay.layer_in_group, ctx.page_size)
         o = ctx.buf("attn_out", (n, self.H * self.hd), ctx.act_dtype)
