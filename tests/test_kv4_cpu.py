@@ -349,3 +349,13 @@ def test_entries_that_can_and_that_cannot(monkeypatch):
     assert [(g.n_layers, g.spec.window, g.four_bits) for g in four.groups] == [(2, None, True), (2, None, False), (1, 9, True)]
     assert [lay.group for lay in four.layers] == [0, 1, 1, 1, 2, 0, -1, 1, 0]
     assert same.kv_bytes_per_token(2) == 5 * 2 * 256 and four.kv_bytes_per_token(2, True) == 3 * 2 * 72 + 2 * 2 * 256
+
+
+def test_the_plain_implementation_has_no_cache_to_keep_in_four_bits(tmp_path, capsys):
+    import tiny
+    from xyntetik_runner_b200.cli import main
+    folder = tiny.make_folder(str(tmp_path / "a"), "A")
+    assert main(["-m", folder, "-p", "ids:7,8", "-n", "2", "--ref", "--kv", "int4"]) == 2
+    said = capsys.readouterr()
+    assert "--kv int4" in said.err and said.out == ""
+    assert main(["-m", folder, "-p", "ids:7,8", "-n", "2", "--ref", "--kv", "same", "--ignore-eos"]) == 0

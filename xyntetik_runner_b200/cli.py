@@ -100,6 +100,9 @@ def run_plain(args) -> int:
     if args.temp > 0 or args.score or args.bench_json:
         print("error: --ref decodes greedily only (no --temp, --score or --bench-json)", file=sys.stderr)
         return 2
+    if args.kv != "same":
+        print(f"error: --ref keeps no cache (no --kv {args.kv})", file=sys.stderr)
+        return 2
     if args.threads:
         import torch
         torch.set_num_threads(args.threads)
