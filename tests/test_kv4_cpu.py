@@ -359,3 +359,11 @@ def test_the_plain_implementation_has_no_cache_to_keep_in_four_bits(tmp_path, ca
     said = capsys.readouterr()
     assert "--kv int4" in said.err and said.out == ""
     assert main(["-m", folder, "-p", "ids:7,8", "-n", "2", "--ref", "--kv", "same", "--ignore-eos"]) == 0
+
+
+def test_lengths_that_are_no_arrays():
+    """Lists, tensors, one array alone: refused as what they are, not by what they lack."""
+    a = np.array([1, 2], dtype=np.int32)
+    for l, p in (([1, 2], [0, 0]), (torch.tensor([1, 2], dtype=torch.int32), torch.zeros(2, dtype=torch.int32)), (a, [0, 0]), (None, None)):
+        with pytest.raises(kernels.KernelError, match="two int32 numpy arrays"):
+            kernels.kv4_plan((l, p), 9, 2, 4, 64, 16, kernels.BF16, 0, 0, 64)

@@ -899,7 +899,7 @@ def kv4_plan(lengths: tuple, n: int, kv_heads: int, group: int, head_dim: int, p
     tokens of the longest, their row tiles of 128 and 64 rows, and the end of the furthest; the most rows of one that attends to the codes; then how those are
     cut, as the launcher takes it.  `rule` False: `most_rows` stands, whatever the portions would cost either way.  Raises where they do not fit `n` tokens."""
     h_len, h_pos = lengths
-    if h_len.dtype != _NP_I32 or h_pos.dtype != _NP_I32 or h_len.ndim != 1 or h_len.shape != h_pos.shape:
+    if not isinstance(h_len, np.ndarray) or not isinstance(h_pos, np.ndarray) or h_len.dtype != _NP_I32 or h_pos.dtype != _NP_I32 or h_len.ndim != 1 or h_len.shape != h_pos.shape:
         raise KernelError("lengths: two int32 numpy arrays, one value a portion")
     said = array("q", (0,) * len(_PLAN))
     if _c.xr_kv4_plan(h_len, h_pos, h_len.size, n, kv_heads, group, head_dim, page_size, code, window, keep_first, most_rows, max_kv_len, int(rule), said) != 0:
@@ -971,7 +971,7 @@ def attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, layer
     args = _kv4_args(cache, layer, page_size, head_dim)
     code = dtype_code(dtype)
     G = heads // K
-    if lengths[0].size != n_seg:
+    if len(lengths) != 2 or not isinstance(lengths[0], np.ndarray) or lengths[0].size != n_seg:
         raise KernelError("lengths: two int32 numpy arrays, one value a portion")
     # portions that the prompt kernels take: bfloat16 on 16-byte borders, head sizes that one of them has
     aligned = kv4_reads_back(dtype, head_dim) and q_row % 8 == 0 and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0
