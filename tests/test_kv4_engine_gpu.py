@@ -248,3 +248,81 @@ def test_command_line(tmp_path):
     a = subprocess.run(cmd, cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert a.returncode == 0, a.stderr
     assert a.stdout.startswith("ids:") and len(a.stdout.split("\n")[0].split(",")) == 5
+
+
+def long_engine(dtype, kv, layers, graphs, model="llama", max_tokens=6144):
+    from xyntetik_runner_b200 import architectures  # noqa: F401
+    from xyntetik_runner_b200.config import registry
+    from xyntetik_runner_b200.engine.engine import EngineParams, random_engine
+    c = llama(128, 6, 2, layers=layers) if model == "llama" else MODELS[model]()
+    arch = registry.resolve(registry.architecture_name(c))
+    return random_engine(arch.config_from_dict(c), 7, EngineParams(dtype=dtype, max_tokens=max_tokens, page_size=64, max_requests=4, max_request_tokens=4096,
+                                                                   max_step_tokens=1024, cuda_graphs=graphs, kv=kv), std=0.08)
+
+
+def long_run(eng, vocab=250):
+    """Three requests of 300 to 3,000 tokens and a fourth that takes the second's pages; single tokens, a few, and none but one request's, in between."""
+    from xyntetik_runner_b200.engine.engine import StepEntry
+    rng = np.random.RandomState(5)
+    out = []
+
+    def step(**tokens):
+        entries = [StepEntry(r, [int(t) for t in rng.randint(0, vocab, n)], list(range(max(0, n - 3), n))) for r, n in tokens.items()]
+        out.append(eng.step(entries).clone())
+    step(a=1000), step(a=900, b=100), step(a=1000, b=24), step(b=900), step(c=300)
+    for _ in range(6):
+        step(a=1, b=1, c=1)
+    step(a=4, b=1, c=2)
+    pages = set(eng.cache.block_table(0, "b").tolist()) - {-1}
+    eng.end("b")
+    step(d=1000), step(a=1, d=30)
+    assert set(eng.cache.block_table(0, "d").tolist()) & pages        # (pages of the one that ended)
+    for _ in range(6):
+        step(a=1, c=1, d=1)
+    for r in "ac":
+        step(**{r: 1}), step(**{r: 1}), step(**{r: 1})
+    eng.check_status()
+    return out
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("layers,graphs", [(1, True), (1, False), (2, True)])
+def test_long_requests_against_quantised_pages(dtype, layers, graphs, monkeypatch):
+    """Requests whose keys are cut into spans that meet in a cluster or through a second kernel, read ahead of the kernel before.  One layer: its rows are the plain
+    form's bit for bit, so that logits are as near as the arithmetic (float32: 1e-4 of the largest, which a span that is lost or read too soon is not)."""
+    from xyntetik_runner_b200 import kernels
+    cuts, real = set(), kernels.kv4_plan
+
+    def plan(*a, **k):
+        said = real(*a, **k)
+        if said[0]:
+            cuts.add((said[12] > 1, bool(said[13])))
+        return said
+    eng = long_engine(dtype, "int4", layers, graphs)
+    with monkeypatch.context() as m:
+        m.setattr(kernels, "kv4_plan", plan)
+        got = long_run(eng)
+    assert {(True, True), (True, False)} <= cuts and (eng.graph_replays > 0) == graphs
+    ref = long_engine(dtype, "same", layers, False)
+    with monkeypatch.context() as m:
+        quantise_pages(ref, m)
+        want = long_run(ref)
+    differ = total = 0
+    for r in "acd":
+        for i, (x, y) in enumerate(zip(rows_of(eng, r), rows_of(ref, r))):
+            assert x.shape == y.shape and (i > 0 or torch.equal(x, y))
+            differ, total = differ + int((x != y).sum()), total + x.numel()
+    assert differ <= (0 if layers == 1 else 1e-4 * total if dtype == "float32" else 0.1 * total)
+    for a, b in zip(got, want):
+        scale, off = float(b.abs().max()), float((a - b).abs().max())
+        if dtype == "float32":
+            assert off <= (1e-4 if differ == 0 else 0.02) * scale, f"{off / scale:.3g}"
+        else:
+            # (see test_engine_against_quantised_pages)
+            rel = float((a - b).norm() / b.norm())
+            assert rel <= 2.0 ** -6 + 0.31 * math.sqrt(differ / total * 2 * layers), f"{rel:.3g}, {differ} of {total}"
+    if graphs:
+        plain = long_run(long_engine(dtype, "int4", layers, False))
+        for a, b in zip(got, plain):
+            # (the same kernels, cut for other lengths at times: sums in another order)
+            assert float((a - b).abs().max()) <= (1e-4 if dtype == "float32" else 0.05) * float(b.abs().max())

@@ -319,3 +319,51 @@ def test_pages_of_no_tokens_are_refused(dtype):
         fn(rows, 2 * K * D, K * D, P, to_rows=True)
         assert torch.equal(pages[0, :, :, :n].permute(2, 0, 1, 3).reshape(n, -1), rows) and rows.any()
         pages.zero_(), rows.zero_()
+
+
+@pytest.mark.parametrize("H,K,D,P,dtype,contexts,T,window,keep", [
+    (8, 2, 128, 64, BF16, [2500, 300, 700], 1, 0, 0), (8, 8, 64, 16, BF16, [2500, 300, 700], 1, 0, 0), (8, 2, 64, 64, F32, [2500, 300, 700], 1, 0, 0),
+    (2, 1, 64, 64, BF16, [9000, 40], 1, 0, 0), (8, 2, 128, 16, BF16, [3000, 1100], 1, 900, 70), (8, 2, 100, 24, BF16, [1200, 500], 3, 0, 0), (4, 2, 256, 64, F32, [900] * 3, 2, 0, 0)])
+def test_rows_of_earlier_steps_read_ahead_of_the_kernel_before(H, K, D, P, dtype, contexts, T, window, keep):
+    """Steps as an engine queues them: a copy of the positions, a store of the step's own rows, the attention, which may read earlier rows at once.  The same bits as
+    a call that waits, whose last step is compared with the plain form."""
+    from xyntetik_runner_b200 import kernels
+    steps, R = 12, len(contexts)
+    ends = [c + steps * T for c in contexts]
+    args, _, held, plain, *_ = attention_case(ends, T, H, K, D, P, dtype, 0, 0, 0, 0, 0)
+    args.update(window=window, keep_first=keep)
+    plain.update(window=window, keep=keep)
+    g = torch.Generator().manual_seed(8)
+    new = [torch.randn(steps, R * T, K * D, generator=g).to(dtype) for _ in (0, 1)]
+    q = torch.randn(steps, R * T, H * D, generator=g).to(dtype)
+    starts = np.repeat(contexts, T) + np.tile(np.arange(T), R)
+    flat = [torch.from_numpy((starts + s * T).astype(np.int32)).pin_memory() for s in range(steps)]
+    first = [torch.from_numpy((np.array(contexts) + s * T).astype(np.int32)).pin_memory() for s in range(steps)]
+    seg = i32(np.repeat(np.arange(R), T))
+    one = np.full(R, T, dtype=np.int32)
+    new_d, q_d, clean, cuts = [x.to(DEV) for x in new], q.to(DEV), args["cache"].clone(), set()
+    outs = {}
+    for early in (False, True):
+        args["cache"].copy_(clean)
+        # (what lies where the steps' rows go: anything)
+        out = torch.full((steps, R * T, H * D), 9.0, dtype=dtype, device=DEV)
+        pos, pos0 = i32(starts), i32(contexts)
+        torch.cuda.synchronize()
+        for s in range(steps):
+            pos.copy_(flat[s], non_blocking=True)
+            pos0.copy_(first[s], non_blocking=True)
+            kernels.kv4_store(new_d[0][s], new_d[1][s], pos, seg, args["block_tables"], args["cache"], args["layer"], P)
+            lengths = one, first[s].numpy()
+            said = dict(zip(kernels._PLAN, kernels.kv4_plan(lengths, R * T, K, H // K, D, P, kernels.dtype_code(dtype), window, keep, 1 << 30, max(ends))))
+            cuts.add((said["splits"] > 1, bool(said["clustered"])))
+            kernels.attention_kv4(q_d[s], out[s], **{**args, "seg_pos0": pos0, "lengths": lengths}, max_kv_len=max(ends), early=early)
+        torch.cuda.synchronize()
+        outs[early] = out
+    assert cuts <= {(True, True), (True, False)} and torch.equal(outs[True], outs[False])
+    full = []
+    for r, (c, e) in enumerate(zip(contexts, ends)):
+        for plane in (0, 1):
+            x = held[2 * r + plane].clone()
+            x[c:] = plain_kv4.quantised_rows(new[plane][:, r * T:(r + 1) * T].reshape(steps * T, K, D))
+            full.append(x)
+    check(outs[True][-1], q[-1], full, plain, [T] * R, np.arange(R) * T, np.array(ends) - T, H, D, dtype)
