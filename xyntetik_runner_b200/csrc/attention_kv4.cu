@@ -31,7 +31,7 @@
 // peak (6.54 TB/s), and as long where the cache fits in L2, with issue slots 44 to 62 % and the integer pipe 35 to 57 % busy and the tensor cores at 19 %: what
 // is left is warps waiting for one another's results.  Around that stand what a launch costs before its first tiles are there (about 9 us
 // with all SMs' first tiles on their way at once, 5.6 with a few) and what the last round of blocks leaves idle.
-// Measured and left: four blocks an SM (64 ragged requests of 40 heads 253 us against 214: registers spill), tiles of 32 keys at three (230), the next tile's scores
+// Measured and left: four blocks an SM (64 ragged requests of 40 heads 253 us against 214: 128 registers a thread, where three leave 168 and spill 36 bytes), tiles of 32 keys at three (230), the next tile's scores
 // interleaved with this tile's values (55 requests of 8,192 keys 119.9 against 107.8), bulk copies instead of cp.async (equal), e4m3 operands (the
 // instruction runs at 0.16 a cycle and SM), equal shares of all tiles for resident blocks (268 and a second kernel against 214).
 //

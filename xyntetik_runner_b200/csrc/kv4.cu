@@ -1,5 +1,5 @@
 // Writing rows of keys and values into a cache in four bits, and reading them back (the layout and its numbers: kv4.cuh).
-// The reference's counterpart is its cache in eight bits (`--kv q8_0`; k_store_kv, src/kernels.cu:2008-2022); the format here is its own.
+// The reference's counterpart is its cache in eight bits (`--kv q8_0`; k_store_kv, src/kernels.cu:2008-2022).
 #include "kv4.cuh"
 #include <math.h>
 

@@ -1,4 +1,5 @@
-// How a cache in four bits holds keys and values.
+// How a cache in four bits holds keys and values.  (A scale from the signed element of largest magnitude is the idea of the q4_0 format; a scale of five
+// bits, which makes every held value a bfloat16, and the bytes' order are this format's own.)
 //
 // A group is 32 neighbouring elements of one token's head; a head of D elements is held as 64, 128 or 256 of them, zeros behind D.
 // With e the group's element of largest magnitude (the positive one of two), s = -e / 8, e rounded to five significant bits (ties

@@ -9,7 +9,8 @@ this -- ``model_forward_batch`` (n consecutive tokens of one sequence, logits
 of the last, src/model.h:667-670) and ``model_batch_decode`` (one token of each
 of n sequences, src/model.h:796-807) -- and carries the rule that a token's
 result must not depend on what else is in the batch (src/gpu.h:127-131); that
-rule holds here for any mixture.
+rule holds here for any mixture, up to the rounding of the kernels that a step's
+sizes choose.
 
 All token-parallel work (norms, products, rotation, SwiGLU) runs on the flat
 token axis; attention runs per token over its request's block table with the

@@ -942,7 +942,8 @@ def attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, layer
     head_dim] (bfloat16 or float32, strided by rows), out [n, heads * head_dim]; portion s is the seg_len[s] rows from seg_start[s] on, at positions
     seg_pos0[s] .., over row s of the block tables.  `lengths` = (seg_len, seg_pos0) on the host (numpy int32): they size the launches; a call
     that is captured in a graph may be replayed with other positions but the same seg_len (say in `max_kv_len` how long the requests may get: the
-    cut suits that, and scratch for rows read back holds that much; 0: as much as the block tables name).  Rows on a page that is not held count as zeros.  Options: see ``attention_simt``.
+    cut suits that, and scratch for rows read back holds that much; 0: as much as the block tables name).  Rows on a page that is not held count as zeros.  Options: see ``attention_simt`` (a bias of
+    the lowest number on every key that a row sees gives the keys' average by the codes, but not through the prompt kernels).
     Single tokens, short portions and whatever the prompt kernels do not take attend to the codes; where longer portions are many rows, they read the
     rows they see back, a few requests at a time (KV4_VALUES_BYTES), into `buf` (``buf(name, shape, dtype)`` gives scratch; None: allocated) and go through the prompt kernels.  `early`: the caller says that
     nothing still running writes the portions, the block tables or rows ahead of a portion's first (an engine's step); they may then be read before
