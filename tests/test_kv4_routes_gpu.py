@@ -249,6 +249,8 @@ def test_rows_read_back_a_few_requests_at_a_time(H, K, D, P, captured, monkeypat
     from xyntetik_runner_b200 import kernels
     contexts, Ts = [400, 90, 300, 5, 700, 200, 120], [100, 1, 60, 5, 90, 0, 120]
     args, q, held, plain, Ts, starts, pos0 = attention_case(contexts, Ts, H, K, D, P, BF16, 0, 0, 0, 0, 0)
+    if captured:
+        args.update({name: args[name].view(1, -1) for name in ("seg_start", "seg_len", "seg_pos0")})       # (so many values, whatever their shape)
     qd, outs, asked = q.to(DEV), [], []
     for pages in (10 ** 6, 9, 1):
         monkeypatch.setattr(kernels, "KV4_VALUES_BYTES", pages * 4 * K * P * D)

@@ -883,7 +883,7 @@ def kv4_read(cache: torch.Tensor, layer: int, page_size: int, block_tables: torc
 KV4_SHORT_ROWS = 64
 _KV4_ALL_ROWS = 1 << 30
 # Bytes of rows that are read back at once (what the latent attention takes for its expanded rows, too): the portions of a step that see more go a few
-# requests at a time, one request at least.  65,536 rows of 8 kv heads of 128 elements.
+# requests at a time, one request at least.  131,072 rows of 8 kv heads of 128 elements.
 KV4_VALUES_BYTES = 1 << 29
 _NP_I32 = np.dtype(np.int32)
 
@@ -1000,7 +1000,9 @@ def attention_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, layer
         half = K * page_size * head_dim
         for a, b, pages, longest, tiles_128, tiles_64, end in groups:
             s = b - a
-            starts, lens, pos0, bt = (seg_start, seg_len, seg_pos0, block_tables) if s == n_seg else (t[a:b] for t in (seg_start, seg_len, seg_pos0, block_tables))
+            starts, lens, pos0, bt = seg_start, seg_len, seg_pos0, block_tables
+            if s != n_seg:
+                starts, lens, pos0, bt = starts.view(-1)[a:b], lens.view(-1)[a:b], pos0.view(-1)[a:b], bt[a:b]
             first, last, long_len, tables = ints[:s], ints[s:2 * s], ints[2 * s:3 * s], ints[3 * s:3 * s + s * max_pages].view(s, max_pages)
             _check(_c.xr_kv4_long(lens.data_ptr(), pos0.data_ptr(), first.data_ptr(), last.data_ptr(), long_len.data_ptr(), tables.data_ptr(), s, max_pages, G,
                                   window, most, _stream()), "attention_kv4")
