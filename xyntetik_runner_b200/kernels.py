@@ -882,9 +882,10 @@ def kv4_read(cache: torch.Tensor, layer: int, page_size: int, block_tables: torc
 # way decides (csrc/attention_kv4.cu: a4_by_codes).
 KV4_SHORT_ROWS = 64
 _KV4_ALL_ROWS = 1 << 30
-# Bytes of rows that are read back at once (what the latent attention takes for its expanded rows, too): the portions of a step that see more go a few
-# requests at a time, one request at least.  131,072 rows of 8 kv heads of 128 elements.
-KV4_VALUES_BYTES = 1 << 29
+# Bytes of rows that are read back at once: the portions of a step that see more go a few requests at a time, one request at least.  524,288 rows of 8 kv heads of 128
+# elements.  Few portions at once leave SMs idle: 8 portions of 128 tokens behind 131,072 keys take 3.53 ms in one go (4.3 GB), 3.56 four at a time, 6.05 two (1 GB), 11.1
+# one by one; 4 of 512 behind 65,536 2.79 ms in one go, 2.86 two at a time.
+KV4_VALUES_BYTES = 1 << 31
 _NP_I32 = np.dtype(np.int32)
 
 
