@@ -31,7 +31,7 @@
 // peak (6.54 TB/s), and as long where the cache fits in L2, with issue slots 44 to 62 % and the integer pipe 35 to 57 % busy and the tensor cores at 19 %: what
 // is left is warps waiting for one another's results.  Around that stand what a launch costs before its first tiles are there (about 9 us
 // with all SMs' first tiles on their way at once, 5.6 with a few) and what the last round of blocks leaves idle.
-// Measured and left: four blocks an SM (64 ragged requests of 40 heads 253 us against 214: 128 registers a thread, where three leave 168 and spill 36 bytes), tiles of 32 keys at three (230), the next tile's scores
+// Measured and left: four blocks an SM (64 ragged requests of 40 heads 253 us against 214: 128 registers a thread, where three leave 168 and spill 24 bytes), tiles of 32 keys at three (230), the next tile's scores
 // interleaved with this tile's values (55 requests of 8,192 keys 119.9 against 107.8), bulk copies instead of cp.async (equal), e4m3 operands (the
 // instruction runs at 0.16 a cycle and SM), equal shares of all tiles for resident blocks (268 and a second kernel against 214).
 //
@@ -209,15 +209,20 @@ __device__ __forceinline__ A4Walk a4_walk(int first_pos, int last_pos, int windo
 // than the one it was planned for).
 __device__ __forceinline__ int a4_spans(const A4Args& a, const A4Walk& w) { return min((w.n + a.span_tiles - 1) / a.span_tiles, a.splits); }
 
-// The place of a row block in the scratch for partial sums: row blocks of all portions that are taken lie one after another.  All lanes of a warp.
-__device__ __forceinline__ int a4_place(const A4Args& a, int seg, int rb, int rows) {
-    if (a.row_blocks == 1) return seg;                               // (one a portion; none for an empty one, whose place stays free)
+// Row blocks of the portions ahead of portion `seg`, of those that are taken.  All lanes of a warp.  (Not inlined: it costs the loop over tiles no register.)
+__device__ __noinline__ int a4_blocks_ahead(const int* seg_len, int seg, int G, int most_rows, int rows) {
     int ahead = 0;
+#pragma unroll 4
     for (int s = threadIdx.x & 31; s < seg; s += 32) {
-        const long long r = (long long)a.seg_len[s] * a.G;
-        if (r > 0 && r <= a.most_rows) ahead += (int)((r + rows - 1) / rows);
+        const long long r = (long long)seg_len[s] * G;
+        if (r > 0 && r <= most_rows) ahead += (int)((r + rows - 1) / rows);
     }
-    return __reduce_add_sync(0xffffffffu, ahead) + rb;
+    return __reduce_add_sync(0xffffffffu, ahead);
+}
+// The place of a row block in the scratch for partial sums: row blocks of all portions that are taken lie one after another.  (One a portion: a place for every
+// portion, empty ones too.)
+__device__ __forceinline__ int a4_place(const A4Args& a, int seg, int rb, int rows) {
+    return a.row_blocks == 1 ? seg : a4_blocks_ahead(a.seg_len, seg, a.G, a.most_rows, rows) + rb;
 }
 
 // NG: groups of 32 elements a held head (2, 4, 8); NT: eight-row tiles a block; F32: float32 queries and outputs, in pieces (NT 1);
@@ -329,6 +334,12 @@ k_kv4_attention(A4Args a) {
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
         if (a.early && old_rows) xr_pdl_wait();
+    }
+    // (where the block's sums will lie, while its first tiles are on their way)
+    int* place_s = reinterpret_cast<int*>(smem + S::SMEM - 16);
+    if (warp == 0 && n_spans > 1 && !a.clustered) {
+        const int place = a4_place(a, seg, rb, RB);
+        if (lane == 0) *place_s = place;
     }
 
     // q.  float32: thread (row g, t) holds the elements that its words of a key hold, 8 NG t ..; k-step 2 w + half: elements 8 w + 4 half ..  bfloat16: thread
@@ -763,7 +774,7 @@ k_kv4_attention(A4Args a) {
     __syncthreads();
     size_t item = 0;
     if (n_spans > 1 && !a.clustered) {
-        const int place = a4_place(a, seg, rb, RB);
+        const int place = *place_s;
         if ((unsigned)place >= (unsigned)a.blocks) return;           // (lengths that the launch was not made for: nothing is written beyond the scratch)
         item = ((size_t)place * a.c.K + kvh) * a.splits + span;
     }
