@@ -326,3 +326,32 @@ def test_long_requests_against_quantised_pages(dtype, layers, graphs, monkeypatc
         for a, b in zip(got, plain):
             # (the same kernels, cut for other lengths at times: sums in another order)
             assert float((a - b).abs().max()) <= (1e-4 if dtype == "float32" else 0.05) * float(b.abs().max())
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_batches_that_are_filled_up(dtype, monkeypatch):
+    """Eleven requests of 1 to 300 tokens: decode steps are filled up to sixteen rows, captured and replayed; what the filling rows leave is nobody's."""
+    from xyntetik_runner_b200.engine.engine import StepEntry
+
+    def go(eng):
+        rng, out = np.random.RandomState(9), []
+        lens = [1, 300, 17, 64, 65, 128, 9, 250, 33, 2, 100]
+        for r, n in enumerate(lens):
+            out.append(eng.step([StepEntry(r, [int(t) for t in rng.randint(0, 250, n)], [n - 1])]).clone())
+        for _ in range(6):
+            out.append(eng.step([StepEntry(r, [int(rng.randint(0, 250))], [0]) for r in range(len(lens))]).clone())
+        eng.check_status()
+        return out
+    four, plain, ref = (engine("llama64", dtype, kv, graphs=graphs, requests=12, max_tokens=4096) for kv, graphs in (("int4", True), ("int4", False), ("same", False)))
+    got, unfilled = go(four), go(plain)
+    assert four.graph_replays > 0 and four._fill_ok and plain.graph_replays == 0
+    with monkeypatch.context() as m:
+        quantise_pages(ref, m)
+        want = go(ref)
+    for a, b, c in zip(got, unfilled, want):
+        assert a.shape == c.shape
+        scale = float(c.abs().max())
+        # (a value on the other side of a border between two codes: see test_engine_against_quantised_pages)
+        assert float((a - b).abs().max()) <= (0.02 if dtype == "float32" else 0.1) * scale
+        assert float((a - c).abs().max()) <= (0.02 if dtype == "float32" else 0.1) * scale
+    assert four.cached_rows(1, 0)[0].shape[0] == 306 and torch.equal(four.cached_rows(1, 0)[0], ref.cached_rows(1, 0)[0])

@@ -369,3 +369,26 @@ def test_rows_of_earlier_steps_read_ahead_of_the_kernel_before(H, K, D, P, dtype
             x[c:] = plain_kv4.quantised_rows(new[plane][:, r * T:(r + 1) * T].reshape(steps * T, K, D))
             full.append(x)
     check(outs[True][-1], q[-1], full, plain, [T] * R, np.arange(R) * T, np.array(ends) - T, H, D, dtype)
+
+
+def test_two_calls_at_once():
+    """On two streams, each with portions that are read back, spans with scratch and single tokens: the bits that each gives alone."""
+    from xyntetik_runner_b200 import kernels
+    cases = [([6000, 300, 300, 700], [1, 210, 8, 7], 32, 4, 128, 64, BF16, 0, 0, 0, 0, 0), ([5000, 400, 80], [2, 130, 1], 66, 33, 48, 24, BF16, 0, 0, 1, 0, 0)]
+    made = [attention_case(*c, seed=i) for i, c in enumerate(cases)]
+    qs = [m[1].to(DEV) for m in made]
+    alone = [torch.empty(q.shape[0], c[2] * c[4], dtype=BF16, device=DEV) for q, c in zip(qs, cases)]
+    for m, q, out in zip(made, qs, alone):
+        kernels.attention_kv4(q, out, **m[0])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    outs = [[torch.empty_like(alone[i]) for _ in range(20)] for i in (0, 1)]
+    torch.cuda.synchronize()
+    for n in range(20):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                kernels.attention_kv4(qs[i], outs[i][n], **made[i][0])
+    torch.cuda.synchronize()
+    kernels.tc_check_status(torch.device(DEV))
+    assert all(torch.equal(out, alone[i]) for i in (0, 1) for out in outs[i])
+    check_many(alone[0], made[0][1], made[0][2], cases[0][1], made[0][5], made[0][6], 32, 128, BF16)
