@@ -16,8 +16,10 @@ struct XrBias {
     int len;
 };
 
+// What a launcher hands on as keep_first: none without a window, and few enough to be rounded up to whole tiles (positions end below that).
+static inline int xr_keep(int window, int keep_first) { return window <= 0 ? 0 : keep_first < 0x7fffff00 ? keep_first : 0x7fffff00; }
 __host__ __device__ __forceinline__ int xr_kept_tiles(int keep_first, int lo, int tile) {
-    const int kept = (int)(((unsigned)keep_first + tile - 1) / tile), first = lo / tile;      // (any keep_first that is not negative)
+    const int kept = (keep_first + tile - 1) / tile, first = lo / tile;
     return kept < first ? kept : first;
 }
 // the tile at place i of a walk whose window begins with tile t_lo

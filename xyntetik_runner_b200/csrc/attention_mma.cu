@@ -135,6 +135,9 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return *reinterpret_cast<uint32_t*>(&v);
 }
 
+// The last position up to `hi` that the block table names: what lies behind it is not held, and the loader looks no page up for it.
+__device__ __forceinline__ int att_held(const AttnMmaArgs& a, int hi) { return (int)min((long long)hi, (long long)a.max_pages * a.page_size - 1); }
+
 // Gather one tile of keys AND values [ATT_TILE][HD] each into shared memory rows of HD + 8 elements.
 // Rows at positions outside [lo, hi] (but for the kept first keys) or on a page the request no longer holds are zero-filled.
 // A thread keeps one 16-byte column and walks rows, so the page of a row is looked up once for K and V.
@@ -155,7 +158,7 @@ __device__ __forceinline__ void load_kv_tile(__nv_bfloat16* kdst, __nv_bfloat16*
             int pi;
             if (a.page_shift >= 0) { pi = kp >> a.page_shift; off = kp & (a.page_size - 1); }
             else { pi = kp / a.page_size; off = kp - pi * a.page_size; }
-            page = pi < a.max_pages ? bt[pi] : -1;
+            page = bt[pi];
         }
         __nv_bfloat16* kd = kdst + r * LD;
         __nv_bfloat16* vd = vdst + r * LD;
@@ -381,7 +384,8 @@ k_attention_rows(AttnMmaArgs a, int n_seg) {
     const int lo = a.window > 0 ? max(0, pos0 + row0 / a.G - a.window + 1) : 0;       // first key any row may read
     const int t_lo = lo / ATT_TILE, t_hi = hi / ATT_TILE, kept_tiles = xr_kept_tiles(a.keep_first, lo, ATT_TILE);
     const int n_tiles = kept_tiles + t_hi - t_lo + 1;
-    load_kv_tile<HD>(kbuf, vbuf, a, bt, kvh, xr_walk_tile(0, kept_tiles, t_lo) * ATT_TILE, lo, hi);
+    const int held = att_held(a, hi);
+    load_kv_tile<HD>(kbuf, vbuf, a, bt, kvh, xr_walk_tile(0, kept_tiles, t_lo) * ATT_TILE, lo, held);
     cp_async_commit();
     __syncthreads();
     uint32_t qf[HD / 16][4];
@@ -403,7 +407,7 @@ k_attention_rows(AttnMmaArgs a, int n_seg) {
         const int cur = i & 1, t = xr_walk_tile(i, kept_tiles, t_lo);
         if (i + 1 < n_tiles) {
             load_kv_tile<HD>(kbuf + (cur ^ 1) * ATT_TILE * LD, vbuf + (cur ^ 1) * ATT_TILE * LD, a, bt, kvh,
-                             xr_walk_tile(i + 1, kept_tiles, t_lo) * ATT_TILE, lo, hi);
+                             xr_walk_tile(i + 1, kept_tiles, t_lo) * ATT_TILE, lo, held);
             cp_async_commit();
             cp_async_wait<1>();
         } else {
@@ -465,11 +469,12 @@ k_attention_keys(AttnMmaArgs a) {
     // (the kept first keys' tiles belong to the first span)
     const int t_lo = lo / ATT_TILE, t_hi = hi / ATT_TILE, kept_tiles = span == 0 ? xr_kept_tiles(a.keep_first, lo, ATT_TILE) : 0;
     const int n_tiles = kept_tiles + t_hi - t_lo + 1;
+    const int held = att_held(a, hi);
     // ring of ATT_KSTAGES tiles: the ATT_KSTAGES - 1 tiles behind the one in use are in flight
 #pragma unroll
     for (int i = 0; i < ATT_KSTAGES - 1; i++) {
         if (i < n_tiles)
-            load_kv_tile<HD>(kbuf + i * ATT_TILE * LD, vbuf + i * ATT_TILE * LD, a, bt, kvh, xr_walk_tile(i, kept_tiles, t_lo) * ATT_TILE, lo, hi);
+            load_kv_tile<HD>(kbuf + i * ATT_TILE * LD, vbuf + i * ATT_TILE * LD, a, bt, kvh, xr_walk_tile(i, kept_tiles, t_lo) * ATT_TILE, lo, held);
         cp_async_commit();
     }
     __syncthreads();
@@ -492,7 +497,7 @@ k_attention_keys(AttnMmaArgs a) {
         int nxt = (i + ATT_KSTAGES - 1) % ATT_KSTAGES;
         if (i + ATT_KSTAGES - 1 < n_tiles)
             load_kv_tile<HD>(kbuf + nxt * ATT_TILE * LD, vbuf + nxt * ATT_TILE * LD, a, bt, kvh,
-                             xr_walk_tile(i + ATT_KSTAGES - 1, kept_tiles, t_lo) * ATT_TILE, lo, hi);
+                             xr_walk_tile(i + ATT_KSTAGES - 1, kept_tiles, t_lo) * ATT_TILE, lo, held);
         cp_async_commit();
         float s[2][4];
         tile_start<2>(s, bias_a, bias_b, a.bias.len, t * ATT_TILE + warp * 16, pos_a, pos_b);
@@ -1616,7 +1621,7 @@ XR_EXPORT int xr_attention_mma(const void* q, void* out, const void* cache_k, co
     if (any_short && splits < spans) return XR_ERR_ARG;
     AttnMmaArgs a{(const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const __nv_bfloat16*)cache_k, seg_start, seg_len, seg_pos0,
                   block_tables, part_acc, part_ml, q_stride, page_stride, v_offset, H, K, H / K, max_pages, page_size, window,
-                  spans, 0, scale, -1, n_layers, layer, status, 16, sink, softcap, window > 0 ? keep_first : 0, {bias, bias_len}};
+                  spans, 0, scale, -1, n_layers, layer, status, 16, sink, softcap, xr_keep(window, keep_first), {bias, bias_len}};
     { long long rows = (long long)(max_seg_len < 1 ? 1 : max_seg_len) * a.G; a.recv_rows = rows < 16 ? (int)rows : 16; }
     a.span = att_choose_span(att_range(max_kv_len, window), (long long)n_seg * K);
     const long long room = (long long)splits * n_seg * K;

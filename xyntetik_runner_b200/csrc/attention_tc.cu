@@ -614,7 +614,7 @@ XR_EXPORT int xr_attention_tc(const void* q, void* out, const void* cache_base, 
     while ((1 << shift) < page_size) shift++;
     AttnTcArgs a{(__nv_bfloat16*)out, seg_start, seg_len, seg_pos0, block_tables, status, H, K, G, max_pages, page_size, shift,
                  window, n_layers, layer, scale * 1.4426950408889634f, n_seg, sink,
-                 softcap > 0.f ? softcap / scale : 0.f, softcap > 0.f ? scale / softcap : 0.f, window > 0 ? keep_first : 0, {bias, bias_len}, 0};
+                 softcap > 0.f ? softcap / scale : 0.f, softcap > 0.f ? scale / softcap : 0.f, xr_keep(window, keep_first), {bias, bias_len}, 0};
     constexpr int SMEM = 10 * TA_ROWS * 128 + 128 + 2 * 2 * 128 * 4, SMEM_MOST = 227 * 1024;
     int smem = SMEM;
     if (bias != nullptr) {
